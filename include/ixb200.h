@@ -392,6 +392,75 @@ int ixb_gdn_conv_step(const void *qkv_raw_device, void *conv_state_device, const
                       void *out_device, int64_t hk, int64_t hv, float eps, ixb_stream_t stream);
 
 /*
+ * A serving step over a paged KV cache: requests that come and go, each with its positions on pages of a pool.  The
+ * reference serves from one static cache row per sequence (ixrun/batching.py:88-234); these calls stand where its batched
+ * generator would hand out, write and read cache rows.  All of them are graph-capturable (lengths, tables and positions are
+ * read from device memory) and follow ixb_set_pdl.
+ *
+ * Layout: a page holds `page` positions (16, 32, 64, 128 or 256) of one request, [page][hkv][head_dim] bf16; the pages of a
+ * pool lie page_stride elements apart (a multiple of 8).  table [requests][width] (int32): entry p is the page of positions
+ * p * page .. of the request.  slot = page number * page + position % page.  free_pages [n_pages]: a stack, its entries
+ * below *n_free are the free pages.  Up to 4096 requests.
+ *
+ * ixb_page_step: q_len[r] new tokens behind the length[r] that request r has.  Takes the pages that they need from the top
+ *   of the stack, in the order of requests and positions, into the table, and writes cu_rows [requests + 1] (the first row
+ *   of every request's new tokens in the packed batch), new_length, new_n_free, and for each of the `rows` rows of the batch
+ *   slot, pos and owner (its request); rows behind the last token: slot -1, pos 0, owner -1.  new_length may be length and
+ *   new_n_free may be n_free.  status [2]: why the step does not fit (1: pages, 2: rows, 4: a table row; 0: it fits) and the
+ *   number of pages that it needs.  A step that does not fit takes nothing and is empty: cu_rows is zero.
+ * ixb_page_release: the pages of the requests with done[r] != 0 go back onto the stack, their lengths become 0.  status [2]:
+ *   4 if the stack cannot take them (nothing is done then), and their number.
+ * ixb_rope_paged: ixb_rope_kv with keys and values into slots: row i is at position pos[i] and goes to slot[i]; a row with a
+ *   slot outside the pool is left alone.  The rotated q goes to out (row pitch out_stride; may be q).  Held in fp32 from
+ *   the norm to the one rounding of the result.
+ * ixb_attn_paged: causal attention of the new tokens of all requests, keys and values already in their pages: row
+ *   cu_rows[r] + t of q [rows] (row pitch q_stride elements, heads contiguous) is token length[r] - (cu_rows[r + 1] -
+ *   cu_rows[r]) + t of request r and sees the positions up to its own.  out [rows][hq][head_dim]; rows that belong to no
+ *   request are left as they are, rows that see no position become zero.  max_q: the most new tokens that a request may
+ *   have, by which kernels are chosen (results do not need it to be true).  A page number outside the pool counts as a page
+ *   of zeros.  head_dim 64, 128 or 256; pointers 16-byte aligned.  scratch: ixb_attn_paged_scratch_bytes of the current
+ *   device, the first 4096 bytes of it zero before the first call and left zero by every call (a buffer of its own for
+ *   launches that may overlap).
+ */
+int ixb_page_step(const int32_t *q_len_device, const int32_t *length_device, int32_t *table_device, const int32_t *free_pages_device,
+                  const int32_t *n_free_device, int64_t requests, int64_t width, int64_t n_pages, int64_t page, int64_t rows,
+                  int32_t *cu_rows_device, int32_t *new_length_device, int32_t *new_n_free_device, int32_t *slot_device,
+                  int32_t *pos_device, int32_t *owner_device, int32_t *status_device, ixb_stream_t stream);
+int ixb_page_release(const uint8_t *done_device, int32_t *length_device, const int32_t *table_device, int32_t *free_pages_device,
+                     int32_t *n_free_device, int64_t requests, int64_t width, int64_t n_pages, int64_t page,
+                     int32_t *status_device, ixb_stream_t stream);
+int ixb_rope_paged(const void *q_device, const void *k_device, const void *v_device, const int32_t *pos_device, const int32_t *slot_device,
+                   void *k_pages_device, void *v_pages_device, const void *q_norm_device, const void *k_norm_device,
+                   const float *cos_device, const float *sin_device, void *out_device, int64_t rows, int64_t hq, int64_t hkv,
+                   int64_t head_dim, int64_t rot_dim, float eps, int64_t q_stride, int64_t kv_stride, int64_t out_stride,
+                   int64_t max_seq, int64_t n_pages, int64_t page, int64_t k_page_stride, int64_t v_page_stride,
+                   ixb_stream_t stream);
+size_t ixb_attn_paged_scratch_bytes(int64_t head_dim);
+int ixb_attn_paged(const void *q_device, const void *k_pages_device, const void *v_pages_device, const int32_t *table_device,
+                   const int32_t *length_device, const int32_t *cu_rows_device, void *out_device, int64_t requests, int64_t width,
+                   int64_t rows, int64_t max_q, int64_t hq, int64_t hkv, int64_t head_dim, int64_t n_pages, int64_t page,
+                   int64_t q_stride, int64_t k_page_stride, int64_t v_page_stride, float scale, void *scratch_device,
+                   size_t scratch_bytes, ixb_stream_t stream);
+/*
+ * What stands between the logits and the token (the reference's generator leaves it to HuggingFace's logits processors):
+ *   x = logits[b][v] (bf16, or fp32 with logits_f32; row pitch in elements); out [rows][vocab] fp32, may be the logits
+ *   where v is among the first n_tokens[b] entries of history row b: x > 0 ? x / repetition[b] : x * repetition[b]
+ *   with c of these behind the first n_prompt[b]:                    x - frequency[b] * c, and - presence[b] where c > 0
+ *   where bias_ids row b [n_bias] names v (the last entry that does): x + its value
+ *   where bit v of the row's mask is 0:                              -infinity
+ * each step rounded to fp32, in this order.  history, n_prompt (then 0), the three penalties, biases and mask may be NULL.  Token numbers outside
+ * the vocabulary are passed over.  mask: n_masks rows of mask_pitch 32-bit words; row b has mask mask_row[b] (none if that is
+ * outside 0 .. n_masks - 1), or mask b where mask_row is NULL.  token [rows] (int64, may be NULL): the lowest v with the
+ * largest x; a NaN counts as the largest.  vocab up to 393216, up to 1048575 tokens and 2047 biases a row.
+ */
+int ixb_logits(const void *logits_device, int logits_f32, int64_t pitch, const int32_t *history_device, int64_t hist_len, int64_t hist_pitch,
+               const int32_t *n_tokens_device, const int32_t *n_prompt_device, const float *repetition_device,
+               const float *presence_device, const float *frequency_device, const int32_t *bias_ids_device,
+               const float *bias_values_device, int64_t n_bias, const void *mask_device, int64_t n_masks, int64_t mask_pitch,
+               const int32_t *mask_row_device, float *out_device, int64_t out_pitch, int64_t *token_device, int64_t rows,
+               int64_t vocab, ixb_stream_t stream);
+
+/*
  * Fused decode + small-M GEMM on the tensor cores (tcgen05, accumulators in
  * TMEM) for 1 <= m_rows <= 64; intended for 9..64 rows (batched decode, MTP
  * verify), below that ixb_gemv is the better call.  Same result definition and

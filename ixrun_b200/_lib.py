@@ -27,6 +27,7 @@ SYMBOLS = (
     "ixb_p6_gemm_scratch_bytes", "ixb_p6_gemm", "ixb_p6_rows",
     "ixb_allreduce_bytes", "ixb_allreduce", "ixb_p6_gemv_push", "ixb_allreduce_finish", "ixb_p6_gemv_allreduce", "ixb_allreduce_spin_limit",
     "ixb_add_rmsnorm", "ixb_allreduce_finish_add_rmsnorm", "ixb_swiglu", "ixb_rope_kv", "ixb_attn_scratch_bytes", "ixb_attn_decode", "ixb_attn_decode_join", "ixb_attn_prefill", "ixb_conv_update", "ixb_gdn_step", "ixb_gdn_conv_step",
+    "ixb_page_step", "ixb_page_release", "ixb_rope_paged", "ixb_attn_paged_scratch_bytes", "ixb_attn_paged", "ixb_logits",
 )
 
 
@@ -171,6 +172,18 @@ def lib():
     L.ixb_gdn_step.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, f32, vp]
     L.ixb_gemv_static.restype = C.c_int
     L.ixb_gemv_static.argtypes = [C.POINTER(Packed), vp, vp, vp, i64, vp, vp, C.c_int, vp]
+    L.ixb_page_step.restype = C.c_int
+    L.ixb_page_step.argtypes = [vp] * 5 + [i64] * 5 + [vp] * 8
+    L.ixb_page_release.restype = C.c_int
+    L.ixb_page_release.argtypes = [vp] * 5 + [i64] * 4 + [vp] * 2
+    L.ixb_rope_paged.restype = C.c_int
+    L.ixb_rope_paged.argtypes = [vp] * 12 + [i64] * 5 + [f32] + [i64] * 8 + [vp]
+    L.ixb_attn_paged_scratch_bytes.restype = sz
+    L.ixb_attn_paged_scratch_bytes.argtypes = [i64]
+    L.ixb_attn_paged.restype = C.c_int
+    L.ixb_attn_paged.argtypes = [vp] * 7 + [i64] * 12 + [f32, vp, sz, vp]
+    L.ixb_logits.restype = C.c_int
+    L.ixb_logits.argtypes = [vp, C.c_int, i64, vp, i64, i64] + [vp] * 7 + [i64, vp, i64, i64, vp, vp, i64, vp, i64, i64, vp]
     _lib = L
     return L
 

@@ -16,7 +16,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 SO = os.path.join(HERE, "libixb200.so")
-SOURCES = ["ixb200.cu"]
+SOURCES = ["ixb200.cu", "ixb_serve.cu"]
 HEADERS = sorted(f for f in os.listdir(CSRC) if f.endswith(".cuh")) + [os.path.join("..", "..", "include", "ixb200.h")]
 
 
@@ -65,7 +65,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
             cmd = [
                 nvcc_path(), "-O3", "-std=c++17", "-lineinfo",
                 "-gencode", "arch=compute_100a,code=sm_100a",
-                "-Xcompiler", "-fPIC", "-shared",
+                "-Xcompiler", "-fPIC", "-shared", "--threads", str(len(SOURCES)),
             ] + ([f"-D{d}" for d in os.environ.get("IXB200_DEFINES", "").split()]) + [
                 "-o", tmp,
             ] + [os.path.join(CSRC, f) for f in SOURCES]

@@ -1,9 +1,7 @@
 // ixb200: C-ABI entry points and kernels of the B200 INT8-X weight path.
 // Built for sm_100a only.  See include/ixb200.h for the contract of each call.
-#include "../../include/ixb200.h"
+#include "ixb_api.cuh"
 #include <cstdlib>
-#include <cuda.h>
-#include <cudaTypedefs.h>
 #include <cuda_fp16.h>
 #include "ixb_common.cuh"
 #include "ixb_gemm_tc.cuh"
@@ -29,7 +27,7 @@ namespace ixb {
 static thread_local char g_err[512] = "";
 static std::atomic<long long> g_launches{0};
 
-static int fail(int code, const char *fmt, ...)
+int fail(int code, const char *fmt, ...)
 {
     va_list ap;
     va_start(ap, fmt);
@@ -38,14 +36,7 @@ static int fail(int code, const char *fmt, ...)
     return code;
 }
 
-#define IXB_CUDA(call)                                                                        \
-    do {                                                                                      \
-        cudaError_t e_ = (call);                                                              \
-        if (e_ != cudaSuccess)                                                                \
-            return fail(IXB_E_CUDA, "%s failed: %s", #call, cudaGetErrorString(e_));          \
-    } while (0)
-
-static int launch_check(const char *what)
+int launch_check(const char *what)
 {
     g_launches.fetch_add(1, std::memory_order_relaxed);
     cudaError_t e = cudaGetLastError();
@@ -53,7 +44,7 @@ static int launch_check(const char *what)
     return IXB_OK;
 }
 
-static int num_sms()
+int num_sms()
 {
     static int cached[64] = {0};
     int dev = 0;
@@ -64,22 +55,6 @@ static int num_sms()
         cached[dev] = n;
     }
     return cached[dev];
-}
-
-// opt-in to more than 48 KB of dynamic shared memory, once per kernel instantiation and device
-template <class K>
-static cudaError_t opt_in_smem(K kernel, bool (&done)[64], int bytes)
-{
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-    if (!done[dev]) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-        if (e != cudaSuccess) return e;
-        done[dev] = true;
-    }
-    return cudaSuccess;
 }
 
 // CTAs of a kernel without dynamic shared memory that fit an SM of the current device, looked up once per instantiation and device
@@ -1061,6 +1036,7 @@ extern "C" size_t ixb_p6_gemv_scratch_bytes(int64_t out_f, int64_t in_f, int64_t
 // ahead of it in the stream has finished: it fetches its first weight blocks and outlier entries, then waits for that
 // kernel to complete before it touches the activations, y or the scratch.
 static std::atomic<int> g_p6_pdl{0};
+bool ixb::pdl_on() { return g_p6_pdl.load() != 0; }
 
 extern "C" int ixb_set_pdl(int on) { return g_p6_pdl.exchange(on ? 1 : 0); }
 
@@ -1084,13 +1060,6 @@ static cudaError_t launch_p6(const P6 &p, const void *x, uint32_t m_rows, const 
     return cudaLaunchKernelEx(&cfg, k_p6_mma<XS, MR>, p, (const __nv_bfloat16 *)x, m_rows, (const __nv_bfloat16 *)bias, y, y_f32,
                               slots, tickets, pl.nb, pl.xstride, pl.cq, pl.cr, pl.unit, push);
 }
-
-#define IXB_GLUE(what, call)                                                                    \
-    do {                                                                                      \
-        cudaError_t e_ = (call);                                                              \
-        if (e_ != cudaSuccess) return fail(IXB_E_CUDA, "%s launch: %s", what, cudaGetErrorString(e_)); \
-        return launch_check(what);                                                            \
-    } while (0)
 
 // The form for few blocks per warp (ixb_p6_short.cuh); 0 CTAs: not for this layer.  The rule does not look at m_rows, so that a row
 // gets the same bits alone or beside others.
@@ -1324,22 +1293,6 @@ extern "C" int ixb_allreduce_finish(void *const *peer_buffers, int rank, int wor
 }
 
 // ------------------------------------------------------- per-token glue kernels
-// one launch with the programmatic-stream-serialization attribute when ixb_set_pdl is on
-template <class... KArgs, class... Args>
-static cudaError_t launch_glue_smem(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args... args)
-{
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = g_p6_pdl.load() ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
-}
 template <class... KArgs, class... Args>
 static cudaError_t launch_glue(void (*kernel)(KArgs...), dim3 grid, dim3 block, cudaStream_t st, Args... args)
 {
@@ -1762,7 +1715,7 @@ static int pr_variant_of(uint32_t m_rows)
 
 // ---- the same on tcgen05 (ixb_p6_umma.cuh)
 // cuTensorMapEncodeTiled, a function of the driver; null if there is none
-static PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder()
+PFN_cuTensorMapEncodeTiled_v12000 ixb::tensor_map_encoder()
 {
     static const PFN_cuTensorMapEncodeTiled_v12000 fn = []() -> PFN_cuTensorMapEncodeTiled_v12000 {
         void *f = nullptr;

@@ -1,0 +1,430 @@
+// Causal attention of every request's new tokens over its pages: the form for few rows (single tokens, short drafts).
+//
+//   row (t, g) of request r and KV head h: new token t < q_len[r], query head h * G + g, position length[r] - q_len[r] + t
+//   out = softmax(scale * q . K[0 .. position]) V[0 .. position]
+//
+// A request's rows of one KV head are packed, row t * G + g, sixteen to a group (the M of mma.sync), so a key is read once for all
+// of them.  Bound: HBM, every key and value once; mma.sync is used as an instruction that multiplies sixteen rows at a time, at a
+// fifth of its rate.
+//
+// Work: all (KV head, request, row group) pairs' blocks of keys (16 per warp of a CTA) in one line, cut into equal ranges, one per
+// CTA, so lengths that differ cost nothing.  A warp takes its 16 keys of every block through its own ring of cp.async stages and
+// keeps a running softmax of its own, so no barrier lies in the loop; the warps' sums meet in shared memory where a pair ends.  A
+// pair that is cut leaves its parts in the scratch, and the CTA that comes last (a ticket) joins them in the order of the keys:
+// the same bits every time.
+//
+// Precision: q K^T bf16 x bf16 in fp32; probabilities as two bf16 numbers whose sum they are to 17 bits; a slice's P V starts from
+// zero and joins the running sums by fp32 fused multiply-adds (the tensor core cuts low bits of what it adds to a large sum).
+//
+// Keys at and behind length, and those of a page number outside the pool, arrive as zeros: nothing is read there, and what lies
+// there does not matter.  A value that is not finite counts for the rows that see it and for no other: a slice that not all rows
+// see is multiplied for one token after the other if it holds such a value.
+#pragma once
+#include "ixb_common.cuh"
+
+namespace ixb {
+
+struct PagedAttn {
+    const __nv_bfloat16 *q, *k, *v;
+    __nv_bfloat16 *out;
+    const int32_t *table, *length, *cu_rows;
+    float *part;
+    uint32_t *tickets;
+    size_t k_stride, v_stride, q_stride;               // elements: page to page, row to row
+    uint32_t requests, width, n_pages, log_page, rows, hq, hkv, group;
+    uint32_t row_lo, row_hi;                           // requests with row_lo < q_len * group <= row_hi are taken
+    float scale;
+};
+
+// what a request has: the row of its first new token, new tokens, its positions in the pages, the position of the first new token
+struct PagedReq {
+    uint32_t row0, n, len;
+    int32_t pos0;
+};
+__device__ __forceinline__ PagedReq paged_req(const PagedAttn &a, uint32_t r)
+{
+    const int32_t c0 = min(max(a.cu_rows[r], 0), (int32_t)a.rows), c1 = min(max(a.cu_rows[r + 1], 0), (int32_t)a.rows), l = a.length[r];
+    PagedReq q;
+    q.row0 = (uint32_t)c0;
+    q.n = (uint32_t)max(c1 - c0, 0);
+    q.len = (uint32_t)min((unsigned long long)max(l, 0), (unsigned long long)a.width << a.log_page);
+    q.pos0 = l - (int32_t)q.n;
+    return q;
+}
+
+__device__ __forceinline__ void pa_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void pa_ldm(uint32_t (&r)[4], uint32_t addr)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void pa_ldmt(uint32_t (&r)[4], uint32_t addr)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t pa_pack(float lo, float hi)
+{
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *(const uint32_t *)&h;
+}
+// the larger magnitudes of two pairs of bf16 numbers, as bits: 0x7f80 and above is not finite
+__device__ __forceinline__ uint32_t pa_larger(uint32_t m, uint32_t x) { return __vmaxu2(m, x & 0x7fff7fffu); }
+__device__ __forceinline__ bool pa_wild(uint32_t m) { return (m & 0xffffu) >= 0x7f80u || m >= 0x7f800000u; }
+
+template <int D>
+struct PaCfg {
+    static constexpr int kWarps = D == 256 ? 4 : 8, kThreads = kWarps * 32;
+    static constexpr int kKeys = 16 * kWarps;          // of a block
+    static constexpr uint32_t kHalf = 16 * D * 2;      // K or V of a warp's slice
+    static constexpr uint32_t kStage = 2 * kHalf;
+    static constexpr int kStages = D == 64 ? 6 : 3;
+    static constexpr uint32_t kRing = kWarps * kStages * kStage;
+    static constexpr int kPitch = D + 8;               // floats of a row in the warps' sums, (maximum, denominator) at D: 8-byte stores without conflicts
+    static constexpr uint32_t kSum = kWarps * 8 * kPitch * 4;
+    static constexpr uint32_t kSmem = kRing + kSum;
+    static constexpr uint32_t kSlot = 16 * D + 32;     // floats of a part: sums [16][D], (maximum, denominator) [16]
+    static_assert(kSmem + 128 <= 227 * 1024, "fits");
+};
+constexpr uint32_t kPaMaxRequests = 4096;
+
+template <int D>
+__global__ void __launch_bounds__(PaCfg<D>::kThreads, 1)
+k_attn_paged(PagedAttn a)
+{
+    using CF = PaCfg<D>;
+    constexpr int NW = CF::kWarps, ST = CF::kStages;
+    extern __shared__ __align__(1024) unsigned char pa_smem[];
+    __shared__ uint32_t sm_warp[NW], sm_last;
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, wid = __shfl_sync(0xffffffffu, tid >> 5, 0), g = lane >> 2, t = lane & 3u;
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(pa_smem) + wid * ST * CF::kStage;
+    float *sum = (float *)(pa_smem + CF::kRing);       // [NW][8][kPitch]; before that the blocks before every request
+    uint32_t *first = (uint32_t *)sum;
+    static_assert(CF::kSum >= 4 * kPaMaxRequests, "fits");
+    const uint32_t R = a.requests, G = a.group, page = 1u << a.log_page;
+    asm volatile("griddepcontrol.launch_dependents;");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    auto key_blocks = [&](const PagedReq &q) { return max(1u, (q.len + CF::kKeys - 1) / CF::kKeys); };
+    auto mine = [&](const PagedReq &q) { return q.n * G > a.row_lo && q.n * G <= a.row_hi; };
+    auto blocks = [&](const PagedReq &q) { return mine(q) ? (q.n * G + 15u) / 16u * key_blocks(q) : 0u; };
+    // ---- the blocks before every request, of one KV head
+    const uint32_t per = (R + CF::kThreads - 1) / CF::kThreads, ra = min(R, tid * per), rb = min(R, ra + per);
+    uint32_t before = 0, total = 0;
+    {
+        uint32_t own = 0;
+        for (uint32_t r = ra; r < rb; ++r) {
+            first[r] = own;
+            own += blocks(paged_req(a, r));
+        }
+        uint32_t v = own;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const uint32_t u = __shfl_up_sync(0xffffffffu, v, d);
+            if (lane >= (uint32_t)d) v += u;
+        }
+        if (lane == 31u) sm_warp[wid] = v;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            if ((uint32_t)w < wid) before += sm_warp[w];
+            total += sm_warp[w];
+        }
+        before += v - own;
+        for (uint32_t r = ra; r < rb; ++r) first[r] += before;
+        __syncthreads();
+    }
+    const unsigned long long W = (unsigned long long)total * a.hkv;
+    const uint32_t N = (uint32_t)min((unsigned long long)gridDim.x, W), me = blockIdx.x;
+    if (me >= N) return;
+    unsigned long long x = W * me / N;
+    const unsigned long long x_end = W * (me + 1ull) / N, x_begin = x;
+    uint32_t h = (uint32_t)(x / total), off = (uint32_t)(x - (unsigned long long)h * total), r;
+    {                                                  // the request of the first block: the last one with first[r] <= off
+        uint32_t lo = 0, hi = R;
+        while (hi - lo > 1u) {
+            const uint32_t mid = (lo + hi) / 2u;
+            if (first[mid] <= off) lo = mid;
+            else hi = mid;
+        }
+        r = lo;
+        off -= first[r];
+    }
+    PagedReq rq = paged_req(a, r);
+    uint32_t kb = key_blocks(rq), rg = off / kb, b0 = off - rg * kb;           // key blocks, row group, first block
+    const float sl2 = a.scale * 1.4426950408889634f;   // scores in units of log2
+    for (;;) {
+        // ---- blocks b0 .. b1 - 1 of row group rg of request r, KV head h
+        const uint32_t b1 = (uint32_t)min((unsigned long long)kb, b0 + (x_end - x));
+        const uint32_t rows = min(16u, rq.n * G - rg * 16u);
+        const int32_t *pages = a.table + (size_t)r * a.width;
+        const __nv_bfloat16 *kh = a.k + (size_t)h * D, *vh = a.v + (size_t)h * D;
+        const size_t key_stride = (size_t)a.hkv * D;
+        int32_t page_l = -1;                           // lane l: the page of the warp's slice of block b0 + 32 i + l
+        uint32_t page_at = 0xffffffffu;
+        auto fetch = [&](uint32_t b, uint32_t slot) {
+            const uint32_t key0 = (b * NW + wid) * 16u;
+            if (b < b1) {                              // uniform
+                const uint32_t win = (b - b0) & ~31u;
+                if (win != page_at) {
+                    page_at = win;
+                    const uint32_t key_l = ((b0 + win + lane) * NW + wid) * 16u;
+                    page_l = key_l < rq.len ? pages[key_l >> a.log_page] : -1;
+                }
+                const int32_t p = __shfl_sync(0xffffffffu, page_l, (int)((b - b0) & 31u));
+                const uint32_t live = (uint32_t)p < a.n_pages && key0 < rq.len ? min(16u, rq.len - key0) : 0u;
+                const size_t row = key0 & (page - 1u);
+                const __nv_bfloat16 *ks = kh + (live ? (size_t)p * a.k_stride + row * key_stride : 0),
+                                    *vs = vh + (live ? (size_t)p * a.v_stride + row * key_stride : 0);
+                constexpr uint32_t CH = D / 8;         // 16-byte pieces of a row
+                const uint32_t dst = ring + slot * CF::kStage;
+#pragma unroll
+                for (uint32_t i = 0; i < 16 * CH / 32; ++i) {
+                    const uint32_t c = i * 32u + lane, rr = c / CH, cc = c % CH, to = rr * (D * 2) + (cc ^ (rr & 7u)) * 16u;
+                    const uint32_t bytes = rr < live ? 16u : 0u;
+                    const size_t from = rr < live ? rr * key_stride + cc * 8u : 0;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + to), "l"(ks + from), "r"(bytes) : "memory");
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + CF::kHalf + to), "l"(vs + from), "r"(bytes) : "memory");
+                }
+            }
+            cp_async_commit();
+        };
+#pragma unroll
+        for (int i = 0; i < ST; ++i) fetch(b0 + i, i);
+        // the rows as A operands: row rg * 16 + m is token (..) / G, head (..) % G
+        uint32_t qf[D / 16][4];
+        int32_t limit[2];                              // the last position that the lane's rows g and g + 8 see
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t m = rg * 16u + g + 8u * i, tok = m / G, gi = m - tok * G;
+            const bool on = g + 8u * i < rows;
+            limit[i] = on ? rq.pos0 + (int32_t)tok : -1;
+            const uint32_t *src = (const uint32_t *)(a.q + (size_t)(rq.row0 + (on ? tok : 0u)) * a.q_stride + ((size_t)h * G + (on ? gi : 0u)) * D) + t;
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+                qf[kk][i] = on ? src[kk * 8] : 0u;
+                qf[kk][i + 2] = on ? src[kk * 8 + 4] : 0u;
+            }
+        }
+        const uint32_t tok0 = rg * 16u / G, tok1 = (rg * 16u + rows - 1u) / G;         // the group's tokens
+        float o[D / 8][4], m_[2] = {-INFINITY, -INFINITY}, l_[2] = {0.f, 0.f};
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+        uint32_t slot = 0;
+        for (uint32_t b = b0; b < b1; ++b) {
+            cp_async_wait<ST - 1>();
+            __syncwarp();
+            const int32_t key0 = (int32_t)((b * NW + wid) * 16u);
+            const uint32_t sk = ring + slot * CF::kStage, sv = sk + CF::kHalf;
+            if ((uint32_t)key0 < rq.len) {             // uniform
+                float s[2][4];
+#pragma unroll
+                for (int n = 0; n < 2; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk) {
+                    uint32_t bk[4];                    // keys 0 .. 15, dimensions 16 kk .. + 15
+                    const uint32_t rr = (lane & 7u) + (lane >> 4) * 8u, cc = 2u * kk + ((lane >> 3) & 1u);
+                    pa_ldm(bk, sk + rr * (D * 2) + (cc ^ (rr & 7u)) * 16u);
+                    pa_mma(s[0], qf[kk], bk[0], bk[1]);
+                    pa_mma(s[1], qf[kk], bk[2], bk[3]);
+                }
+                float mx[2] = {-INFINITY, -INFINITY}, corr[2], base[2];
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float v = key0 + n * 8 + 2 * (int32_t)t + (i & 1) > limit[i >> 1] ? -INFINITY : s[n][i] * sl2;
+                        s[n][i] = v;
+                        mx[i >> 1] = fmaxf(mx[i >> 1], v);
+                    }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+                    mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+                    const float mn = fmaxf(m_[i], mx[i]);
+                    base[i] = mn == -INFINITY ? 0.f : mn;              // nothing so far: sums stay zero
+                    corr[i] = exp2f(m_[i] - base[i]);
+                    m_[i] = mn;
+                    l_[i] *= corr[i];
+                }
+                uint32_t ph[4], pl[4];                 // probabilities as A operands, leading and trailing bits
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float p0 = exp2f(s[n][2 * i] - base[i]), p1 = exp2f(s[n][2 * i + 1] - base[i]);
+                        l_[i] += p0 + p1;
+                        const uint32_t hi = pa_pack(p0, p1);
+                        ph[2 * n + i] = hi;
+                        pl[2 * n + i] = pa_pack(p0 - __uint_as_float(hi << 16), p1 - __uint_as_float(hi & 0xffff0000u));
+                    }
+                uint32_t big = 0;
+#pragma unroll
+                for (int d2 = 0; d2 < D / 16; ++d2) {
+                    uint32_t bv[4];
+                    const uint32_t rr = lane & 15u, cc = 2u * d2 + (lane >> 4);
+                    pa_ldm(bv, sv + rr * (D * 2) + (cc ^ (rr & 7u)) * 16u);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) big = pa_larger(big, bv[i]);
+                }
+                const bool wild = __any_sync(0xffffffffu, pa_wild(big));
+                if (!wild) {
+#pragma unroll
+                    for (int d2 = 0; d2 < D / 16; ++d2) {
+                        uint32_t bv[4];                // keys 0 .. 15, dimensions 16 d2 .. + 15
+                        const uint32_t rr = lane & 15u, cc = 2u * d2 + (lane >> 4);
+                        pa_ldmt(bv, sv + rr * (D * 2) + (cc ^ (rr & 7u)) * 16u);
+#pragma unroll
+                        for (int n = 0; n < 2; ++n) {
+                            float w[4] = {0.f, 0.f, 0.f, 0.f};
+                            pa_mma(w, pl, bv[2 * n], bv[2 * n + 1]);
+                            pa_mma(w, ph, bv[2 * n], bv[2 * n + 1]);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) o[2 * d2 + n][i] = fmaf(o[2 * d2 + n][i], corr[i >> 1], w[i]);
+                        }
+                    }
+                } else {
+                    // one token after the other, with the values that it does not see taken out, into the rows of that token
+                    for (uint32_t tok = tok0; tok <= tok1; ++tok) {
+                        const int32_t last = rq.pos0 + (int32_t)tok;
+#pragma unroll
+                        for (int d2 = 0; d2 < D / 16; ++d2) {
+                            uint32_t bv[4];
+                            const uint32_t rr = lane & 15u, cc = 2u * d2 + (lane >> 4);
+                            pa_ldmt(bv, sv + rr * (D * 2) + (cc ^ (rr & 7u)) * 16u);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {              // keys 2 t, 2 t + 1 (+ 8 for odd i)
+                                const int32_t key = key0 + 2 * (int32_t)t + 8 * (i & 1);
+                                bv[i] &= key > last ? 0u : key + 1 > last ? 0xffffu : 0xffffffffu;
+                            }
+#pragma unroll
+                            for (int n = 0; n < 2; ++n) {
+                                float w[4] = {0.f, 0.f, 0.f, 0.f};
+                                pa_mma(w, pl, bv[2 * n], bv[2 * n + 1]);
+                                float u[4] = {0.f, 0.f, 0.f, 0.f};
+                                pa_mma(u, ph, bv[2 * n], bv[2 * n + 1]);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {          // (0 * infinity in the trailing bits is no reason for a NaN)
+                                    const bool fin = fabsf(w[i]) < INFINITY;
+                                    const float add = fin ? u[i] + w[i] : u[i];
+                                    if (limit[i >> 1] == last) o[2 * d2 + n][i] = fmaf(o[2 * d2 + n][i], corr[i >> 1], add);
+                                }
+                            }
+                        }
+                    }
+                }
+            }
+            __syncwarp();                              // the stage is read
+            fetch(b + ST, slot);
+            slot = slot + 1u == (uint32_t)ST ? 0u : slot + 1u;
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            l_[i] += __shfl_xor_sync(0xffffffffu, l_[i], 1);
+            l_[i] += __shfl_xor_sync(0xffffffffu, l_[i], 2);
+        }
+        // ---- the warps' sums; whole: this is all of the pair
+        const bool whole = b0 == 0u && b1 == kb;
+        const unsigned long long x0 = x - b0;          // the pair's first block
+        float *dst = a.part + (size_t)(2u * me + (x == x_begin ? 0u : 1u)) * CF::kSlot;
+        auto out_row = [&](uint32_t m) {               // row m of the group
+            const uint32_t q = rg * 16u + m, tok = q / G;
+            return a.out + ((size_t)(rq.row0 + tok) * a.hq + h * G + (q - tok * G)) * D;
+        };
+        auto write_out = [&](uint32_t m, uint32_t d4, const float4 &v, float l) {
+            const uint32_t tok = (rg * 16u + m) / G;
+            const bool sees = rq.pos0 + (int32_t)tok >= 0 && rq.len > 0u;      // a row that sees nothing is zero
+            const float inv = sees ? 1.f / l : 0.f;
+            *(uint2 *)(out_row(m) + d4 * 4) = sees ? make_uint2(pa_pack(v.x * inv, v.y * inv), pa_pack(v.z * inv, v.w * inv)) : make_uint2(0u, 0u);
+        };
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {                  // rows 0 .. 7, rows 8 .. 15
+            if (rows <= 8u * i) break;                 // uniform
+            __syncthreads();
+            if (g + 8u * i < rows) {
+                float *to = sum + (wid * 8u + g) * CF::kPitch + 2u * t;
+#pragma unroll
+                for (int n = 0; n < D / 8; ++n) *(float2 *)(to + n * 8) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+                if (t == 0) *(float2 *)(sum + (wid * 8u + g) * CF::kPitch + D) = make_float2(m_[i], l_[i]);
+            }
+            __syncthreads();
+            for (uint32_t it = tid; it < min(8u, rows - 8u * i) * (D / 4); it += CF::kThreads) {
+                const uint32_t row = it / (D / 4), d4 = it % (D / 4);
+                float M = -INFINITY, L = 0.f;
+#pragma unroll
+                for (int w = 0; w < NW; ++w) M = fmaxf(M, sum[(w * 8u + row) * CF::kPitch + D]);
+                const float mb = M == -INFINITY ? 0.f : M;
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int w = 0; w < NW; ++w) {
+                    const float2 ml = *(const float2 *)(sum + (w * 8u + row) * CF::kPitch + D);
+                    const float f = exp2f(ml.x - mb);
+                    const float4 u = *(const float4 *)(sum + (w * 8u + row) * CF::kPitch + d4 * 4);
+                    L = fmaf(ml.y, f, L);
+                    v.x = fmaf(u.x, f, v.x); v.y = fmaf(u.y, f, v.y); v.z = fmaf(u.z, f, v.z); v.w = fmaf(u.w, f, v.w);
+                }
+                const uint32_t m = row + 8u * i;
+                if (whole) {
+                    write_out(m, d4, v, L);
+                } else {
+                    *(float4 *)(dst + m * D + d4 * 4) = v;
+                    if (d4 == 0u) *(float2 *)(dst + 16 * D + 2 * m) = make_float2(M, L);
+                }
+            }
+        }
+        if (!whole) {
+            // the CTA of block y is the last c with W c / N <= y
+            const uint32_t c0 = (uint32_t)(((x0 + 1ull) * N - 1ull) / W), c1 = (uint32_t)(((x0 + kb) * N - 1ull) / W), parts = c1 - c0 + 1u;
+            __threadfence();
+            __syncthreads();
+            // numbers whose sum is zero, so the ticket is zero again when all have come
+            if (tid == 0) {
+                const uint32_t add = me == c0 ? 1u - parts : 1u;
+                sm_last = atomicAdd(a.tickets + c0, add) + add == 0u;
+            }
+            __syncthreads();
+            if (sm_last) {
+                __threadfence();
+                auto slot_of = [&](uint32_t c) { return a.part + (size_t)(2u * c + (c == c0 && W * c0 / N != x0 ? 1u : 0u)) * CF::kSlot; };
+                for (uint32_t it = tid; it < rows * (D / 4); it += CF::kThreads) {
+                    const uint32_t m = it / (D / 4), d4 = it % (D / 4);
+                    float M = -INFINITY, L = 0.f;
+                    for (uint32_t c = c0; c <= c1; ++c) M = fmaxf(M, __ldcg((const float2 *)(slot_of(c) + 16 * D) + m).x);
+                    const float mb = M == -INFINITY ? 0.f : M;
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+                    for (uint32_t c = c0; c <= c1; ++c) {
+                        const float2 ml = __ldcg((const float2 *)(slot_of(c) + 16 * D) + m);
+                        const float4 u = __ldcg((const float4 *)(slot_of(c) + m * D) + d4);
+                        const float f = exp2f(ml.x - mb);
+                        L = fmaf(ml.y, f, L);
+                        v.x = fmaf(u.x, f, v.x); v.y = fmaf(u.y, f, v.y); v.z = fmaf(u.z, f, v.z); v.w = fmaf(u.w, f, v.w);
+                    }
+                    write_out(m, d4, v, L);
+                }
+            }
+        }
+        x += b1 - b0;
+        if (x >= x_end) break;
+        // ---- the next pair: row group, request, KV head
+        if (++rg * 16u >= rq.n * G) {
+            rg = 0;
+            do {
+                if (++r == R) {
+                    r = 0;
+                    ++h;
+                }
+                rq = paged_req(a, r);
+            } while (!mine(rq) && h < a.hkv);          // (there is one, unless the lengths change under the kernel)
+            if (h >= a.hkv) break;
+            kb = key_blocks(rq);
+        }
+        b0 = 0;
+    }
+    cp_async_wait<0>();
+}
+
+}  // namespace ixb

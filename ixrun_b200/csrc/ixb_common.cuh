@@ -405,7 +405,7 @@ __device__ __forceinline__ void stage_chunks(uint32_t *dst, const void *base, ui
 // result.  (a0, c0) are the block's rank-table entries, (a1, c1) those of the
 // next block (ignored for the last block, whose slices run to the stream end).
 // General version: every slice is copied by a loop over the whole warp.
-__device__ __noinline__ SlotSrc stage_block_any(const Streams &s, uint32_t b, bool last, uint32_t a0, uint32_t c0,
+static __device__ __noinline__ SlotSrc stage_block_any(const Streams &s, uint32_t b, bool last, uint32_t a0, uint32_t c0,
                                                 uint32_t a1, uint32_t c1, uint32_t *slot, int lane)
 {
     SlotSrc src;

@@ -1,0 +1,198 @@
+// C-ABI entry points of a serving step over a paged KV cache: page tables, rotary embedding and write, attention, rules on logits.
+// See include/ixb200.h for the contract of each call.
+#include "ixb_api.cuh"
+#include "ixb_attn_paged.cuh"
+#include "ixb_logits.cuh"
+#include "ixb_paged.cuh"
+
+#include <algorithm>
+
+using namespace ixb;
+
+// a page holds 16, 32, ... 256 positions; 0: something else
+static uint32_t log_page(int64_t page)
+{
+    for (uint32_t l = 4; l <= 8; ++l)
+        if (page == 1ll << l) return l;
+    return 0;
+}
+
+static int page_shape(int64_t requests, int64_t width, int64_t n_pages, int64_t page)
+{
+    if (requests <= 0 || requests > kPageMaxRequests) return fail(IXB_E_UNSUPPORTED, "%lld requests: 1..%d", (long long)requests, kPageMaxRequests);
+    if (!log_page(page)) return fail(IXB_E_UNSUPPORTED, "pages of %lld positions: 16, 32, 64, 128 or 256", (long long)page);
+    if (width <= 0 || n_pages <= 0 || n_pages > 0x7fffffffll / page || width > 0x7fffffffll / page) return fail(IXB_E_ARG, "bad shape");
+    return IXB_OK;
+}
+
+extern "C" int ixb_page_step(const int32_t *q_len, const int32_t *length, int32_t *table, const int32_t *free_pages, const int32_t *n_free,
+                             int64_t requests, int64_t width, int64_t n_pages, int64_t page, int64_t rows, int32_t *cu_rows, int32_t *new_length,
+                             int32_t *new_n_free, int32_t *slot, int32_t *pos, int32_t *owner, int32_t *status, ixb_stream_t stream)
+{
+    if (!q_len || !length || !table || !free_pages || !n_free || !cu_rows || !new_length || !new_n_free || !status) return fail(IXB_E_ARG, "NULL pointer argument");
+    if (rows < 0 || rows > 0x7fffffffll || (rows && (!slot || !pos || !owner))) return fail(IXB_E_ARG, "bad rows");
+    const int rc = page_shape(requests, width, n_pages, page);
+    if (rc) return rc;
+    const PageStep s = {q_len, length, free_pages, n_free, table, cu_rows, new_length, new_n_free, slot, pos, owner, status, (uint32_t)requests,
+                        (uint32_t)width, (uint32_t)n_pages, log_page(page), (uint32_t)rows};
+    static bool attr_set[64] = {false};
+    IXB_CUDA(opt_in_smem(k_page_step, attr_set, 3 * (kPageMaxRequests + 1) * 4));
+    cudaLaunchConfig_t cfg = {};
+    // two rows a thread, and one CTA as long as that takes no longer
+    cfg.gridDim = dim3((unsigned)std::min<int64_t>(kPageMaxCtas, std::max<int64_t>(1, (rows + 2 * kPageThreads - 1) / (2 * kPageThreads))));
+    cfg.blockDim = dim3(kPageThreads);
+    cfg.dynamicSmemBytes = 3 * ((size_t)requests + 1) * 4;
+    cfg.stream = (cudaStream_t)stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cfg.gridDim.x;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_on() ? 2 : 1;
+    IXB_GLUE("k_page_step", cudaLaunchKernelEx(&cfg, k_page_step, s));
+}
+
+extern "C" int ixb_page_release(const uint8_t *done, int32_t *length, const int32_t *table, int32_t *free_pages, int32_t *n_free, int64_t requests,
+                                int64_t width, int64_t n_pages, int64_t page, int32_t *status, ixb_stream_t stream)
+{
+    if (!done || !length || !table || !free_pages || !n_free || !status) return fail(IXB_E_ARG, "NULL pointer argument");
+    const int rc = page_shape(requests, width, n_pages, page);
+    if (rc) return rc;
+    const PageRelease s = {done, table, length, free_pages, n_free, status, (uint32_t)requests, (uint32_t)width, (uint32_t)n_pages, log_page(page)};
+    IXB_GLUE("k_page_release", launch_glue_smem(k_page_release, dim3(1), dim3(kPageThreads), ((size_t)requests + 1) * 4, (cudaStream_t)stream, s));
+}
+
+extern "C" int ixb_rope_paged(const void *q, const void *k, const void *v, const int32_t *pos, const int32_t *slot, void *k_pages, void *v_pages,
+                              const void *q_norm, const void *k_norm, const float *cos_tab, const float *sin_tab, void *out, int64_t rows,
+                              int64_t hq, int64_t hkv, int64_t head_dim, int64_t rot_dim, float eps, int64_t q_stride, int64_t kv_stride,
+                              int64_t out_stride, int64_t max_seq, int64_t n_pages, int64_t page, int64_t k_page_stride, int64_t v_page_stride,
+                              ixb_stream_t stream)
+{
+    if (!q || !k || !v || !pos || !slot || !k_pages || !v_pages || !cos_tab || !sin_tab || !out) return fail(IXB_E_ARG, "NULL pointer argument");
+    if (rows <= 0 || rows > 0x7fffffffll || hq <= 0 || hkv <= 0 || hq > 65535 || hkv > 65535 || max_seq <= 0 || max_seq > 0x7fffffffll) return fail(IXB_E_ARG, "bad shape");
+    if (head_dim != 64 && head_dim != 128 && head_dim != 256) return fail(IXB_E_UNSUPPORTED, "head_dim=%lld: 64, 128 or 256", (long long)head_dim);
+    if (rot_dim <= 0 || rot_dim > head_dim || (rot_dim & 1)) return fail(IXB_E_ARG, "rot_dim must be even and at most head_dim");
+    const int rc = page_shape(1, 1, n_pages, page);
+    if (rc) return rc;
+    if (q_stride < hq * head_dim || kv_stride < hkv * head_dim || out_stride < hq * head_dim || k_page_stride < page * hkv * head_dim ||
+        v_page_stride < page * hkv * head_dim)
+        return fail(IXB_E_ARG, "bad strides");
+    const RopePaged s = {(const __nv_bfloat16 *)q, (const __nv_bfloat16 *)k, (const __nv_bfloat16 *)v, (__nv_bfloat16 *)out, (__nv_bfloat16 *)k_pages,
+                         (__nv_bfloat16 *)v_pages, pos, slot, (const __nv_bfloat16 *)q_norm, (const __nv_bfloat16 *)k_norm, cos_tab, sin_tab,
+                         (uint32_t)hq, (uint32_t)hkv, (uint32_t)rot_dim, (uint32_t)max_seq, log_page(page), eps, (size_t)q_stride, (size_t)kv_stride,
+                         (size_t)out_stride, (size_t)k_page_stride, (size_t)v_page_stride, (size_t)(n_pages * page)};
+    const uintptr_t all = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)out | (uintptr_t)q_norm |
+                          (uintptr_t)k_norm | (uintptr_t)cos_tab | (uintptr_t)sin_tab;
+    const cudaStream_t st = (cudaStream_t)stream;
+    // pieces of eight elements: rotated ones fill whole threads, and everything lies on 16 bytes
+    if (rot_dim % 16 == 0 && (all & 15u) == 0 && ((q_stride | kv_stride | out_stride | k_page_stride | v_page_stride) & 7) == 0) {
+        IXB_GLUE("k_rope_paged", head_dim == 64    ? launch_glue_smem(k_rope_paged<64>, dim3((unsigned)rows), dim3(128), 0, st, s)
+                                 : head_dim == 128 ? launch_glue_smem(k_rope_paged<128>, dim3((unsigned)rows), dim3(128), 0, st, s)
+                                                   : launch_glue_smem(k_rope_paged<256>, dim3((unsigned)rows), dim3(128), 0, st, s));
+    }
+    IXB_GLUE("k_rope_paged_any", launch_glue_smem(k_rope_paged_any, dim3((unsigned)rows), dim3(128), 0, st, s, (uint32_t)head_dim));
+}
+
+// ------------------------------------------------------------------------------------------------ attention over pages
+template <int D>
+static size_t pa_part_bytes(int ctas) { return (size_t)ctas * 2 * PaCfg<D>::kSlot * 4; }
+static size_t attn_parts(int64_t head_dim)
+{
+    return head_dim == 64 ? pa_part_bytes<64>(num_sms()) : head_dim == 128 ? pa_part_bytes<128>(num_sms()) : pa_part_bytes<256>(num_sms());
+}
+constexpr size_t kPaTicketBytes = 4096;                // a word per CTA; zero between launches
+
+extern "C" size_t ixb_attn_paged_scratch_bytes(int64_t head_dim)
+{
+    if (head_dim != 64 && head_dim != 128 && head_dim != 256) return 0;
+    return kPaTicketBytes + attn_parts(head_dim);
+}
+
+template <int D>
+static cudaError_t launch_attn_paged(const PagedAttn &a, cudaStream_t st)
+{
+    static bool attr_set[64] = {false};
+    const cudaError_t e = opt_in_smem(k_attn_paged<D>, attr_set, (int)PaCfg<D>::kSmem);
+    if (e != cudaSuccess) return e;
+    return launch_glue_smem(k_attn_paged<D>, dim3((unsigned)num_sms()), dim3(PaCfg<D>::kThreads), PaCfg<D>::kSmem, st, a);
+}
+
+extern "C" int ixb_attn_paged(const void *q, const void *k_pages, const void *v_pages, const int32_t *table, const int32_t *length,
+                              const int32_t *cu_rows, void *out, int64_t requests, int64_t width, int64_t rows, int64_t max_q, int64_t hq,
+                              int64_t hkv, int64_t head_dim, int64_t n_pages, int64_t page, int64_t q_stride, int64_t k_page_stride,
+                              int64_t v_page_stride, float scale, void *scratch, size_t scratch_bytes, ixb_stream_t stream)
+{
+    if (!q || !k_pages || !v_pages || !table || !length || !cu_rows || !out || !scratch) return fail(IXB_E_ARG, "NULL pointer argument");
+    int rc = page_shape(requests, width, n_pages, page);
+    if (rc) return rc;
+    if (hq <= 0 || hkv <= 0 || hkv > 65535 || hq % hkv) return fail(IXB_E_ARG, "query heads must be a multiple of KV heads");
+    if (head_dim != 64 && head_dim != 128 && head_dim != 256) return fail(IXB_E_UNSUPPORTED, "head_dim=%lld: 64, 128 or 256", (long long)head_dim);
+    if (rows <= 0 || rows > 0x7fffffffll / hq || max_q <= 0) return fail(IXB_E_ARG, "bad rows");
+    if (q_stride < hq * head_dim || (q_stride & 7) || k_page_stride < page * hkv * head_dim || v_page_stride < page * hkv * head_dim ||
+        ((k_page_stride | v_page_stride) & 7))
+        return fail(IXB_E_ARG, "bad strides");
+    if (((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)out | (uintptr_t)scratch) & 15u)
+        return fail(IXB_E_ARG, "q, pages, output or scratch are not 16-byte aligned");
+    if (scratch_bytes < ixb_attn_paged_scratch_bytes(head_dim)) return fail(IXB_E_SCRATCH, "attention scratch too small");
+    PagedAttn a = {};
+    a.q = (const __nv_bfloat16 *)q;
+    a.k = (const __nv_bfloat16 *)k_pages;
+    a.v = (const __nv_bfloat16 *)v_pages;
+    a.out = (__nv_bfloat16 *)out;
+    a.table = table;
+    a.length = length;
+    a.cu_rows = cu_rows;
+    a.tickets = (uint32_t *)scratch;
+    a.part = (float *)((unsigned char *)scratch + kPaTicketBytes);
+    a.k_stride = (size_t)k_page_stride;
+    a.v_stride = (size_t)v_page_stride;
+    a.q_stride = (size_t)q_stride;
+    a.requests = (uint32_t)requests;
+    a.width = (uint32_t)width;
+    a.n_pages = (uint32_t)n_pages;
+    a.log_page = log_page(page);
+    a.rows = (uint32_t)rows;
+    a.hq = (uint32_t)hq;
+    a.hkv = (uint32_t)hkv;
+    a.group = (uint32_t)(hq / hkv);
+    a.row_lo = 0;
+    a.row_hi = 0xffffffffu;
+    a.scale = scale;
+    const cudaStream_t st = (cudaStream_t)stream;
+    IXB_GLUE("k_attn_paged", head_dim == 64 ? launch_attn_paged<64>(a, st) : head_dim == 128 ? launch_attn_paged<128>(a, st) : launch_attn_paged<256>(a, st));
+}
+
+// ------------------------------------------------------------------------------------------------ rules on logits
+template <bool F32, bool VEC>
+static cudaError_t launch_logits(const LogitRules &s, cudaStream_t st)
+{
+    static bool attr_set[64] = {false};
+    const cudaError_t e = opt_in_smem(k_logits<F32, VEC>, attr_set, (int)kLgMaxBins * 4);
+    if (e != cudaSuccess) return e;
+    return launch_glue_smem(k_logits<F32, VEC>, dim3(s.rows * kLgCtas), dim3(kLgThreads), s.history || s.n_bias ? (size_t)s.slice * 4 : 0, st, s);
+}
+
+extern "C" int ixb_logits(const void *logits, int logits_f32, int64_t pitch, const int32_t *history, int64_t hist_len, int64_t hist_pitch,
+                          const int32_t *n_tokens, const int32_t *n_prompt, const float *repetition, const float *presence, const float *frequency,
+                          const int32_t *bias_ids, const float *bias_values, int64_t n_bias, const void *mask, int64_t n_masks, int64_t mask_pitch,
+                          const int32_t *mask_row, float *out, int64_t out_pitch, int64_t *token, int64_t rows, int64_t vocab, ixb_stream_t stream)
+{
+    if (!logits || !out || (history && !n_tokens) || (n_bias && (!bias_ids || !bias_values))) return fail(IXB_E_ARG, "NULL pointer argument");
+    if (rows <= 0 || rows > 0x7fffffffll / kLgCtas || vocab <= 0) return fail(IXB_E_ARG, "bad shape");
+    if (vocab > (int64_t)kLgMaxBins * kLgCtas) return fail(IXB_E_UNSUPPORTED, "vocabulary of %lld: at most %lld", (long long)vocab, (long long)kLgMaxBins * kLgCtas);
+    if (pitch < vocab || out_pitch < vocab || (history && (hist_len < 0 || hist_pitch < hist_len)) || (mask && (n_masks <= 0 || mask_pitch < (vocab + 31) / 32)))
+        return fail(IXB_E_ARG, "bad pitch");
+    if (hist_len > kLgMaxTokens || hist_pitch > 0x7fffffffll || n_bias < 0 || n_bias > kLgMaxBias || n_masks > 0x7fffffffll || mask_pitch > 0x7fffffffll)
+        return fail(IXB_E_UNSUPPORTED, "at most %lld tokens and %lld biases a row", (long long)kLgMaxTokens, (long long)kLgMaxBias);
+    LogitRules s = {logits, history, n_tokens, n_prompt, repetition, presence, frequency, bias_ids, bias_values, (const uint32_t *)mask, mask_row,
+                    out, (long long *)token, (size_t)pitch, (size_t)out_pitch, (uint32_t)rows, (uint32_t)vocab, 0, (uint32_t)hist_len,
+                    (uint32_t)hist_pitch, (uint32_t)n_bias, (uint32_t)((vocab + 31) / 32), (uint32_t)mask_pitch, (uint32_t)n_masks};
+    s.slice = (uint32_t)((vocab + 32 * kLgCtas - 1) / (32 * kLgCtas) * 32);
+    if (s.slice > kLgMaxBins) return fail(IXB_E_UNSUPPORTED, "vocabulary of %lld is too large", (long long)vocab);
+    const cudaStream_t st = (cudaStream_t)stream;
+    const bool vec = (((uintptr_t)logits | (uintptr_t)out) & 15u) == 0 && (rows == 1 || ((pitch & (logits_f32 ? 3 : 7)) == 0 && (out_pitch & 3) == 0));
+    IXB_GLUE("k_logits", logits_f32 ? (vec ? launch_logits<true, true>(s, st) : launch_logits<true, false>(s, st))
+                                    : (vec ? launch_logits<false, true>(s, st) : launch_logits<false, false>(s, st)));
+}

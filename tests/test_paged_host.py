@@ -1,0 +1,86 @@
+"""Argument checks of the paged-cache and logits entry points, on the CPU: they come before any CUDA call."""
+import ctypes
+
+import pytest
+import torch
+
+P = 4096                                               # a pointer that no call gets as far as to use
+
+
+def call(name, **changed):
+    from ixrun_b200 import _lib
+
+    args = dict(ARGS[name])
+    assert set(changed) <= set(args), changed
+    args.update(changed)
+    rc = getattr(_lib.lib(), name)(*args.values())
+    return rc, _lib.lib().ixb_last_error().decode()
+
+
+ARGS = {
+    "ixb_page_step": dict(q_len=P, length=P, table=P, free=P, n_free=P, requests=2, width=3, n_pages=4, page=16, rows=5, cu_rows=P, new_length=P,
+                          new_n_free=P, slot=P, pos=P, owner=P, status=P, stream=None),
+    "ixb_page_release": dict(done=P, length=P, table=P, free=P, n_free=P, requests=2, width=3, n_pages=4, page=16, status=P, stream=None),
+    "ixb_rope_paged": dict(q=P, k=P, v=P, pos=P, slot=P, k_pages=P, v_pages=P, q_norm=None, k_norm=None, cos=P, sin=P, out=P, rows=3, hq=4, hkv=2,
+                           head_dim=64, rot_dim=64, eps=1e-6, q_stride=256, kv_stride=128, out_stride=256, max_seq=9, n_pages=4, page=16,
+                           k_page_stride=2048, v_page_stride=2048, stream=None),
+    "ixb_attn_paged": dict(q=P, k_pages=P, v_pages=P, table=P, length=P, cu_rows=P, out=P, requests=2, width=3, rows=5, max_q=5, hq=4, hkv=2, head_dim=64,
+                           n_pages=4, page=16, q_stride=256, k_page_stride=2048, v_page_stride=2048, scale=0.1, scratch=P, scratch_bytes=1 << 40,
+                           stream=None),
+    "ixb_logits": dict(logits=P, f32=0, pitch=64, history=P, hist_len=7, hist_pitch=7, n_tokens=P, n_prompt=P, repetition=None, presence=None, frequency=None,
+                       bias_ids=None, bias_values=None, n_bias=0, mask=None, n_masks=0, mask_pitch=0, mask_row=None, out=P, out_pitch=64, token=P, rows=1,
+                       vocab=64, stream=None),
+}
+BAD = [
+    ("ixb_page_step", dict(q_len=None), 1), ("ixb_page_step", dict(status=None), 1), ("ixb_page_step", dict(requests=0), 2),
+    ("ixb_page_step", dict(requests=4097), 2), ("ixb_page_step", dict(page=24), 2), ("ixb_page_step", dict(page=512), 2), ("ixb_page_step", dict(rows=-1), 1),
+    ("ixb_page_step", dict(slot=None), 1), ("ixb_page_step", dict(n_pages=1 << 28), 1), ("ixb_page_step", dict(width=0), 1),
+    ("ixb_page_release", dict(done=None), 1), ("ixb_page_release", dict(page=0), 2), ("ixb_page_release", dict(n_pages=0), 1),
+    ("ixb_rope_paged", dict(slot=None), 1), ("ixb_rope_paged", dict(head_dim=96), 2), ("ixb_rope_paged", dict(rot_dim=66), 1),
+    ("ixb_rope_paged", dict(rot_dim=33), 1), ("ixb_rope_paged", dict(q_stride=255), 1), ("ixb_rope_paged", dict(kv_stride=64), 1),
+    ("ixb_rope_paged", dict(v_page_stride=2040), 1), ("ixb_rope_paged", dict(rows=0), 1), ("ixb_rope_paged", dict(page=17), 2),
+    ("ixb_attn_paged", dict(scratch=None), 1), ("ixb_attn_paged", dict(hq=5), 1), ("ixb_attn_paged", dict(head_dim=80), 2), ("ixb_attn_paged", dict(rows=0), 1),
+    ("ixb_attn_paged", dict(max_q=0), 1), ("ixb_attn_paged", dict(q_stride=260), 1), ("ixb_attn_paged", dict(k_page_stride=2052), 1),
+    ("ixb_attn_paged", dict(q=P + 8), 1), ("ixb_attn_paged", dict(out=P + 2), 1), ("ixb_attn_paged", dict(scratch_bytes=4096), 4),
+    ("ixb_attn_paged", dict(requests=5000), 2),
+    ("ixb_logits", dict(logits=None), 1), ("ixb_logits", dict(n_tokens=None), 1), ("ixb_logits", dict(pitch=63), 1), ("ixb_logits", dict(out_pitch=63), 1),
+    ("ixb_logits", dict(vocab=393217, pitch=400000, out_pitch=400000), 2), ("ixb_logits", dict(hist_pitch=6), 1), ("ixb_logits", dict(n_bias=3), 1),
+    ("ixb_logits", dict(n_bias=2048, bias_ids=P, bias_values=P), 2), ("ixb_logits", dict(mask=P, n_masks=1, mask_pitch=1), 1),
+    ("ixb_logits", dict(hist_len=1 << 20, hist_pitch=1 << 20), 2), ("ixb_logits", dict(rows=0), 1),
+]
+
+
+@pytest.mark.parametrize("name,changed,code", BAD, ids=lambda v: str(v) if not isinstance(v, dict) else "-".join(v))
+def test_bad_arguments_are_refused_before_any_cuda_call(name, changed, code):
+    rc, text = call(name, **changed)
+    assert rc == code and text
+
+
+def test_scratch_sizes():
+    from ixrun_b200 import _lib
+
+    f = _lib.lib().ixb_attn_paged_scratch_bytes
+    assert f(96) == 0 and all(f(d) > 4096 for d in (64, 128, 256))
+
+
+def test_host_tensors_are_refused():
+    from ixrun_b200.logits import apply_rules
+    from ixrun_b200.paged import page_release, page_step
+
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
+    with pytest.raises(ValueError):
+        page_step(i(2), i(2), i(2, 3), i(4), i(1), 16, 5)
+    with pytest.raises(ValueError):
+        page_release(i(2).bool(), i(2), i(2, 3), i(4), i(1), 16)
+    with pytest.raises(ValueError):
+        apply_rules(torch.zeros(1, 64))
+
+
+def test_ctypes_arguments_match_the_names_here():
+    from ixrun_b200 import _lib
+
+    for name, args in ARGS.items():
+        types = getattr(_lib.lib(), name).argtypes
+        assert len(types) == len(args), name
+        for t, (key, value) in zip(types, args.items()):
+            assert (t in (ctypes.c_float,)) == isinstance(value, float), (name, key)
