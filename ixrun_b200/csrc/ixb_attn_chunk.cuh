@@ -1,0 +1,747 @@
+// Causal attention of every request's new tokens over its pages: the form for many rows (chunks of prompts), on tcgen05.
+// Formulas and packing of rows as in ixb_attn_paged.cuh.
+//
+//   CTA      one per SM; a range of key tiles (128 keys) out of all (KV head, request, row tile) units' in one line, equal in cost, so
+//            lengths that differ cost nothing.  A unit that is cut leaves its parts in the scratch, k_attn_chunk_join adds them up.
+//   unit     128 or 256 packed rows (128 with heads of 256) of one request and KV head
+//   step     Q K^T of 128 rows and a key tile into tensor memory (S), softmax in registers (a thread is a row), the probabilities as
+//            bf16 over S in tensor memory, P V into the accumulator there.  Two steps are in flight in two slots: the two row tiles
+//            of a unit; or, with one row tile, even and odd key tiles (each with an accumulator and a softmax of its own; heads of 256
+//            leave room for one accumulator, there they share it).
+//   warps    0 .. 3, 4 .. 7  softmax of the two slots (heads of 256: 0 .. 3); they also bring Q and write the results
+//            then            one that issues the MMAs, one that asks for K and V (TMA, a box per page and 64 dimensions, 128-byte
+//                            swizzle), in a ring of [128 keys][128 dimensions] (64 with heads of 64)
+//
+// The accumulator is rescaled only when a row's maximum has grown by more than 2^8 (a running maximum that lags changes no ratio).
+// Precision: scores and sums fp32, probabilities bf16 for P V (half a step 2^-9 of each, as the result's own rounding; the tensor
+// core takes no wider operand beside bf16 values), their sum from the fp32 values.
+//
+// Keys that no row of the unit sees are not read; the rows of V behind the last key are zeroed up to a multiple of 16 and not
+// multiplied beyond.  A value that is not finite counts for the rows that see it and for no other: where a key tile is not
+// seen by all rows, the softmax warps look for such values and take the tile's P V themselves if there is one.
+//
+// Every wait on an mbarrier is bounded and counts this CTA's own copies and products; where one runs out the CTA's outputs
+// become NaN, and it carries on to its end with nothing in flight and tensor memory released.
+#pragma once
+#include "ixb_attn_paged.cuh"
+#include <cuda.h>
+
+namespace ixb {
+
+constexpr uint32_t kPcWaitLimit = 1u << 15, kPcWaitNs = 20000;     // polls, each of at most so many nanoseconds
+constexpr uint32_t kPcKeys = 128;
+constexpr uint32_t kPcMinCost = 4;                     // key tiles of a CTA at least
+
+template <int D>
+struct PcCfg {
+    static constexpr int kTiles = D == 256 ? 1 : 2;    // row tiles of a unit at most
+    static constexpr int kGroups = kTiles;             // of softmax warps
+    static constexpr uint32_t kUnitRows = 128u * kTiles;
+    static constexpr int kUD = D < 128 ? D : 128;      // dimensions of a ring unit
+    static constexpr int kNU = D / kUD;                // ring units of a key tile's K or V
+    static constexpr uint32_t kPanel = kPcKeys * 128;  // 64 dimensions of 128 rows: rows of 128 bytes
+    static constexpr uint32_t kUnit = kUD / 64 * kPanel;
+    static constexpr uint32_t kQTile = D / 64 * kPanel;
+    static constexpr uint32_t kStages = D == 64 ? 8 : 5;
+    static constexpr uint32_t kRingOff = kTiles * kQTile;
+    static constexpr uint32_t kBarOff = kRingOff + kStages * kUnit;
+    static constexpr uint32_t kBars = 2 * kStages + 10;
+    static constexpr uint32_t kSmem = kBarOff + kBars * 8 + 64 + 1024;         // (stages start on 1024 bytes)
+    static constexpr int kSoftWarps = 4 * kGroups, kMmaWarp = kSoftWarps, kLoadWarp = kSoftWarps + 1, kThreads = (kSoftWarps + 2) * 32;
+    static constexpr uint32_t kPart = kUnitRows * (D + 2);                     // floats: sums [tile][D / 4][128][4], (maximum, denominator) [rows]
+    static constexpr uint32_t kO = 256;                // tensor memory: S or P of the slots at 0 and 128, accumulators from here
+    static_assert(kSmem + 1120 <= 227 * 1024 && kStages * kUnit >= 4 * (kPaMaxRequests + 1) && kUnit % 1024 == 0, "fits");
+};
+
+// a unit that was cut, under the number of the CTA that has its first key tile; parts 0: none
+struct PcCut {
+    uint32_t parts, request, tile, head, first_slot;
+};
+
+__device__ __forceinline__ bool pc_wait(uint32_t mbar, uint32_t parity)
+{
+    for (uint32_t it = 0; it < kPcWaitLimit; ++it) {
+        uint32_t done;
+        asm volatile("{\n\t.reg .pred p;\n\t"
+                     "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+                     "selp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(done) : "r"(mbar), "r"(parity), "r"(kPcWaitNs) : "memory");
+        if (done) return true;
+    }
+    return false;
+}
+__device__ __forceinline__ void pc_arrive(uint32_t mbar)
+{
+    asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.shared::cta.b64 st, [%0];\n\t}" ::"r"(mbar) : "memory");
+}
+// operand in shared memory, 128-byte swizzle, version 1.  K-major: groups of eight rows sbo bytes apart.  MN-major: 64 elements of a row
+// are one swizzled line, lbo bytes to the next 64, sbo to the next eight rows.
+__device__ __forceinline__ uint64_t pc_desc(uint32_t addr, uint32_t lbo, uint32_t sbo)
+{
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | (uint64_t)(lbo >> 4) << 16 | (uint64_t)(sbo >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+// kind::f16, bf16 x bf16 -> fp32, M = 128; b_mn: B is MN-major
+__device__ __forceinline__ constexpr uint32_t pc_idesc(uint32_t n, uint32_t b_mn) { return 1u << 4 | 1u << 7 | 1u << 10 | b_mn << 16 | (n >> 3) << 17 | (128u >> 4) << 24; }
+__device__ __forceinline__ void pc_mma_ss(uint32_t el, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc)
+{
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
+                 :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0u), "r"(el) : "memory");
+}
+__device__ __forceinline__ void pc_mma_ts(uint32_t el, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc)
+{
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}"
+                 :: "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0u), "r"(el) : "memory");
+}
+__device__ __forceinline__ void pc_commit(uint32_t el, uint32_t mbar)
+{
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(mbar), "r"(el) : "memory");
+}
+// 32 columns of this lane's row
+__device__ __forceinline__ void pc_ld32(uint32_t addr, uint32_t *r)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+                   "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+                   "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void pc_st32(uint32_t addr, const uint32_t *r)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+                 "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+                 :: "r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+                    "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+                    "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
+                    "r"(r[30]), "r"(r[31]) : "memory");
+}
+__device__ __forceinline__ void pc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void pc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// loaded registers are used behind the wait only
+__device__ __forceinline__ void pc_pin(uint32_t *r)
+{
+#pragma unroll
+    for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(r[i]));
+}
+__device__ __forceinline__ float pc_exp2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// a unit of a request: rows, keys that any of them sees, key tiles (one even if there is nothing to see: its rows become zero), cost
+struct PcUnit {
+    uint32_t rows, keys, tiles, weight;
+};
+template <int D>
+__device__ __forceinline__ PcUnit pc_unit(const PagedReq &q, uint32_t G, uint32_t tile)
+{
+    constexpr uint32_t TR = PcCfg<D>::kUnitRows;
+    PcUnit u;
+    const uint32_t all = q.n * G, m0 = tile * TR;
+    u.rows = min(TR, all - m0);
+    const int32_t last = q.pos0 + (int32_t)((m0 + u.rows - 1u) / G);
+    u.keys = last < 0 ? 0u : min((uint32_t)last + 1u, q.len);
+    u.tiles = max(1u, (u.keys + kPcKeys - 1u) / kPcKeys);
+    u.weight = u.rows > 128u ? 2u : 1u;
+    return u;
+}
+
+// the CTA's way through its units; every role walks it for itself
+template <int D>
+struct PcWalk {
+    unsigned long long x, x_end, x_begin;              // cost before the next key tile
+    uint32_t h, r, tile, kt0, kt1;                     // this segment: key tiles kt0 .. kt1 - 1 of the unit
+    PagedReq rq;
+    PcUnit u;
+    __device__ __forceinline__ static bool mine(const PagedAttn &a, const PagedReq &q) { return q.n * a.group > a.row_lo && q.n * a.group <= a.row_hi; }
+    __device__ __forceinline__ void cut()
+    {
+        const unsigned long long left = x_end - x;     // tiles whose first cost unit lies before x_end
+        kt1 = (uint32_t)min((unsigned long long)u.tiles, kt0 + (left + u.weight - 1u) / u.weight);
+    }
+    // the next segment; false: there is none
+    __device__ __forceinline__ bool next(const PagedAttn &a)
+    {
+        x += (unsigned long long)(kt1 - kt0) * u.weight;
+        if (x >= x_end) return false;
+        kt0 = 0;
+        if (++tile * PcCfg<D>::kUnitRows >= rq.n * a.group) {
+            tile = 0;
+            do {
+                if (++r == a.requests) {
+                    r = 0;
+                    ++h;
+                }
+                rq = paged_req(a, r);
+            } while (!mine(a, rq) && h < a.hkv);       // (there is one, unless the lengths change under the kernel)
+            if (h >= a.hkv) return false;
+        }
+        u = pc_unit<D>(rq, a.group, tile);
+        cut();
+        return true;
+    }
+};
+
+template <int D>
+__global__ void __launch_bounds__(PcCfg<D>::kThreads, 1)
+k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, PcCut *cuts)
+{
+    using CF = PcCfg<D>;
+    extern __shared__ __align__(16) unsigned char pc_smem_raw[];
+    unsigned char *smem = pc_smem_raw + ((1024u - ((uint32_t)__cvta_generic_to_shared(pc_smem_raw) & 1023u)) & 1023u);
+    const uint32_t s0 = (uint32_t)__cvta_generic_to_shared(smem);
+    const uint32_t tid = threadIdx.x, lane = tid & 31u;
+    const int warp = __shfl_sync(0xffffffffu, (int)(tid >> 5), 0);
+    const uint32_t ring = s0 + CF::kRingOff, full0 = s0 + CF::kBarOff, empty0 = full0 + 8u * CF::kStages, q_full = empty0 + 8u * CF::kStages,
+                   q_free = q_full + 8u, s_full0 = q_free + 8u, p_full0 = s_full0 + 16u, o_full0 = p_full0 + 16u, pv_done = o_full0 + 16u,
+                   done_bar = pv_done + 8u;
+    uint32_t *tmem_slot = (uint32_t *)(smem + CF::kBarOff + CF::kBars * 8);
+    volatile uint32_t *wild_s = tmem_slot + 1;         // [2]: the slot's P V is done by its softmax warps
+    __shared__ uint32_t sm_warp[CF::kThreads / 32];
+    __shared__ float2 sm_ml[128];
+    asm volatile("griddepcontrol.launch_dependents;");
+    if (tid == 0) {
+        auto init = [&](uint32_t bar, uint32_t n, uint32_t count) {
+            for (uint32_t i = 0; i < n; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar + 8u * i), "r"(count) : "memory");
+        };
+        init(full0, 2u * CF::kStages, 1u);
+        init(q_full, 1u, CF::kSoftWarps);
+        init(q_free, 1u, 1u);
+        init(s_full0, 2u, 1u);
+        init(p_full0, 2u, 4u);
+        init(o_full0, 2u, 1u);
+        init(pv_done, 2u, 1u);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    // ---- the cost before every request, of one KV head (over the ring, which is empty)
+    uint32_t *first = (uint32_t *)(smem + CF::kRingOff);
+    const uint32_t R = a.requests, G = a.group, me = blockIdx.x;
+    const uint32_t per = (R + CF::kThreads - 1) / CF::kThreads, ra = min(R, tid * per), rb = min(R, ra + per);
+    uint32_t total = 0;
+    {
+        uint32_t own = 0, before = 0;
+        for (uint32_t r = ra; r < rb; ++r) {
+            first[r] = own;
+            const PagedReq q = paged_req(a, r);
+            if (PcWalk<D>::mine(a, q))
+                for (uint32_t t = 0; t * CF::kUnitRows < q.n * G; ++t) {
+                    const PcUnit u = pc_unit<D>(q, G, t);
+                    own += u.tiles * u.weight;
+                }
+        }
+        uint32_t v = own;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const uint32_t w = __shfl_up_sync(0xffffffffu, v, d);
+            if (lane >= (uint32_t)d) v += w;
+        }
+        if (lane == 31u) sm_warp[warp] = v;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < CF::kThreads / 32; ++w) {
+            if (w < warp) before += sm_warp[w];
+            total += sm_warp[w];
+        }
+        before += v - own;
+        for (uint32_t r = ra; r < rb; ++r) first[r] += before;
+        __syncthreads();
+    }
+    const unsigned long long W = (unsigned long long)total * a.hkv;
+    const uint32_t N = (uint32_t)min((unsigned long long)gridDim.x, (W + kPcMinCost - 1u) / kPcMinCost);
+    if (me >= N) {
+        if (tid == 0) cuts[me].parts = 0u;
+        return;
+    }
+    PcWalk<D> w;
+    w.x = w.x_begin = W * me / N;
+    w.x_end = W * (me + 1ull) / N;
+    {
+        w.h = (uint32_t)(w.x / total);
+        uint32_t off = (uint32_t)(w.x - (unsigned long long)w.h * total), lo = 0, hi = R;
+        while (hi - lo > 1u) {                         // the last request with first[r] <= off
+            const uint32_t mid = (lo + hi) / 2u;
+            if (first[mid] <= off) lo = mid;
+            else hi = mid;
+        }
+        w.r = lo;
+        off -= first[lo];
+        w.rq = paged_req(a, lo);
+        w.u = pc_unit<D>(w.rq, G, 0u);
+        w.tile = 0;
+        while (off >= w.u.tiles * w.u.weight) {
+            off -= w.u.tiles * w.u.weight;
+            w.u = pc_unit<D>(w.rq, G, ++w.tile);
+        }
+        w.kt0 = (off + w.u.weight - 1u) / w.u.weight;  // a tile that began before this range is its predecessor's
+        w.x += w.kt0 * w.u.weight - off;
+        w.kt1 = w.kt0;
+        if (w.kt0 < w.u.tiles && w.x < w.x_end) w.cut();
+    }
+    // (an empty first segment: the range begins inside the last tile of a unit)
+    bool work = w.kt1 > w.kt0 || w.next(a);
+    if (warp == CF::kMmaWarp) {
+        const uint32_t slot_addr = (uint32_t)__cvta_generic_to_shared(tmem_slot);
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot_addr), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");               // (the ring held the requests' costs)
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+    bool ok = true;
+
+    if (warp == CF::kLoadWarp) {
+        // ---- K and V of every key tile, in the order K0 V0 K1 V1 ..; a box is a page's (at most 128) keys and 64 dimensions
+        const uint32_t bp = min(1u << a.log_page, kPcKeys), boxes = kPcKeys / bp * (CF::kUD / 64);
+        const uint32_t bk = lane / (CF::kUD / 64), panel = lane % (CF::kUD / 64);      // of lane < boxes: keys bk * bp .., 64 dimensions
+        uint32_t n = 0;
+        for (bool more = work; more && ok; more = w.next(a)) {
+            const int32_t *pages = a.table + (size_t)w.r * a.width;
+            auto page_of = [&](uint32_t kt) {
+                const uint32_t key = kt * kPcKeys + bk * bp;
+                return lane < boxes && kt < w.kt1 && key < w.u.keys ? pages[key >> a.log_page] : 0;
+            };
+            int32_t page = page_of(w.kt0);
+            for (uint32_t kt = w.kt0; kt < w.kt1 && ok; ++kt) {
+                const uint32_t key = kt * kPcKeys + bk * bp, row = key & ((1u << a.log_page) - 1u);
+                const bool on = lane < boxes && key < w.u.keys;
+                const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, on)) * bp * 128u;
+                const int32_t page_n = page_of(kt + 1u);
+#pragma unroll
+                for (uint32_t i = 0; i < 2u * CF::kNU; ++i, ++n) {
+                    const uint32_t st = n % CF::kStages, bar = full0 + 8u * st;
+                    ok = ok && pc_wait(empty0 + 8u * st, (n / CF::kStages & 1u) ^ 1u);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    if (lane == 0) asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(bar), "r"(bytes) : "memory");
+                    __syncwarp();
+                    if (on)
+                        asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                                     :: "r"(ring + st * CF::kUnit + panel * CF::kPanel + bk * bp * 128u), "l"(i < (uint32_t)CF::kNU ? &kmap : &vmap),
+                                        "r"((i % CF::kNU) * CF::kUD + panel * 64u), "r"(w.h), "r"(row), "r"(page), "r"(bar) : "memory");
+                    __syncwarp();
+                }
+                page = page_n;
+            }
+        }
+        // the copies that may still be in flight (the tensor core's warp waits for them too, unless it gave up)
+        bool landed = true;
+        for (uint32_t j = n > CF::kStages ? n - CF::kStages : 0u; j < n; ++j)
+            landed = pc_wait(full0 + 8u * (j % CF::kStages), j / CF::kStages & 1u) && landed;
+        ok = ok && landed;
+    } else if (warp == CF::kMmaWarp) {
+        uint32_t el;
+        asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(el));
+        uint32_t n0 = 0, seg = 0, p0 = 0, p1 = 0;      // before this segment: ring units, segments, steps of the two slots
+        for (bool more = work; more && ok; more = w.next(a), ++seg) {
+            const bool two = w.u.weight == 2u;         // two row tiles: a key tile is two steps
+            const uint32_t tiles = w.kt1 - w.kt0, steps = two ? 2u * tiles : tiles;
+            auto wait = [&](uint32_t bar, uint32_t parity) {
+                ok = ok && pc_wait(bar, parity);
+                ok = __all_sync(0xffffffffu, ok);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            };
+            auto unit = [&](uint32_t j, uint32_t i) { return n0 + (2u * j + i) * CF::kNU; };   // key tile j's K (i = 0) or V (1)
+            auto qk = [&](uint32_t st) {
+                const uint32_t slot = st & 1u, j = two ? st >> 1 : st, q = s0 + (two ? slot * CF::kQTile : 0u);
+                const bool last_use = !two || slot;
+#pragma unroll
+                for (int c = 0; c < CF::kNU; ++c) {
+                    const uint32_t n = unit(j, 0u) + c, rs = n % CF::kStages;
+                    wait(full0 + 8u * rs, n / CF::kStages & 1u);
+                    if (!ok) return;
+#pragma unroll
+                    for (int kk = 0; kk < CF::kUD / 16; ++kk)
+                        pc_mma_ss(el, tmem + slot * 128u, pc_desc(q + (c * (CF::kUD / 64) + kk / 4) * CF::kPanel + (kk % 4) * 32u, 16u, 1024u),
+                                  pc_desc(ring + rs * CF::kUnit + (kk / 4) * CF::kPanel + (kk % 4) * 32u, 16u, 1024u), pc_idesc(128u, 0u), (c || kk) ? 1u : 0u);
+                    if (last_use) pc_commit(el, empty0 + 8u * rs);
+                }
+                pc_commit(el, s_full0 + 8u * slot);
+                if (st + 1u == steps) pc_commit(el, q_free);
+            };
+            wait(q_full, seg & 1u);
+            if (ok) qk(0u);
+            if (ok && steps > 1u) qk(1u);
+            for (uint32_t st = 0; st < steps && ok; ++st) {
+                const uint32_t slot = st & 1u, j = two ? st >> 1 : st, kt = w.kt0 + j;
+                const bool last_use = !two || slot;
+                const uint32_t valid = w.u.keys > kt * kPcKeys ? min(kPcKeys, w.u.keys - kt * kPcKeys) : 0u;
+                wait(p_full0 + 8u * slot, ((slot ? p1 : p0) + (st >> 1)) & 1u);
+                if (!ok) break;
+                const bool wild = wild_s[slot] != 0u;
+                const uint32_t o = tmem + CF::kO + (CF::kTiles == 2 ? slot * 128u : 0u);
+                const uint32_t acc = (CF::kTiles == 2 ? st >= 2u : st >= 1u) ? 1u : 0u;
+#pragma unroll
+                for (int c = 0; c < CF::kNU; ++c) {
+                    const uint32_t n = unit(j, 1u) + c, rs = n % CF::kStages, base = ring + rs * CF::kUnit;
+                    wait(full0 + 8u * rs, n / CF::kStages & 1u);
+                    if (!ok) break;
+                    if (valid & 15u) {                 // (both steps of a tile do it: the same zeros)
+                        const uint32_t z0 = valid, z1 = (valid + 15u) & ~15u;
+                        for (uint32_t i = lane; i < (z1 - z0) * (CF::kUD / 8); i += 32u) {
+                            const uint32_t row = z0 + i / (CF::kUD / 8), p = i % (CF::kUD / 8);
+                            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(base + (p >> 3) * CF::kPanel + row * 128u + (p & 7u) * 16u), "r"(0u) : "memory");
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                    }
+                    if (!wild) {
+                        if (valid == kPcKeys) {
+#pragma unroll
+                            for (uint32_t kk = 0; kk < kPcKeys / 16u; ++kk)
+                                pc_mma_ts(el, o + c * CF::kUD, tmem + slot * 128u + kk * 8u, pc_desc(base + kk * 2048u, CF::kPanel, 1024u), pc_idesc(CF::kUD, 1u),
+                                          kk ? 1u : acc);
+                        } else {
+                            for (uint32_t kk = 0; kk * 16u < valid; ++kk)
+                                pc_mma_ts(el, o + c * CF::kUD, tmem + slot * 128u + kk * 8u, pc_desc(base + kk * 2048u, CF::kPanel, 1024u), pc_idesc(CF::kUD, 1u),
+                                          kk ? 1u : acc);
+                        }
+                    }
+                    if (last_use) pc_commit(el, empty0 + 8u * rs);
+                }
+                if (!ok) break;
+                if (CF::kTiles == 1) pc_commit(el, pv_done);
+                if (st + 1u == steps || (CF::kTiles == 2 && st + 2u == steps)) pc_commit(el, o_full0 + 8u * (CF::kTiles == 2 ? slot : 0u));
+                if (CF::kTiles == 2 && steps == 1u) pc_commit(el, o_full0 + 8u);       // (the other slot has no step)
+                if (st + 2u < steps) qk(st + 2u);
+            }
+            n0 += 2u * tiles * CF::kNU;
+            p0 += (steps + 1u) >> 1;
+            p1 += steps >> 1;
+        }
+        pc_commit(el, done_bar);
+    } else {
+        // ---- softmax: group gr of four warps has a slot (heads of 256: both); a thread is a row
+        const uint32_t gr = (uint32_t)warp >> 2, row_t = tid & 127u, lanes = ((uint32_t)warp & 3u) << 21;
+        const float sl2 = a.scale * 1.4426950408889634f;
+        uint32_t c0s = 0, c1s = 0, pv_cnt = 0, seg = 0, n0 = 0;       // before this segment: steps of the slots, of both, segments, ring units
+        uint32_t cut_parts = 0, cut_r = 0, cut_tile = 0, cut_h = 0, cut_slot = 0;
+        for (bool more = work; more; more = w.next(a), ++seg) {
+            const bool two = w.u.weight == 2u;
+            const uint32_t tiles = w.kt1 - w.kt0, steps = two ? 2u * tiles : tiles;
+            // ---- Q: rows of the unit into [tile][64 dimensions][128 rows], swizzled; rows behind the last are zero
+            if (seg) ok = ok && pc_wait(q_free, (seg - 1u) & 1u);
+            const uint32_t m0 = w.tile * CF::kUnitRows;
+            for (uint32_t i = tid; i < (two ? 256u : 128u) * (D / 8); i += CF::kSoftWarps * 32u) {
+                const uint32_t m = i / (D / 8), ch = i % (D / 8), q = m0 + m, tok = q / G;
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (m < w.u.rows) v = *(const uint4 *)(a.q + (size_t)(w.rq.row0 + tok) * a.q_stride + ((size_t)w.h * G + (q - tok * G)) * D + ch * 8u);
+                const uint32_t rr = m & 127u;
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(s0 + (m >> 7) * CF::kQTile + (ch >> 3) * CF::kPanel + rr * 128u + ((ch ^ rr) & 7u) * 16u),
+                             "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) pc_arrive(q_full);
+            // ---- this thread's row
+            const uint32_t m = (two ? gr * 128u : 0u) + row_t;                 // in the unit
+            const bool valid = m < w.u.rows;
+            const int32_t limit = valid ? w.rq.pos0 + (int32_t)((m0 + m) / G) : -1;
+            const bool warp_on = (m & ~31u) < w.u.rows;                        // (warp uniform) some row is there
+            const int32_t low_warp = w.rq.pos0 + (int32_t)((m0 + (m & ~31u)) / G), low_tile = w.rq.pos0 + (int32_t)((m0 + (m & ~127u)) / G);
+            const uint32_t o_at = tmem + lanes + CF::kO + (CF::kTiles == 2 ? gr * 128u : 0u);
+            float mb = -INFINITY, l = 0.f;             // the maximum that the sums are relative to (in units of log2), the denominator
+            bool any = false;                          // (group uniform) the accumulator holds something
+            const uint32_t stride = CF::kTiles == 2 ? 2u : 1u;
+            for (uint32_t st = CF::kTiles == 2 ? gr : 0u; st < steps; st += stride) {
+                const uint32_t slot = st & 1u, j = two ? st >> 1 : st, kt = w.kt0 + j, s_at = tmem + lanes + slot * 128u;
+                const int32_t key0 = (int32_t)(kt * kPcKeys), key_last = min(key0 + (int32_t)kPcKeys, (int32_t)w.u.keys) - 1;
+                ok = ok && pc_wait(s_full0 + 8u * slot, ((slot ? c1s : c0s) + (st >> 1)) & 1u);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                bool wild = false;
+                if (key_last > low_tile) {             // (group uniform) not every row sees every key: is there a value that is not finite?
+                    uint32_t big = 0;
+                    for (int c = 0; c < CF::kNU; ++c) {
+                        const uint32_t n = n0 + (2u * j + 1u) * CF::kNU + c, rs = n % CF::kStages;
+                        ok = ok && pc_wait(full0 + 8u * rs, n / CF::kStages & 1u);
+                        for (uint32_t i = row_t; i < (uint32_t)(key_last - key0 + 1) * (CF::kUD / 8); i += 128u) {
+                            uint4 v;
+                            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                                         : "r"(ring + rs * CF::kUnit + (i & 7u) * 16u + (i >> 3) / (CF::kUD / 64) * 128u + (i >> 3) % (CF::kUD / 64) * CF::kPanel) : "memory");
+                            big = pa_larger(pa_larger(pa_larger(pa_larger(big, v.x), v.y), v.z), v.w);
+                        }
+                    }
+                    uint32_t found;
+                    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                                 : "=r"(found) : "r"((uint32_t)pa_wild(big)), "r"(1u + gr) : "memory");
+                    wild = found != 0u;
+                }
+                if (row_t == 0) wild_s[slot] = wild;
+                ok = __all_sync(0xffffffffu, ok);
+                if (warp_on && ok) {
+                    uint32_t s[128];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) pc_ld32(s_at + 32u * c, s + 32 * c);
+                    pc_wait_ld();
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) pc_pin(s + 32 * c);
+                    if (key0 + (int32_t)kPcKeys - 1 > low_warp) {              // (warp uniform)
+#pragma unroll
+                        for (int c = 0; c < 128; ++c)
+                            if (key0 + c > limit) s[c] = 0xff800000u;
+                    }
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int c = 0; c < 128; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(s[c]));
+                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
+                    if (CF::kTiles == 1 && st) {       // the accumulator is the step before's too
+                        ok = ok && pc_wait(pv_done, (pv_cnt + st - 1u) & 1u);
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    }
+                    if (__any_sync(0xffffffffu, top > mb + 8.f)) {             // (false for -inf; the first maximum of a row is larger than -inf)
+                        const float mn = fmaxf(mb, top), f = pc_exp2(mb - (mn == -INFINITY ? 0.f : mn));
+                        mb = mn;
+                        l *= f;
+                        if (any) {
+#pragma unroll 1
+                            for (int c = 0; c < D / 32; ++c) {
+                                uint32_t o[32];
+                                pc_ld32(o_at + 32u * c, o);
+                                pc_wait_ld();
+                                pc_pin(o);
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                                pc_st32(o_at + 32u * c, o);
+                            }
+                            pc_wait_st();
+                        }
+                    }
+                    const float nb = mb == -INFINITY ? 0.f : -mb;
+                    float la[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int c = 0; c < 128; c += 2) {
+                        const float p0 = pc_exp2(fmaf(__uint_as_float(s[c]), sl2, nb)), p1 = pc_exp2(fmaf(__uint_as_float(s[c + 1]), sl2, nb));
+                        la[c >> 1 & 3] += p0 + p1;
+                        s[c / 2] = pa_pack(p0, p1);
+                    }
+                    l += (la[0] + la[1]) + (la[2] + la[3]);
+                    pc_st32(s_at, s);
+                    pc_st32(s_at + 32u, s + 32);
+                    pc_wait_st();
+                    if (wild) {
+                        // P V of this tile for this thread's row: what the row does not see is left out
+#pragma unroll 1
+                        for (int c = 0; c < D / 32; ++c) {
+                            uint32_t o[32];
+                            if (any) {
+                                pc_ld32(o_at + 32u * c, o);
+                                pc_wait_ld();
+                                pc_pin(o);
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) o[i] = 0u;
+                            }
+                            const uint32_t n = n0 + (2u * j + 1u) * CF::kNU + c / (CF::kUD / 32), rs = n % CF::kStages, cc = c % (CF::kUD / 32);
+                            const uint32_t vb = ring + rs * CF::kUnit + (cc >> 1) * CF::kPanel;
+#pragma unroll 1
+                            for (uint32_t k = 0; k < kPcKeys; ++k) {
+                                uint32_t pp;
+                                asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(pp) : "r"(s_at + k / 2u) : "memory");
+                                pc_wait_ld();
+                                asm volatile("" : "+r"(pp));
+                                const float p = __uint_as_float(k & 1u ? pp & 0xffff0000u : pp << 16);
+                                if (key0 + (int32_t)k <= limit) {
+#pragma unroll
+                                    for (uint32_t q = 0; q < 4u; ++q) {
+                                        uint32_t v[4];
+                                        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                                                     : "r"(vb + k * 128u + ((((cc & 1u) * 4u + q) ^ k) & 7u) * 16u) : "memory");
+#pragma unroll
+                                        for (int e = 0; e < 4; ++e) {
+                                            o[8 * q + 2 * e] = __float_as_uint(fmaf(p, __uint_as_float(v[e] << 16), __uint_as_float(o[8 * q + 2 * e])));
+                                            o[8 * q + 2 * e + 1] = __float_as_uint(fmaf(p, __uint_as_float(v[e] & 0xffff0000u), __uint_as_float(o[8 * q + 2 * e + 1])));
+                                        }
+                                    }
+                                }
+                                __syncwarp();
+                            }
+                            pc_st32(o_at + 32u * c, o);
+                        }
+                        pc_wait_st();
+                    }
+                } else if (CF::kTiles == 1 && st) {    // (keeps up with the barrier's phases)
+                    ok = ok && pc_wait(pv_done, (pv_cnt + st - 1u) & 1u);
+                }
+                any = true;
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) pc_arrive(p_full0 + 8u * slot);
+            }
+            pv_cnt += steps;
+            c0s += (steps + 1u) >> 1;
+            c1s += steps >> 1;
+            n0 += 2u * tiles * CF::kNU;
+            // ---- the unit's sums
+            ok = ok && pc_wait(o_full0 + 8u * gr, seg & 1u);
+            if (CF::kTiles == 1) ok = ok && pc_wait(pv_done, (pv_cnt - 1u) & 1u);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (!ok) l = __int_as_float(0x7fc00000);
+            const bool whole = w.kt0 == 0u && w.kt1 == w.u.tiles;
+            const bool sees = limit >= 0 && w.u.keys > 0u;                     // (of this row: anything at all, in any segment)
+            const unsigned long long x0 = w.x - (unsigned long long)w.kt0 * w.u.weight;
+            const uint32_t slot_n = 2u * me + (w.kt0 ? 0u : 1u);               // a unit's first part is this CTA's last segment
+            float *part = a.part + (size_t)slot_n * CF::kPart;
+            if (!whole && w.kt0 == 0u) {
+                const uint32_t c1 = (uint32_t)(((x0 + (unsigned long long)(w.u.tiles - 1u) * w.u.weight + 1ull) * N - 1ull) / W);
+                cut_parts = c1 - me + 1u;
+                cut_r = w.r;
+                cut_tile = w.tile;
+                cut_h = w.h;
+                cut_slot = slot_n;
+            }
+            const bool merge = CF::kTiles == 2 && !two;                        // both groups have a part of the same rows
+            float other_l = 0.f, f_own = 1.f, f_other = 0.f;
+            const uint32_t xbuf = s0 + CF::kQTile;                             // [columns][128 rows] floats: the second row tile's Q, unused here
+            constexpr int XC = CF::kQTile / 512 < D ? (int)(CF::kQTile / 512) : D;     // columns that fit
+            __nv_bfloat16 *dst = a.out;
+            if (valid) {
+                const uint32_t q = m0 + m, tok = q / G;
+                dst = a.out + ((size_t)(w.rq.row0 + tok) * a.hq + (size_t)w.h * G + (q - tok * G)) * D;
+            }
+            if (merge) {
+                // (Q of this unit's second tile is not there, and the next unit's is written behind this)
+                if (gr == 1u) sm_ml[row_t] = make_float2(mb, l);
+                asm volatile("barrier.cta.sync 3, 256;" ::: "memory");
+                if (gr == 0u) {
+                    const float2 o = sm_ml[row_t];
+                    const float mn = fmaxf(mb, o.x), mz = mn == -INFINITY ? 0.f : mn;
+                    f_own = pc_exp2(mb - mz);
+                    f_other = pc_exp2(o.x - mz);
+                    other_l = o.y;
+                    mb = mn;
+                    l = l * f_own + other_l * f_other;
+                    if (steps < 2u) f_other = 0.f;
+                }
+            }
+            const float inv = 1.f / l;
+#pragma unroll 1
+            for (int c0 = 0; c0 < D; c0 += merge ? XC : D) {
+                const int c1 = merge ? min(D, c0 + XC) : D;
+                if (merge) {
+                    if (gr == 1u && steps > 1u && warp_on) {
+#pragma unroll 1
+                        for (int c = c0; c < c1; c += 32) {
+                            uint32_t o[32];
+                            pc_ld32(o_at + c, o);
+                            pc_wait_ld();
+                            pc_pin(o);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) asm volatile("st.shared.u32 [%0], %1;" ::"r"(xbuf + ((c - c0 + i) * 128u + row_t) * 4u), "r"(o[i]) : "memory");
+                        }
+                    }
+                    asm volatile("barrier.cta.sync 3, 256;" ::: "memory");
+                }
+                if (warp_on && (!merge || gr == 0u)) {
+#pragma unroll 1
+                    for (int c = c0; c < c1; c += 32) {
+                        uint32_t o[32];
+                        pc_ld32(o_at + c, o);
+                        pc_wait_ld();
+                        pc_pin(o);
+                        if (merge) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) {
+                                float v = __uint_as_float(o[i]) * f_own;
+                                if (steps > 1u) {
+                                    uint32_t u;
+                                    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(u) : "r"(xbuf + ((c - c0 + i) * 128u + row_t) * 4u) : "memory");
+                                    v = fmaf(__uint_as_float(u), f_other, v);
+                                }
+                                o[i] = __float_as_uint(v);
+                            }
+                        }
+                        if (whole) {
+                            if (valid) {
+#pragma unroll
+                                for (int i = 0; i < 32; i += 8) {
+                                    uint32_t v[4];
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e)
+                                        v[e] = sees || !ok ? pa_pack(__uint_as_float(o[i + 2 * e]) * inv, __uint_as_float(o[i + 2 * e + 1]) * inv) : 0u;
+                                    *(uint4 *)(dst + c + i) = make_uint4(v[0], v[1], v[2], v[3]);
+                                }
+                            }
+                        } else if (valid) {
+#pragma unroll
+                            for (int i = 0; i < 32; i += 4)
+                                *(uint4 *)(part + (((m >> 7) * (D / 4) + (c + i) / 4) * 128u + (m & 127u)) * 4u) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                        }
+                    }
+                }
+                if (merge) asm volatile("barrier.cta.sync 3, 256;" ::: "memory");
+            }
+            if (!whole && valid && (!merge || gr == 0u)) *(float2 *)(part + CF::kUnitRows * D + 2u * m) = make_float2(mb, l);
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");   // (the accumulators are read: the next unit's may be written)
+        }
+        if (tid == 0) {
+            cuts[me].request = cut_r;
+            cuts[me].tile = cut_tile;
+            cuts[me].head = cut_h;
+            cuts[me].first_slot = cut_slot;
+            cuts[me].parts = cut_parts;
+        }
+    }
+    __syncwarp();
+    ok = pc_wait(done_bar, 0u) && ok;                  // (the MMAs that were issued are done, whoever gave up)
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == CF::kMmaWarp) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+// The parts of the units that were cut.  grid (CTAs of k_attn_chunk, row tiles x groups of 32 dimensions), a thread per row.
+template <int D>
+__global__ void __launch_bounds__(128)
+k_attn_chunk_join(PagedAttn a, const PcCut *cuts)
+{
+    using CF = PcCfg<D>;
+    asm volatile("griddepcontrol.launch_dependents;");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const PcCut cut = cuts[blockIdx.x];
+    if (cut.parts == 0u) return;
+    const PagedReq rq = paged_req(a, cut.request);
+    const PcUnit u = pc_unit<D>(rq, a.group, cut.tile);
+    const uint32_t tile = blockIdx.y / (D / 32), c0 = blockIdx.y % (D / 32) * 8u, row = threadIdx.x, m = tile * 128u + row;
+    if (m >= u.rows) return;
+    auto part = [&](uint32_t p) { return a.part + (size_t)(p ? 2u * (blockIdx.x + p) : cut.first_slot) * CF::kPart; };
+    float M = -INFINITY, L = 0.f;
+    for (uint32_t p = 0; p < cut.parts; ++p) M = fmaxf(M, ((const float2 *)(part(p) + CF::kUnitRows * D))[m].x);
+    const float mz = M == -INFINITY ? 0.f : M;
+    float4 v[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (uint32_t p = 0; p < cut.parts; ++p) {
+        const float2 ml = ((const float2 *)(part(p) + CF::kUnitRows * D))[m];
+        const float f = pc_exp2(ml.x - mz);
+        L = fmaf(ml.y, f, L);
+        const float4 *src = (const float4 *)part(p) + (size_t)(tile * (D / 4) + c0) * 128u + row;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            const float4 s = src[c * 128];
+            v[c].x = fmaf(s.x, f, v[c].x); v[c].y = fmaf(s.y, f, v[c].y); v[c].z = fmaf(s.z, f, v[c].z); v[c].w = fmaf(s.w, f, v[c].w);
+        }
+    }
+    const uint32_t q = cut.tile * CF::kUnitRows + m, tok = q / a.group;
+    const bool sees = rq.pos0 + (int32_t)tok >= 0 && u.keys > 0u;
+    const float inv = 1.f / L;
+    __nv_bfloat16 *dst = a.out + ((size_t)(rq.row0 + tok) * a.hq + (size_t)cut.head * a.group + (q - tok * a.group)) * D + c0 * 4u;
+#pragma unroll
+    for (int c = 0; c < 8; c += 2)
+        *(uint4 *)(dst + c * 4) = sees ? make_uint4(pa_pack(v[c].x * inv, v[c].y * inv), pa_pack(v[c].z * inv, v[c].w * inv),
+                                                    pa_pack(v[c + 1].x * inv, v[c + 1].y * inv), pa_pack(v[c + 1].z * inv, v[c + 1].w * inv))
+                                       : make_uint4(0u, 0u, 0u, 0u);
+}
+
+}  // namespace ixb

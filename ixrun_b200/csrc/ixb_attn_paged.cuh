@@ -98,7 +98,7 @@ k_attn_paged(PagedAttn a)
 {
     using CF = PaCfg<D>;
     constexpr int NW = CF::kWarps, ST = CF::kStages;
-    extern __shared__ __align__(1024) unsigned char pa_smem[];
+    extern __shared__ __align__(16) unsigned char pa_smem[];
     __shared__ uint32_t sm_warp[NW], sm_last;
     const uint32_t tid = threadIdx.x, lane = tid & 31u, wid = __shfl_sync(0xffffffffu, tid >> 5, 0), g = lane >> 2, t = lane & 3u;
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(pa_smem) + wid * ST * CF::kStage;

@@ -1,6 +1,7 @@
 // C-ABI entry points of a serving step over a paged KV cache: page tables, rotary embedding and write, attention, rules on logits.
 // See include/ixb200.h for the contract of each call.
 #include "ixb_api.cuh"
+#include "ixb_attn_chunk.cuh"
 #include "ixb_attn_paged.cuh"
 #include "ixb_logits.cuh"
 #include "ixb_paged.cuh"
@@ -96,27 +97,59 @@ extern "C" int ixb_rope_paged(const void *q, const void *k, const void *v, const
 }
 
 // ------------------------------------------------------------------------------------------------ attention over pages
-template <int D>
-static size_t pa_part_bytes(int ctas) { return (size_t)ctas * 2 * PaCfg<D>::kSlot * 4; }
-static size_t attn_parts(int64_t head_dim)
-{
-    return head_dim == 64 ? pa_part_bytes<64>(num_sms()) : head_dim == 128 ? pa_part_bytes<128>(num_sms()) : pa_part_bytes<256>(num_sms());
-}
-constexpr size_t kPaTicketBytes = 4096;                // a word per CTA; zero between launches
+// Requests with at most this many rows (new tokens times query heads of a KV head) go through k_attn_paged, one group of rows; the
+// others through k_attn_chunk.
+constexpr uint32_t kAttnFewRows = 16;
+constexpr size_t kPaTicketBytes = 4096, kPaCutBytes = 8192;       // a word, a PcCut per CTA; the tickets are zero between launches
 
+template <int D>
+static size_t attn_part_bytes()                        // the two kernels run one after the other
+{
+    return (size_t)num_sms() * 2 * 4 * std::max<size_t>(PaCfg<D>::kSlot, PcCfg<D>::kPart);
+}
 extern "C" size_t ixb_attn_paged_scratch_bytes(int64_t head_dim)
 {
     if (head_dim != 64 && head_dim != 128 && head_dim != 256) return 0;
-    return kPaTicketBytes + attn_parts(head_dim);
+    return kPaTicketBytes + kPaCutBytes + (head_dim == 64 ? attn_part_bytes<64>() : head_dim == 128 ? attn_part_bytes<128>() : attn_part_bytes<256>());
+}
+
+// a pool as a tensor of [pages][page][kv heads][D]: boxes of 64 dimensions of one head of (at most 128) positions of a page
+static CUresult pool_map(CUtensorMap *map, const __nv_bfloat16 *pool, size_t page_stride, const PagedAttn &a, uint32_t D)
+{
+    const uint32_t page = 1u << a.log_page;
+    const cuuint64_t dims[4] = {D, a.hkv, page, a.n_pages}, strides[3] = {D * 2ull, (cuuint64_t)a.hkv * D * 2, (cuuint64_t)page_stride * 2};
+    const cuuint32_t box[4] = {64, 1, std::min(page, kPcKeys), 1}, one[4] = {1, 1, 1, 1};
+    return tensor_map_encoder()(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<__nv_bfloat16 *>(pool), dims, strides, box, one,
+                                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
 template <int D>
-static cudaError_t launch_attn_paged(const PagedAttn &a, cudaStream_t st)
+static int attn_paged_run(PagedAttn a, PcCut *cuts, int64_t max_q, cudaStream_t st)
 {
+    const unsigned sms = (unsigned)num_sms();
+    const bool few = max_q * a.group <= kAttnFewRows, both = !few && a.requests > 1u;
+    if (few || both) {
+        if (both) a.row_hi = kAttnFewRows;
+        static bool attr_set[64] = {false};
+        IXB_CUDA(opt_in_smem(k_attn_paged<D>, attr_set, (int)PaCfg<D>::kSmem));
+        IXB_CUDA(launch_glue_smem(k_attn_paged<D>, dim3(sms), dim3(PaCfg<D>::kThreads), PaCfg<D>::kSmem, st, a));
+        const int rc = launch_check("k_attn_paged");
+        if (rc || few) return rc;
+        a.row_lo = kAttnFewRows;
+        a.row_hi = 0xffffffffu;
+    }
+    if (!tensor_map_encoder()) return fail(IXB_E_UNSUPPORTED, "the driver has no cuTensorMapEncodeTiled");
+    CUtensorMap kmap, vmap;
+    CUresult r = pool_map(&kmap, a.k, a.k_stride, a, D);
+    if (r == CUDA_SUCCESS) r = pool_map(&vmap, a.v, a.v_stride, a, D);
+    if (r != CUDA_SUCCESS) return fail(IXB_E_CUDA, "tensor map of a pool: error %d", (int)r);
     static bool attr_set[64] = {false};
-    const cudaError_t e = opt_in_smem(k_attn_paged<D>, attr_set, (int)PaCfg<D>::kSmem);
-    if (e != cudaSuccess) return e;
-    return launch_glue_smem(k_attn_paged<D>, dim3((unsigned)num_sms()), dim3(PaCfg<D>::kThreads), PaCfg<D>::kSmem, st, a);
+    IXB_CUDA(opt_in_smem(k_attn_chunk<D>, attr_set, (int)PcCfg<D>::kSmem));
+    IXB_CUDA(launch_glue_smem(k_attn_chunk<D>, dim3(sms), dim3(PcCfg<D>::kThreads), PcCfg<D>::kSmem, st, a, kmap, vmap, cuts));
+    const int rc = launch_check("k_attn_chunk");
+    if (rc) return rc;
+    IXB_GLUE("k_attn_chunk_join", launch_glue_smem(k_attn_chunk_join<D>, dim3(sms, PcCfg<D>::kTiles * (D / 32)), dim3(128), 0, st, a, (const PcCut *)cuts));
 }
 
 extern "C" int ixb_attn_paged(const void *q, const void *k_pages, const void *v_pages, const int32_t *table, const int32_t *length,
@@ -135,6 +168,8 @@ extern "C" int ixb_attn_paged(const void *q, const void *k_pages, const void *v_
         return fail(IXB_E_ARG, "bad strides");
     if (((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)out | (uintptr_t)scratch) & 15u)
         return fail(IXB_E_ARG, "q, pages, output or scratch are not 16-byte aligned");
+    if ((size_t)num_sms() * std::max(sizeof(PcCut), sizeof(uint32_t)) > kPaCutBytes || (size_t)num_sms() * 4 > kPaTicketBytes)
+        return fail(IXB_E_UNSUPPORTED, "a device of %d SMs", num_sms());
     if (scratch_bytes < ixb_attn_paged_scratch_bytes(head_dim)) return fail(IXB_E_SCRATCH, "attention scratch too small");
     PagedAttn a = {};
     a.q = (const __nv_bfloat16 *)q;
@@ -145,7 +180,7 @@ extern "C" int ixb_attn_paged(const void *q, const void *k_pages, const void *v_
     a.length = length;
     a.cu_rows = cu_rows;
     a.tickets = (uint32_t *)scratch;
-    a.part = (float *)((unsigned char *)scratch + kPaTicketBytes);
+    a.part = (float *)((unsigned char *)scratch + kPaTicketBytes + kPaCutBytes);
     a.k_stride = (size_t)k_page_stride;
     a.v_stride = (size_t)v_page_stride;
     a.q_stride = (size_t)q_stride;
@@ -160,8 +195,10 @@ extern "C" int ixb_attn_paged(const void *q, const void *k_pages, const void *v_
     a.row_lo = 0;
     a.row_hi = 0xffffffffu;
     a.scale = scale;
+    if (!(scale > 0.f && scale <= 3.4e38f)) return fail(IXB_E_ARG, "the scale must be positive and finite");
+    PcCut *cuts = (PcCut *)((unsigned char *)scratch + kPaTicketBytes);
     const cudaStream_t st = (cudaStream_t)stream;
-    IXB_GLUE("k_attn_paged", head_dim == 64 ? launch_attn_paged<64>(a, st) : head_dim == 128 ? launch_attn_paged<128>(a, st) : launch_attn_paged<256>(a, st));
+    return head_dim == 64 ? attn_paged_run<64>(a, cuts, max_q, st) : head_dim == 128 ? attn_paged_run<128>(a, cuts, max_q, st) : attn_paged_run<256>(a, cuts, max_q, st);
 }
 
 // ------------------------------------------------------------------------------------------------ rules on logits

@@ -225,6 +225,8 @@ class AttnPaged:
             raise ValueError(f"length [R], cu_rows [R+1], table [R, width] with R of 1..{MAX_REQUESTS}")
         if max_q is not None and max_q < 1:
             raise ValueError("max_q must be positive")
+        if scale is not None and not 0.0 < scale < float("inf"):
+            raise ValueError("scale must be positive")
         if out is None:
             out = torch.empty(rows, self.hq * self.d, dtype=torch.bfloat16, device=q.device)
         elif out.numel() != rows * self.hq * self.d:
