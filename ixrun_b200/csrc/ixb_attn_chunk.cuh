@@ -9,7 +9,7 @@
 //            of a unit; or, with one row tile, even and odd key tiles (each with an accumulator and a softmax of its own; heads of 256
 //            leave room for one accumulator, there they share it).
 //   warps    0 .. 3, 4 .. 7  softmax of the two slots (heads of 256: 0 .. 3); they also bring Q and write the results
-//            then            one that issues the MMAs, one that asks for K and V (TMA, a box per page and 64 dimensions, 128-byte
+//            then            (of four) one that issues the MMAs, one that asks for K and V (TMA, a box per page and 64 dimensions, 128-byte
 //                            swizzle), in a ring of [128 keys][128 dimensions] (64 with heads of 64)
 //
 // The accumulator is rescaled only when a row's maximum has grown by more than 2^8 (a running maximum that lags changes no ratio).
@@ -28,9 +28,9 @@
 
 namespace ixb {
 
-constexpr uint32_t kPcWaitLimit = 1u << 15, kPcWaitNs = 20000;     // polls, each of at most so many nanoseconds
+constexpr uint32_t kPcWaitLimit = 1u << 20;            // polls
 constexpr uint32_t kPcKeys = 128;
-constexpr uint32_t kPcMinCost = 4;                     // key tiles of a CTA at least
+constexpr uint32_t kPcMinCost = 2;                     // of a CTA at least: the heaviest key tile (so that every CTA has the first of one)
 
 template <int D>
 struct PcCfg {
@@ -47,7 +47,10 @@ struct PcCfg {
     static constexpr uint32_t kBarOff = kRingOff + kStages * kUnit;
     static constexpr uint32_t kBars = 2 * kStages + 10;
     static constexpr uint32_t kSmem = kBarOff + kBars * 8 + 64 + 1024;         // (stages start on 1024 bytes)
-    static constexpr int kSoftWarps = 4 * kGroups, kMmaWarp = kSoftWarps, kLoadWarp = kSoftWarps + 1, kThreads = (kSoftWarps + 2) * 32;
+    static constexpr int kSoftWarps = 4 * kGroups, kMmaWarp = kSoftWarps, kLoadWarp = kSoftWarps + 1, kThreads = (kSoftWarps + 4) * 32;
+    // Registers of a thread: a softmax thread keeps a row of 128 scores.  With two groups of them the launch's 168 are dealt out
+    // again (256 x 216 + 128 x 72 = 384 x 168); with one 255 are left for everybody.
+    static constexpr bool kDeal = kGroups == 2;
     static constexpr uint32_t kPart = kUnitRows * (D + 2);                     // floats: sums [tile][D / 4][128][4], (maximum, denominator) [rows]
     static constexpr uint32_t kO = 256;                // tensor memory: S or P of the slots at 0 and 128, accumulators from here
     static_assert(kSmem + 1120 <= 227 * 1024 && kStages * kUnit >= 4 * (kPaMaxRequests + 1) && kUnit % 1024 == 0, "fits");
@@ -63,9 +66,9 @@ __device__ __forceinline__ bool pc_wait(uint32_t mbar, uint32_t parity)
     for (uint32_t it = 0; it < kPcWaitLimit; ++it) {
         uint32_t done;
         asm volatile("{\n\t.reg .pred p;\n\t"
-                     "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+                     "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
                      "selp.u32 %0, 1, 0, p;\n\t}"
-                     : "=r"(done) : "r"(mbar), "r"(parity), "r"(kPcWaitNs) : "memory");
+                     : "=r"(done) : "r"(mbar), "r"(parity) : "memory");
         if (done) return true;
     }
     return false;
@@ -225,19 +228,35 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
     // ---- the cost before every request, of one KV head (over the ring, which is empty)
     uint32_t *first = (uint32_t *)(smem + CF::kRingOff);
     const uint32_t R = a.requests, G = a.group, me = blockIdx.x;
+    auto cost_of = [&](const PagedReq &q, uint32_t t) {
+        if (t * CF::kUnitRows >= q.n * G) return 0u;
+        const PcUnit u = pc_unit<D>(q, G, t);
+        return u.tiles * u.weight;
+    };
     const uint32_t per = (R + CF::kThreads - 1) / CF::kThreads, ra = min(R, tid * per), rb = min(R, ra + per);
     uint32_t total = 0;
+    if (R <= 2u * CF::kThreads / 32u) {                // few requests, perhaps of many tiles: a warp each
+        for (uint32_t r = (uint32_t)warp; r < R; r += CF::kThreads / 32) {
+            const PagedReq q = paged_req(a, r);
+            uint32_t own = 0;
+            if (PcWalk<D>::mine(a, q))
+                for (uint32_t t = lane; t * CF::kUnitRows < q.n * G; t += 32u) own += cost_of(q, t);
+            own = __reduce_add_sync(0xffffffffu, own);
+            if (lane == 0) first[r] = own;
+        }
+    } else {
+        for (uint32_t r = ra; r < rb; ++r) {
+            const PagedReq q = paged_req(a, r);
+            uint32_t own = 0;
+            if (PcWalk<D>::mine(a, q))
+                for (uint32_t t = 0; t * CF::kUnitRows < q.n * G; ++t) own += cost_of(q, t);
+            first[r] = own;
+        }
+    }
+    __syncthreads();
     {
         uint32_t own = 0, before = 0;
-        for (uint32_t r = ra; r < rb; ++r) {
-            first[r] = own;
-            const PagedReq q = paged_req(a, r);
-            if (PcWalk<D>::mine(a, q))
-                for (uint32_t t = 0; t * CF::kUnitRows < q.n * G; ++t) {
-                    const PcUnit u = pc_unit<D>(q, G, t);
-                    own += u.tiles * u.weight;
-                }
-        }
+        for (uint32_t r = ra; r < rb; ++r) own += first[r];
         uint32_t v = own;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -252,7 +271,11 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             total += sm_warp[w];
         }
         before += v - own;
-        for (uint32_t r = ra; r < rb; ++r) first[r] += before;
+        for (uint32_t r = ra; r < rb; ++r) {
+            const uint32_t c = first[r];
+            first[r] = before;
+            before += c;
+        }
         __syncthreads();
     }
     const unsigned long long W = (unsigned long long)total * a.hkv;
@@ -275,12 +298,25 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
         w.r = lo;
         off -= first[lo];
         w.rq = paged_req(a, lo);
-        w.u = pc_unit<D>(w.rq, G, 0u);
-        w.tile = 0;
-        while (off >= w.u.tiles * w.u.weight) {
-            off -= w.u.tiles * w.u.weight;
-            w.u = pc_unit<D>(w.rq, G, ++w.tile);
+        for (w.tile = 0;; w.tile += 32u) {             // its tile: 32 at a time (off is less than the request's cost)
+            const uint32_t c = cost_of(w.rq, w.tile + lane);
+            uint32_t v = c;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const uint32_t u = __shfl_up_sync(0xffffffffu, v, d);
+                if (lane >= (uint32_t)d) v += u;
+            }
+            const uint32_t hit = __ballot_sync(0xffffffffu, v > off);
+            if (hit) {
+                const int l = __ffs(hit) - 1;
+                off -= __shfl_sync(0xffffffffu, v - c, l);
+                w.tile += (uint32_t)l;
+                break;
+            }
+            if ((w.tile + 32u) * CF::kUnitRows >= w.rq.n * G) break;           // (not so, unless the lengths change under the kernel)
+            off -= __shfl_sync(0xffffffffu, v, 31);
         }
+        w.u = pc_unit<D>(w.rq, G, w.tile);
         w.kt0 = (off + w.u.weight - 1u) / w.u.weight;  // a tile that began before this range is its predecessor's
         w.x += w.kt0 * w.u.weight - off;
         w.kt1 = w.kt0;
@@ -301,6 +337,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
     bool ok = true;
 
     if (warp == CF::kLoadWarp) {
+        if (CF::kDeal) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         // ---- K and V of every key tile, in the order K0 V0 K1 V1 ..; a box is a page's (at most 128) keys and 64 dimensions
         const uint32_t bp = min(1u << a.log_page, kPcKeys), boxes = kPcKeys / bp * (CF::kUD / 64);
         const uint32_t bk = lane / (CF::kUD / 64), panel = lane % (CF::kUD / 64);      // of lane < boxes: keys bk * bp .., 64 dimensions
@@ -340,6 +377,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             landed = pc_wait(full0 + 8u * (j % CF::kStages), j / CF::kStages & 1u) && landed;
         ok = ok && landed;
     } else if (warp == CF::kMmaWarp) {
+        if (CF::kDeal) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         uint32_t el;
         asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(el));
         uint32_t n0 = 0, seg = 0, p0 = 0, p1 = 0;      // before this segment: ring units, segments, steps of the two slots
@@ -420,7 +458,8 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             p1 += steps >> 1;
         }
         pc_commit(el, done_bar);
-    } else {
+    } else if (warp < CF::kSoftWarps) {
+        if (CF::kDeal) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         // ---- softmax: group gr of four warps has a slot (heads of 256: both); a thread is a row
         const uint32_t gr = (uint32_t)warp >> 2, row_t = tid & 127u, lanes = ((uint32_t)warp & 3u) << 21;
         const float sl2 = a.scale * 1.4426950408889634f;
@@ -431,14 +470,21 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             const uint32_t tiles = w.kt1 - w.kt0, steps = two ? 2u * tiles : tiles;
             // ---- Q: rows of the unit into [tile][64 dimensions][128 rows], swizzled; rows behind the last are zero
             if (seg) ok = ok && pc_wait(q_free, (seg - 1u) & 1u);
-            const uint32_t m0 = w.tile * CF::kUnitRows;
-            for (uint32_t i = tid; i < (two ? 256u : 128u) * (D / 8); i += CF::kSoftWarps * 32u) {
-                const uint32_t m = i / (D / 8), ch = i % (D / 8), q = m0 + m, tok = q / G;
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (m < w.u.rows) v = *(const uint4 *)(a.q + (size_t)(w.rq.row0 + tok) * a.q_stride + ((size_t)w.h * G + (q - tok * G)) * D + ch * 8u);
-                const uint32_t rr = m & 127u;
-                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(s0 + (m >> 7) * CF::kQTile + (ch >> 3) * CF::kPanel + rr * 128u + ((ch ^ rr) & 7u) * 16u),
-                             "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+            const uint32_t m0 = w.tile * CF::kUnitRows, tok0 = m0 / G, rem0 = m0 - tok0 * G;
+            {
+                constexpr uint32_t CH = D / 8, STEP = CF::kSoftWarps * 32 / CH;        // 16-byte pieces of a row, rows at a time
+                const uint32_t ch = tid % CH;
+                const __nv_bfloat16 *src = a.q + (size_t)(w.rq.row0 + tok0) * a.q_stride + (size_t)w.h * G * D + ch * 8u;
+#pragma unroll 4
+                for (uint32_t m = tid / CH; m < (two ? 256u : 128u); m += STEP) {
+                    const uint32_t q = rem0 + m, tok = G == 1u ? q : __umulhi(q, a.group_magic), rr = m & 127u;
+                    const bool on = m < w.u.rows;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                                 ::"r"(s0 + (m >> 7) * CF::kQTile + (ch >> 3) * CF::kPanel + rr * 128u + ((ch ^ rr) & 7u) * 16u),
+                                 "l"(src + (on ? tok * a.q_stride + (size_t)(q - tok * G) * D : 0)), "r"(on ? 16u : 0u) : "memory");
+                }
+                cp_async_commit();
+                cp_async_wait<0>();
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -690,6 +736,8 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             cuts[me].first_slot = cut_slot;
             cuts[me].parts = cut_parts;
         }
+    } else {
+        if (CF::kDeal) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     }
     __syncwarp();
     ok = pc_wait(done_bar, 0u) && ok;                  // (the MMAs that were issued are done, whoever gave up)

@@ -32,6 +32,7 @@ struct PagedAttn {
     uint32_t *tickets;
     size_t k_stride, v_stride, q_stride;               // elements: page to page, row to row
     uint32_t requests, width, n_pages, log_page, rows, hq, hkv, group;
+    uint32_t group_magic;                              // ceil(2^32 / group): x / group = umulhi(x, magic) for x * group < 2^32, group > 1
     uint32_t row_lo, row_hi;                           // requests with row_lo < q_len * group <= row_hi are taken
     float scale;
 };
@@ -104,7 +105,7 @@ k_attn_paged(PagedAttn a)
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(pa_smem) + wid * ST * CF::kStage;
     float *sum = (float *)(pa_smem + CF::kRing);       // [NW][8][kPitch]; before that the blocks before every request
     uint32_t *first = (uint32_t *)sum;
-    static_assert(CF::kSum >= 4 * kPaMaxRequests, "fits");
+    static_assert(CF::kSum >= 4 * kPaMaxRequests && CF::kRing >= 256 * 16 * 8, "fits");       // (parts of a pair: at most a CTA each)
     const uint32_t R = a.requests, G = a.group, page = 1u << a.log_page;
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -378,33 +379,39 @@ k_attn_paged(PagedAttn a)
         if (!whole) {
             // the CTA of block y is the last c with W c / N <= y
             const uint32_t c0 = (uint32_t)(((x0 + 1ull) * N - 1ull) / W), c1 = (uint32_t)(((x0 + kb) * N - 1ull) / W), parts = c1 - c0 + 1u;
-            __threadfence();
             __syncthreads();
             // numbers whose sum is zero, so the ticket is zero again when all have come
             if (tid == 0) {
                 const uint32_t add = me == c0 ? 1u - parts : 1u;
+                __threadfence();                       // the CTA's parts (behind the barrier) before the ticket
                 sm_last = atomicAdd(a.tickets + c0, add) + add == 0u;
+                __threadfence();
             }
             __syncthreads();
             if (sm_last) {
-                __threadfence();
-                auto slot_of = [&](uint32_t c) { return a.part + (size_t)(2u * c + (c == c0 && W * c0 / N != x0 ? 1u : 0u)) * CF::kSlot; };
+                const uint32_t behind = W * c0 / N != x0 ? 1u : 0u;
+                auto slot_of = [&](uint32_t c) { return a.part + (size_t)(2u * c + (c == c0 ? behind : 0u)) * CF::kSlot; };
+                // what every part counts, for every row: all of the parts' numbers are requested at once
+                float2 *ml = (float2 *)pa_smem;        // [parts][rows] (maximum, denominator): the ring is empty
+                for (uint32_t i = tid; i < parts * rows; i += CF::kThreads) ml[i] = __ldcg((const float2 *)(slot_of(c0 + i / rows) + 16 * D) + i % rows);
+                __syncthreads();
                 for (uint32_t it = tid; it < rows * (D / 4); it += CF::kThreads) {
                     const uint32_t m = it / (D / 4), d4 = it % (D / 4);
                     float M = -INFINITY, L = 0.f;
-                    for (uint32_t c = c0; c <= c1; ++c) M = fmaxf(M, __ldcg((const float2 *)(slot_of(c) + 16 * D) + m).x);
+                    for (uint32_t p = 0; p < parts; ++p) M = fmaxf(M, ml[p * rows + m].x);
                     const float mb = M == -INFINITY ? 0.f : M;
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-                    for (uint32_t c = c0; c <= c1; ++c) {
-                        const float2 ml = __ldcg((const float2 *)(slot_of(c) + 16 * D) + m);
-                        const float4 u = __ldcg((const float4 *)(slot_of(c) + m * D) + d4);
-                        const float f = exp2f(ml.x - mb);
-                        L = fmaf(ml.y, f, L);
+#pragma unroll 8
+                    for (uint32_t p = 0; p < parts; ++p) {
+                        const float4 u = __ldcg((const float4 *)(slot_of(c0 + p) + m * D) + d4);
+                        const float2 e = ml[p * rows + m];
+                        const float f = exp2f(e.x - mb);
+                        L = fmaf(e.y, f, L);
                         v.x = fmaf(u.x, f, v.x); v.y = fmaf(u.y, f, v.y); v.z = fmaf(u.z, f, v.z); v.w = fmaf(u.w, f, v.w);
                     }
                     write_out(m, d4, v, L);
                 }
+                __syncthreads();                       // the ring is free again
             }
         }
         x += b1 - b0;

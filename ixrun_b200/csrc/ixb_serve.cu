@@ -160,7 +160,7 @@ extern "C" int ixb_attn_paged(const void *q, const void *k_pages, const void *v_
     if (!q || !k_pages || !v_pages || !table || !length || !cu_rows || !out || !scratch) return fail(IXB_E_ARG, "NULL pointer argument");
     int rc = page_shape(requests, width, n_pages, page);
     if (rc) return rc;
-    if (hq <= 0 || hkv <= 0 || hkv > 65535 || hq % hkv) return fail(IXB_E_ARG, "query heads must be a multiple of KV heads");
+    if (hq <= 0 || hkv <= 0 || hq > 65535 || hq % hkv) return fail(IXB_E_ARG, "query heads must be a multiple of KV heads");
     if (head_dim != 64 && head_dim != 128 && head_dim != 256) return fail(IXB_E_UNSUPPORTED, "head_dim=%lld: 64, 128 or 256", (long long)head_dim);
     if (rows <= 0 || rows > 0x7fffffffll / hq || max_q <= 0) return fail(IXB_E_ARG, "bad rows");
     if (q_stride < hq * head_dim || (q_stride & 7) || k_page_stride < page * hkv * head_dim || v_page_stride < page * hkv * head_dim ||
@@ -168,7 +168,7 @@ extern "C" int ixb_attn_paged(const void *q, const void *k_pages, const void *v_
         return fail(IXB_E_ARG, "bad strides");
     if (((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)out | (uintptr_t)scratch) & 15u)
         return fail(IXB_E_ARG, "q, pages, output or scratch are not 16-byte aligned");
-    if ((size_t)num_sms() * std::max(sizeof(PcCut), sizeof(uint32_t)) > kPaCutBytes || (size_t)num_sms() * 4 > kPaTicketBytes)
+    if (num_sms() > 256 || (size_t)num_sms() * sizeof(PcCut) > kPaCutBytes)
         return fail(IXB_E_UNSUPPORTED, "a device of %d SMs", num_sms());
     if (scratch_bytes < ixb_attn_paged_scratch_bytes(head_dim)) return fail(IXB_E_SCRATCH, "attention scratch too small");
     PagedAttn a = {};
@@ -192,6 +192,7 @@ extern "C" int ixb_attn_paged(const void *q, const void *k_pages, const void *v_
     a.hq = (uint32_t)hq;
     a.hkv = (uint32_t)hkv;
     a.group = (uint32_t)(hq / hkv);
+    a.group_magic = (uint32_t)(((1ull << 32) + a.group - 1) / a.group);
     a.row_lo = 0;
     a.row_hi = 0xffffffffu;
     a.scale = scale;
