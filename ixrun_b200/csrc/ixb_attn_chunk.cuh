@@ -30,7 +30,7 @@ namespace ixb {
 
 constexpr uint32_t kPcWaitLimit = 1u << 20;            // polls
 constexpr uint32_t kPcKeys = 128;
-constexpr uint32_t kPcMinCost = 2;                     // of a CTA at least: the heaviest key tile (so that every CTA has the first of one)
+constexpr uint32_t kPcMinCost = 4;                     // key tiles of a CTA, unless there are more units than that makes CTAs
 
 template <int D>
 struct PcCfg {
@@ -45,7 +45,7 @@ struct PcCfg {
     static constexpr uint32_t kStages = D == 64 ? 8 : 5;
     static constexpr uint32_t kRingOff = kTiles * kQTile;
     static constexpr uint32_t kBarOff = kRingOff + kStages * kUnit;
-    static constexpr uint32_t kBars = 2 * kStages + 10;
+    static constexpr uint32_t kBars = 2 * kStages + 12;
     static constexpr uint32_t kSmem = kBarOff + kBars * 8 + 64 + 1024;         // (stages start on 1024 bytes)
     static constexpr int kSoftWarps = 4 * kGroups, kMmaWarp = kSoftWarps, kLoadWarp = kSoftWarps + 1, kThreads = (kSoftWarps + 4) * 32;
     // Registers of a thread: a softmax thread keeps a row of 128 scores.  With two groups of them the launch's 168 are dealt out
@@ -130,6 +130,37 @@ __device__ __forceinline__ void pc_pin(uint32_t *r)
 #pragma unroll
     for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(r[i]));
 }
+// two fp32 numbers in a register pair
+__device__ __forceinline__ uint64_t pc_pair(float lo, float hi)
+{
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+    return v;
+}
+__device__ __forceinline__ float pc_lo(uint64_t v)
+{
+    float lo, hi;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+    return lo;
+}
+__device__ __forceinline__ float pc_hi(uint64_t v)
+{
+    float lo, hi;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+    return hi;
+}
+__device__ __forceinline__ uint64_t pc_fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t pc_add2(uint64_t a, uint64_t b)
+{
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
 __device__ __forceinline__ float pc_exp2(float x)
 {
     float y;
@@ -158,7 +189,7 @@ __device__ __forceinline__ PcUnit pc_unit(const PagedReq &q, uint32_t G, uint32_
 // the CTA's way through its units; every role walks it for itself
 template <int D>
 struct PcWalk {
-    unsigned long long x, x_end, x_begin;              // cost before the next key tile
+    unsigned long long x, x_end;                       // cost before the next key tile, and where the CTA's range ends
     uint32_t h, r, tile, kt0, kt1;                     // this segment: key tiles kt0 .. kt1 - 1 of the unit
     PagedReq rq;
     PcUnit u;
@@ -202,11 +233,11 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
     const uint32_t tid = threadIdx.x, lane = tid & 31u;
     const int warp = __shfl_sync(0xffffffffu, (int)(tid >> 5), 0);
     const uint32_t ring = s0 + CF::kRingOff, full0 = s0 + CF::kBarOff, empty0 = full0 + 8u * CF::kStages, q_full = empty0 + 8u * CF::kStages,
-                   q_free = q_full + 8u, s_full0 = q_free + 8u, p_full0 = s_full0 + 16u, o_full0 = p_full0 + 16u, pv_done = o_full0 + 16u,
+                   q_free = q_full + 8u, s_full0 = q_free + 8u, p_full0 = s_full0 + 16u, p_half0 = p_full0 + 16u, o_full0 = p_half0 + 16u, pv_done = o_full0 + 16u,
                    done_bar = pv_done + 8u;
     uint32_t *tmem_slot = (uint32_t *)(smem + CF::kBarOff + CF::kBars * 8);
     volatile uint32_t *wild_s = tmem_slot + 1;         // [2]: the slot's P V is done by its softmax warps
-    __shared__ uint32_t sm_warp[CF::kThreads / 32];
+    __shared__ uint32_t sm_warp[CF::kThreads / 32], sm_units, sm_two;
     __shared__ float2 sm_ml[128];
     asm volatile("griddepcontrol.launch_dependents;");
     if (tid == 0) {
@@ -217,13 +248,20 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
         init(q_full, 1u, CF::kSoftWarps);
         init(q_free, 1u, 1u);
         init(s_full0, 2u, 1u);
-        init(p_full0, 2u, 4u);
+        init(p_full0, 4u, 4u);                         // (and p_half0)
         init(o_full0, 2u, 1u);
         init(pv_done, 2u, 1u);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
+        sm_units = sm_two = 0u;
     }
+    if (warp == CF::kMmaWarp) {
+        const uint32_t slot_addr = (uint32_t)__cvta_generic_to_shared(tmem_slot);
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot_addr), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    __syncthreads();
     asm volatile("griddepcontrol.wait;" ::: "memory");
     // ---- the cost before every request, of one KV head (over the ring, which is empty)
     uint32_t *first = (uint32_t *)(smem + CF::kRingOff);
@@ -232,6 +270,10 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
         if (t * CF::kUnitRows >= q.n * G) return 0u;
         const PcUnit u = pc_unit<D>(q, G, t);
         return u.tiles * u.weight;
+    };
+    auto count = [&](const PagedReq &q) {
+        atomicAdd(&sm_units, (q.n * G + CF::kUnitRows - 1u) / CF::kUnitRows);
+        if (CF::kTiles == 2 && q.n * G > 128u) sm_two = 1u;
     };
     const uint32_t per = (R + CF::kThreads - 1) / CF::kThreads, ra = min(R, tid * per), rb = min(R, ra + per);
     uint32_t total = 0;
@@ -242,7 +284,10 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             if (PcWalk<D>::mine(a, q))
                 for (uint32_t t = lane; t * CF::kUnitRows < q.n * G; t += 32u) own += cost_of(q, t);
             own = __reduce_add_sync(0xffffffffu, own);
-            if (lane == 0) first[r] = own;
+            if (lane == 0) {
+                first[r] = own;
+                if (own) count(q);
+            }
         }
     } else {
         for (uint32_t r = ra; r < rb; ++r) {
@@ -251,6 +296,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             if (PcWalk<D>::mine(a, q))
                 for (uint32_t t = 0; t * CF::kUnitRows < q.n * G; ++t) own += cost_of(q, t);
             first[r] = own;
+            if (own) count(q);
         }
     }
     __syncthreads();
@@ -279,16 +325,25 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
         __syncthreads();
     }
     const unsigned long long W = (unsigned long long)total * a.hkv;
-    const uint32_t N = (uint32_t)min((unsigned long long)gridDim.x, (W + kPcMinCost - 1u) / kPcMinCost);
+    // CTAs: one for every four key tiles, or every unit if that is more; with units of two row tiles a range is at least as long as a
+    // key tile's cost, so that every CTA between the first and the last of a unit has a key tile of it
+    unsigned long long n_max = max((unsigned long long)sm_units * a.hkv, (W + kPcMinCost - 1u) / kPcMinCost);
+    if (sm_two) n_max = min(n_max, max(W / 2u, 1ull));
+    const uint32_t N = (uint32_t)min((unsigned long long)gridDim.x, n_max);
+    auto part_of = [&](uint32_t c) { return W < 1u << 24 ? (unsigned long long)((uint32_t)W * c / N) : W * c / N; };      // (N at most 256)
+    auto cta_of = [&](unsigned long long y) {          // the last c with part_of(c) <= y
+        return W < 1u << 24 ? (((uint32_t)y + 1u) * N - 1u) / (uint32_t)W : (uint32_t)(((y + 1ull) * N - 1ull) / W);
+    };
     if (me >= N) {
         if (tid == 0) cuts[me].parts = 0u;
+        if (warp == CF::kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*tmem_slot), "r"(512u) : "memory");
         return;
     }
     PcWalk<D> w;
-    w.x = w.x_begin = W * me / N;
-    w.x_end = W * (me + 1ull) / N;
+    w.x = part_of(me);
+    w.x_end = part_of(me + 1u);
     {
-        w.h = (uint32_t)(w.x / total);
+        w.h = W < 1u << 24 ? (uint32_t)w.x / total : (uint32_t)(w.x / total);
         uint32_t off = (uint32_t)(w.x - (unsigned long long)w.h * total), lo = 0, hi = R;
         while (hi - lo > 1u) {                         // the last request with first[r] <= off
             const uint32_t mid = (lo + hi) / 2u;
@@ -324,11 +379,6 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
     }
     // (an empty first segment: the range begins inside the last tile of a unit)
     bool work = w.kt1 > w.kt0 || w.next(a);
-    if (warp == CF::kMmaWarp) {
-        const uint32_t slot_addr = (uint32_t)__cvta_generic_to_shared(tmem_slot);
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot_addr), "r"(512u) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");               // (the ring held the requests' costs)
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -414,7 +464,8 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
                 const uint32_t slot = st & 1u, j = two ? st >> 1 : st, kt = w.kt0 + j;
                 const bool last_use = !two || slot;
                 const uint32_t valid = w.u.keys > kt * kPcKeys ? min(kPcKeys, w.u.keys - kt * kPcKeys) : 0u;
-                wait(p_full0 + 8u * slot, ((slot ? p1 : p0) + (st >> 1)) & 1u);
+                const uint32_t p_par = ((slot ? p1 : p0) + (st >> 1)) & 1u;
+                wait(p_half0 + 8u * slot, p_par);      // the first 64 keys' probabilities
                 if (!ok) break;
                 const bool wild = wild_s[slot] != 0u;
                 const uint32_t o = tmem + CF::kO + (CF::kTiles == 2 ? slot * 128u : 0u);
@@ -433,17 +484,25 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         __syncwarp();
                     }
-                    if (!wild) {
-                        if (valid == kPcKeys) {
+                    auto pv = [&](uint32_t kk) {
+                        pc_mma_ts(el, o + c * CF::kUD, tmem + slot * 128u + kk * 8u, pc_desc(base + kk * 2048u, CF::kPanel, 1024u), pc_idesc(CF::kUD, 1u), kk ? 1u : acc);
+                    };
+                    const uint32_t steps16 = wild ? 0u : (valid + 15u) / 16u;
+                    if (steps16 >= 4u) {
 #pragma unroll
-                            for (uint32_t kk = 0; kk < kPcKeys / 16u; ++kk)
-                                pc_mma_ts(el, o + c * CF::kUD, tmem + slot * 128u + kk * 8u, pc_desc(base + kk * 2048u, CF::kPanel, 1024u), pc_idesc(CF::kUD, 1u),
-                                          kk ? 1u : acc);
-                        } else {
-                            for (uint32_t kk = 0; kk * 16u < valid; ++kk)
-                                pc_mma_ts(el, o + c * CF::kUD, tmem + slot * 128u + kk * 8u, pc_desc(base + kk * 2048u, CF::kPanel, 1024u), pc_idesc(CF::kUD, 1u),
-                                          kk ? 1u : acc);
-                        }
+                        for (uint32_t kk = 0; kk < 4u; ++kk) pv(kk);
+                    } else {
+                        for (uint32_t kk = 0; kk < steps16; ++kk) pv(kk);
+                    }
+                    if (c == 0) {
+                        wait(p_full0 + 8u * slot, p_par);
+                        if (!ok) break;
+                    }
+                    if (steps16 == 8u) {
+#pragma unroll
+                        for (uint32_t kk = 4; kk < 8u; ++kk) pv(kk);
+                    } else {
+                        for (uint32_t kk = 4; kk < steps16; ++kk) pv(kk);
                     }
                     if (last_use) pc_commit(el, empty0 + 8u * rs);
                 }
@@ -563,17 +622,28 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
                         }
                     }
                     const float nb = mb == -INFINITY ? 0.f : -mb;
-                    float la[4] = {0.f, 0.f, 0.f, 0.f};
+                    uint64_t la = 0, lb = 0;           // pairs of sums
+                    const uint64_t sl2_2 = pc_pair(sl2, sl2), nb_2 = pc_pair(nb, nb);
 #pragma unroll
-                    for (int c = 0; c < 128; c += 2) {
-                        const float p0 = pc_exp2(fmaf(__uint_as_float(s[c]), sl2, nb)), p1 = pc_exp2(fmaf(__uint_as_float(s[c + 1]), sl2, nb));
-                        la[c >> 1 & 3] += p0 + p1;
-                        s[c / 2] = pa_pack(p0, p1);
+                    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                        for (int c = 64 * half; c < 64 * half + 64; c += 2) {
+                            const uint64_t x = pc_fma2(pc_pair(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), sl2_2, nb_2);
+                            const float p0 = pc_exp2(pc_lo(x)), p1 = pc_exp2(pc_hi(x));
+                            if (c & 2) la = pc_add2(la, pc_pair(p0, p1));
+                            else lb = pc_add2(lb, pc_pair(p0, p1));
+                            s[c / 2] = pa_pack(p0, p1);
+                        }
+                        pc_st32(s_at + 32u * half, s + 32 * half);
+                        pc_wait_st();
+                        if (half == 0) {
+                            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                            __syncwarp();
+                            if (lane == 0) pc_arrive(p_half0 + 8u * slot);
+                        }
                     }
-                    l += (la[0] + la[1]) + (la[2] + la[3]);
-                    pc_st32(s_at, s);
-                    pc_st32(s_at + 32u, s + 32);
-                    pc_wait_st();
+                    la = pc_add2(la, lb);
+                    l += pc_lo(la) + pc_hi(la);
                     if (wild) {
                         // P V of this tile for this thread's row: what the row does not see is left out
 #pragma unroll 1
@@ -615,8 +685,10 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
                         }
                         pc_wait_st();
                     }
-                } else if (CF::kTiles == 1 && st) {    // (keeps up with the barrier's phases)
-                    ok = ok && pc_wait(pv_done, (pv_cnt + st - 1u) & 1u);
+                } else {
+                    if (CF::kTiles == 1 && st) ok = ok && pc_wait(pv_done, (pv_cnt + st - 1u) & 1u);        // (keeps up with the barrier's phases)
+                    __syncwarp();
+                    if (lane == 0) pc_arrive(p_half0 + 8u * slot);
                 }
                 any = true;
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -638,8 +710,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             const uint32_t slot_n = 2u * me + (w.kt0 ? 0u : 1u);               // a unit's first part is this CTA's last segment
             float *part = a.part + (size_t)slot_n * CF::kPart;
             if (!whole && w.kt0 == 0u) {
-                const uint32_t c1 = (uint32_t)(((x0 + (unsigned long long)(w.u.tiles - 1u) * w.u.weight + 1ull) * N - 1ull) / W);
-                cut_parts = c1 - me + 1u;
+                cut_parts = cta_of(x0 + (unsigned long long)(w.u.tiles - 1u) * w.u.weight) - me + 1u;
                 cut_r = w.r;
                 cut_tile = w.tile;
                 cut_h = w.h;
