@@ -28,7 +28,6 @@
 
 namespace ixb {
 
-constexpr uint32_t kPcWaitLimit = 1u << 20;            // polls
 constexpr uint32_t kPcKeys = 128;
 constexpr uint32_t kPcMinCost = 4;                     // key tiles of a CTA, unless there are more units than that makes CTAs
 
@@ -46,14 +45,14 @@ struct PcCfg {
     static constexpr uint32_t kRingOff = kTiles * kQTile;
     static constexpr uint32_t kBarOff = kRingOff + kStages * kUnit;
     static constexpr uint32_t kBars = 2 * kStages + 12;
-    static constexpr uint32_t kSmem = kBarOff + kBars * 8 + 64 + 1024;         // (stages start on 1024 bytes)
+    static constexpr uint32_t kSmem = kBarOff + kBars * 8 + 1024 + 128;        // and a few words; no static arrays: stages start on 1024 bytes
     static constexpr int kSoftWarps = 4 * kGroups, kMmaWarp = kSoftWarps, kLoadWarp = kSoftWarps + 1, kThreads = (kSoftWarps + 4) * 32;
     // Registers of a thread: a softmax thread keeps a row of 128 scores.  With two groups of them the launch's 168 are dealt out
     // again (256 x 216 + 128 x 72 = 384 x 168); with one 255 are left for everybody.
     static constexpr bool kDeal = kGroups == 2;
     static constexpr uint32_t kPart = kUnitRows * (D + 2);                     // floats: sums [tile][D / 4][128][4], (maximum, denominator) [rows]
     static constexpr uint32_t kO = 256;                // tensor memory: S or P of the slots at 0 and 128, accumulators from here
-    static_assert(kSmem + 1120 <= 227 * 1024 && kStages * kUnit >= 4 * (kPaMaxRequests + 1) && kUnit % 1024 == 0, "fits");
+    static_assert(kSmem <= 227 * 1024 && kStages * kUnit >= 4 * (kPaMaxRequests + 1) && kUnit % 1024 == 0, "fits");
 };
 
 // a unit that was cut, under the number of the CTA that has its first key tile; parts 0: none
@@ -61,18 +60,6 @@ struct PcCut {
     uint32_t parts, request, tile, head, first_slot;
 };
 
-__device__ __forceinline__ bool pc_wait(uint32_t mbar, uint32_t parity)
-{
-    for (uint32_t it = 0; it < kPcWaitLimit; ++it) {
-        uint32_t done;
-        asm volatile("{\n\t.reg .pred p;\n\t"
-                     "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-                     "selp.u32 %0, 1, 0, p;\n\t}"
-                     : "=r"(done) : "r"(mbar), "r"(parity) : "memory");
-        if (done) return true;
-    }
-    return false;
-}
 __device__ __forceinline__ void pc_arrive(uint32_t mbar)
 {
     asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.shared::cta.b64 st, [%0];\n\t}" ::"r"(mbar) : "memory");
@@ -161,13 +148,6 @@ __device__ __forceinline__ uint64_t pc_add2(uint64_t a, uint64_t b)
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
-__device__ __forceinline__ float pc_exp2(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // a unit of a request: rows, keys that any of them sees, key tiles (one even if there is nothing to see: its rows become zero), cost
 struct PcUnit {
     uint32_t rows, keys, tiles, weight;
@@ -227,18 +207,17 @@ __global__ void __launch_bounds__(PcCfg<D>::kThreads, 1)
 k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, PcCut *cuts)
 {
     using CF = PcCfg<D>;
-    extern __shared__ __align__(16) unsigned char pc_smem_raw[];
-    unsigned char *smem = pc_smem_raw + ((1024u - ((uint32_t)__cvta_generic_to_shared(pc_smem_raw) & 1023u)) & 1023u);
+    extern __shared__ __align__(1024) unsigned char pc_smem[];
+    unsigned char *smem = pc_smem;
     const uint32_t s0 = (uint32_t)__cvta_generic_to_shared(smem);
     const uint32_t tid = threadIdx.x, lane = tid & 31u;
     const int warp = __shfl_sync(0xffffffffu, (int)(tid >> 5), 0);
     const uint32_t ring = s0 + CF::kRingOff, full0 = s0 + CF::kBarOff, empty0 = full0 + 8u * CF::kStages, q_full = empty0 + 8u * CF::kStages,
                    q_free = q_full + 8u, s_full0 = q_free + 8u, p_full0 = s_full0 + 16u, p_half0 = p_full0 + 16u, o_full0 = p_half0 + 16u, pv_done = o_full0 + 16u,
                    done_bar = pv_done + 8u;
-    uint32_t *tmem_slot = (uint32_t *)(smem + CF::kBarOff + CF::kBars * 8);
-    volatile uint32_t *wild_s = tmem_slot + 1;         // [2]: the slot's P V is done by its softmax warps
-    __shared__ uint32_t sm_warp[CF::kThreads / 32], sm_units, sm_two;
-    __shared__ float2 sm_ml[128];
+    float2 *sm_ml = (float2 *)(smem + CF::kBarOff + CF::kBars * 8);            // [128]
+    uint32_t *tmem_slot = (uint32_t *)(sm_ml + 128), &sm_units = tmem_slot[1], &sm_two = tmem_slot[2], *sm_warp = tmem_slot + 8;
+    volatile uint32_t *wild_s = tmem_slot + 4;         // [2]: the slot's P V is done by its softmax warps
     asm volatile("griddepcontrol.launch_dependents;");
     if (tid == 0) {
         auto init = [&](uint32_t bar, uint32_t n, uint32_t count) {
@@ -407,7 +386,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
 #pragma unroll
                 for (uint32_t i = 0; i < 2u * CF::kNU; ++i, ++n) {
                     const uint32_t st = n % CF::kStages, bar = full0 + 8u * st;
-                    ok = ok && pc_wait(empty0 + 8u * st, (n / CF::kStages & 1u) ^ 1u);
+                    ok = ok && pa_wait(empty0 + 8u * st, (n / CF::kStages & 1u) ^ 1u);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     if (lane == 0) asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(bar), "r"(bytes) : "memory");
@@ -424,7 +403,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
         // the copies that may still be in flight (the tensor core's warp waits for them too, unless it gave up)
         bool landed = true;
         for (uint32_t j = n > CF::kStages ? n - CF::kStages : 0u; j < n; ++j)
-            landed = pc_wait(full0 + 8u * (j % CF::kStages), j / CF::kStages & 1u) && landed;
+            landed = pa_wait(full0 + 8u * (j % CF::kStages), j / CF::kStages & 1u) && landed;
         ok = ok && landed;
     } else if (warp == CF::kMmaWarp) {
         if (CF::kDeal) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
@@ -435,7 +414,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             const bool two = w.u.weight == 2u;         // two row tiles: a key tile is two steps
             const uint32_t tiles = w.kt1 - w.kt0, steps = two ? 2u * tiles : tiles;
             auto wait = [&](uint32_t bar, uint32_t parity) {
-                ok = ok && pc_wait(bar, parity);
+                ok = ok && pa_wait(bar, parity);
                 ok = __all_sync(0xffffffffu, ok);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             };
@@ -528,7 +507,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             const bool two = w.u.weight == 2u;
             const uint32_t tiles = w.kt1 - w.kt0, steps = two ? 2u * tiles : tiles;
             // ---- Q: rows of the unit into [tile][64 dimensions][128 rows], swizzled; rows behind the last are zero
-            if (seg) ok = ok && pc_wait(q_free, (seg - 1u) & 1u);
+            if (seg) ok = ok && pa_wait(q_free, (seg - 1u) & 1u);
             const uint32_t m0 = w.tile * CF::kUnitRows, tok0 = m0 / G, rem0 = m0 - tok0 * G;
             {
                 constexpr uint32_t CH = D / 8, STEP = CF::kSoftWarps * 32 / CH;        // 16-byte pieces of a row, rows at a time
@@ -561,14 +540,14 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             for (uint32_t st = CF::kTiles == 2 ? gr : 0u; st < steps; st += stride) {
                 const uint32_t slot = st & 1u, j = two ? st >> 1 : st, kt = w.kt0 + j, s_at = tmem + lanes + slot * 128u;
                 const int32_t key0 = (int32_t)(kt * kPcKeys), key_last = min(key0 + (int32_t)kPcKeys, (int32_t)w.u.keys) - 1;
-                ok = ok && pc_wait(s_full0 + 8u * slot, ((slot ? c1s : c0s) + (st >> 1)) & 1u);
+                ok = ok && pa_wait(s_full0 + 8u * slot, ((slot ? c1s : c0s) + (st >> 1)) & 1u);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 bool wild = false;
                 if (key_last > low_tile) {             // (group uniform) not every row sees every key: is there a value that is not finite?
                     uint32_t big = 0;
                     for (int c = 0; c < CF::kNU; ++c) {
                         const uint32_t n = n0 + (2u * j + 1u) * CF::kNU + c, rs = n % CF::kStages;
-                        ok = ok && pc_wait(full0 + 8u * rs, n / CF::kStages & 1u);
+                        ok = ok && pa_wait(full0 + 8u * rs, n / CF::kStages & 1u);
                         for (uint32_t i = row_t; i < (uint32_t)(key_last - key0 + 1) * (CF::kUD / 8); i += 128u) {
                             uint4 v;
                             asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
@@ -600,11 +579,11 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
                     for (int c = 0; c < 128; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(s[c]));
                     const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
                     if (CF::kTiles == 1 && st) {       // the accumulator is the step before's too
-                        ok = ok && pc_wait(pv_done, (pv_cnt + st - 1u) & 1u);
+                        ok = ok && pa_wait(pv_done, (pv_cnt + st - 1u) & 1u);
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     }
                     if (__any_sync(0xffffffffu, top > mb + 8.f)) {             // (false for -inf; the first maximum of a row is larger than -inf)
-                        const float mn = fmaxf(mb, top), f = pc_exp2(mb - (mn == -INFINITY ? 0.f : mn));
+                        const float mn = fmaxf(mb, top), f = pa_exp2(mb - (mn == -INFINITY ? 0.f : mn));
                         mb = mn;
                         l *= f;
                         if (any) {
@@ -629,7 +608,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
 #pragma unroll
                         for (int c = 64 * half; c < 64 * half + 64; c += 2) {
                             const uint64_t x = pc_fma2(pc_pair(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), sl2_2, nb_2);
-                            const float p0 = pc_exp2(pc_lo(x)), p1 = pc_exp2(pc_hi(x));
+                            const float p0 = pa_exp2(pc_lo(x)), p1 = pa_exp2(pc_hi(x));
                             if (c & 2) la = pc_add2(la, pc_pair(p0, p1));
                             else lb = pc_add2(lb, pc_pair(p0, p1));
                             s[c / 2] = pa_pack(p0, p1);
@@ -686,7 +665,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
                         pc_wait_st();
                     }
                 } else {
-                    if (CF::kTiles == 1 && st) ok = ok && pc_wait(pv_done, (pv_cnt + st - 1u) & 1u);        // (keeps up with the barrier's phases)
+                    if (CF::kTiles == 1 && st) ok = ok && pa_wait(pv_done, (pv_cnt + st - 1u) & 1u);        // (keeps up with the barrier's phases)
                     __syncwarp();
                     if (lane == 0) pc_arrive(p_half0 + 8u * slot);
                 }
@@ -700,8 +679,8 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             c1s += steps >> 1;
             n0 += 2u * tiles * CF::kNU;
             // ---- the unit's sums
-            ok = ok && pc_wait(o_full0 + 8u * gr, seg & 1u);
-            if (CF::kTiles == 1) ok = ok && pc_wait(pv_done, (pv_cnt - 1u) & 1u);
+            ok = ok && pa_wait(o_full0 + 8u * gr, seg & 1u);
+            if (CF::kTiles == 1) ok = ok && pa_wait(pv_done, (pv_cnt - 1u) & 1u);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (!ok) l = __int_as_float(0x7fc00000);
             const bool whole = w.kt0 == 0u && w.kt1 == w.u.tiles;
@@ -732,8 +711,8 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
                 if (gr == 0u) {
                     const float2 o = sm_ml[row_t];
                     const float mn = fmaxf(mb, o.x), mz = mn == -INFINITY ? 0.f : mn;
-                    f_own = pc_exp2(mb - mz);
-                    f_other = pc_exp2(o.x - mz);
+                    f_own = pa_exp2(mb - mz);
+                    f_other = pa_exp2(o.x - mz);
                     other_l = o.y;
                     mb = mn;
                     l = l * f_own + other_l * f_other;
@@ -811,7 +790,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
         if (CF::kDeal) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     }
     __syncwarp();
-    ok = pc_wait(done_bar, 0u) && ok;                  // (the MMAs that were issued are done, whoever gave up)
+    ok = pa_wait(done_bar, 0u) && ok;                  // (the MMAs that were issued are done, whoever gave up)
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (warp == CF::kMmaWarp) {
@@ -843,7 +822,7 @@ k_attn_chunk_join(PagedAttn a, const PcCut *cuts)
     for (int c = 0; c < 8; ++c) v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
     for (uint32_t p = 0; p < cut.parts; ++p) {
         const float2 ml = ((const float2 *)(part(p) + CF::kUnitRows * D))[m];
-        const float f = pc_exp2(ml.x - mz);
+        const float f = pa_exp2(ml.x - mz);
         L = fmaf(ml.y, f, L);
         const float4 *src = (const float4 *)part(p) + (size_t)(tile * (D / 4) + c0) * 128u + row;
 #pragma unroll

@@ -113,12 +113,11 @@ extern "C" size_t ixb_attn_paged_scratch_bytes(int64_t head_dim)
     return kPaTicketBytes + kPaCutBytes + (head_dim == 64 ? attn_part_bytes<64>() : head_dim == 128 ? attn_part_bytes<128>() : attn_part_bytes<256>());
 }
 
-// a pool as a tensor of [pages][page][kv heads][D]: boxes of 64 dimensions of one head of (at most 128) positions of a page
-static CUresult pool_map(CUtensorMap *map, const __nv_bfloat16 *pool, size_t page_stride, const PagedAttn &a, uint32_t D)
+// a pool as a tensor of [pages][page][kv heads][D]: boxes of 64 dimensions of one head of `keys` positions of a page
+static CUresult pool_map(CUtensorMap *map, const __nv_bfloat16 *pool, size_t page_stride, const PagedAttn &a, uint32_t D, uint32_t keys)
 {
-    const uint32_t page = 1u << a.log_page;
-    const cuuint64_t dims[4] = {D, a.hkv, page, a.n_pages}, strides[3] = {D * 2ull, (cuuint64_t)a.hkv * D * 2, (cuuint64_t)page_stride * 2};
-    const cuuint32_t box[4] = {64, 1, std::min(page, kPcKeys), 1}, one[4] = {1, 1, 1, 1};
+    const cuuint64_t dims[4] = {D, a.hkv, 1ull << a.log_page, a.n_pages}, strides[3] = {D * 2ull, (cuuint64_t)a.hkv * D * 2, (cuuint64_t)page_stride * 2};
+    const cuuint32_t box[4] = {64, 1, keys, 1}, one[4] = {1, 1, 1, 1};
     return tensor_map_encoder()(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<__nv_bfloat16 *>(pool), dims, strides, box, one,
                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -129,26 +128,30 @@ static int attn_paged_run(PagedAttn a, PcCut *cuts, int64_t max_q, cudaStream_t 
 {
     const unsigned sms = (unsigned)num_sms();
     const bool few = max_q * a.group <= kAttnFewRows, both = !few && a.requests > 1u;
+    if (!tensor_map_encoder()) return fail(IXB_E_UNSUPPORTED, "the driver has no cuTensorMapEncodeTiled");
+    CUtensorMap kmap, vmap;
+    auto maps = [&](uint32_t keys) {
+        CUresult r = pool_map(&kmap, a.k, a.k_stride, a, D, keys);
+        if (r == CUDA_SUCCESS) r = pool_map(&vmap, a.v, a.v_stride, a, D, keys);
+        return r == CUDA_SUCCESS ? IXB_OK : fail(IXB_E_CUDA, "tensor map of a pool: error %d", (int)r);
+    };
+    int rc;
     if (few || both) {
         if (both) a.row_hi = kAttnFewRows;
+        if ((rc = maps(16))) return rc;
         static bool attr_set[64] = {false};
         IXB_CUDA(opt_in_smem(k_attn_paged<D>, attr_set, (int)PaCfg<D>::kSmem));
-        IXB_CUDA(launch_glue_smem(k_attn_paged<D>, dim3(sms), dim3(PaCfg<D>::kThreads), PaCfg<D>::kSmem, st, a));
-        const int rc = launch_check("k_attn_paged");
+        IXB_CUDA(launch_glue_smem(k_attn_paged<D>, dim3(sms), dim3(PaCfg<D>::kThreads), PaCfg<D>::kSmem, st, a, kmap, vmap));
+        rc = launch_check("k_attn_paged");
         if (rc || few) return rc;
         a.row_lo = kAttnFewRows;
         a.row_hi = 0xffffffffu;
     }
-    if (!tensor_map_encoder()) return fail(IXB_E_UNSUPPORTED, "the driver has no cuTensorMapEncodeTiled");
-    CUtensorMap kmap, vmap;
-    CUresult r = pool_map(&kmap, a.k, a.k_stride, a, D);
-    if (r == CUDA_SUCCESS) r = pool_map(&vmap, a.v, a.v_stride, a, D);
-    if (r != CUDA_SUCCESS) return fail(IXB_E_CUDA, "tensor map of a pool: error %d", (int)r);
+    if ((rc = maps(std::min(1u << a.log_page, kPcKeys)))) return rc;
     static bool attr_set[64] = {false};
     IXB_CUDA(opt_in_smem(k_attn_chunk<D>, attr_set, (int)PcCfg<D>::kSmem));
     IXB_CUDA(launch_glue_smem(k_attn_chunk<D>, dim3(sms), dim3(PcCfg<D>::kThreads), PcCfg<D>::kSmem, st, a, kmap, vmap, cuts));
-    const int rc = launch_check("k_attn_chunk");
-    if (rc) return rc;
+    if ((rc = launch_check("k_attn_chunk"))) return rc;
     IXB_GLUE("k_attn_chunk_join", launch_glue_smem(k_attn_chunk_join<D>, dim3(sms, PcCfg<D>::kTiles * (D / 32)), dim3(128), 0, st, a, (const PcCut *)cuts));
 }
 
