@@ -207,6 +207,12 @@ class _PythonHost:
     def p6(*_):
         return lambda x, bias, many: None
 
+    @staticmethod
+    def page_step(*_):
+        return None
+
+    rope_paged = attn_paged = logits = page_step
+
 
 def host():
     """The extension for the host side of a call (csrc/ixb_host.cpp), built first if it is missing or stale; where that
@@ -223,6 +229,7 @@ def host():
             _host = _PythonHost
             return _host
         L = lib()
+        _ixbhost.bind_serve(*(C.cast(f, C.c_void_p).value for f in (L.ixb_page_step, L.ixb_rope_paged, L.ixb_attn_paged, L.ixb_logits)))
         _ixbhost.bind(C.cast(L.ixb_p6_gemv, C.c_void_p).value, C.cast(L.ixb_p6_rows, C.c_void_p).value, check)
         _host = _ixbhost
     return _host

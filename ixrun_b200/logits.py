@@ -37,6 +37,10 @@ def apply_rules(logits, history=None, n_tokens=None, n_prompt=None, repetition=N
     bias_ids are passed over (-1 as padding).  n_prompt None: everything counts as generated; penalties None: 1, 0, 0 (fp32 [B]).
     Writes out (fp32 [B, V], may be the fp32 logits; allocated if None) and token (int64 [B], may be None): the lowest index
     of the largest value.  Returns out."""
+    if out is None and logits.dim() == 2:
+        out = torch.empty(logits.shape, dtype=torch.float32, device=logits.device)
+    if out is not None and _lib.host().logits(logits, history, n_tokens, n_prompt, repetition, presence, frequency, bias_ids, bias_values, mask, mask_row, out, token):
+        return out
     if logits.dim() != 2 or not logits.is_cuda:
         raise ValueError("logits: a CUDA tensor [B, V] expected")
     dev, (b, v) = logits.get_device(), logits.shape
@@ -73,8 +77,6 @@ def apply_rules(logits, history=None, n_tokens=None, n_prompt=None, repetition=N
         if mask is None:
             raise ValueError("mask_row without mask")
         _on(dev, mask_row, i32, (b,), "mask_row")
-    if out is None:
-        out = torch.empty(b, v, dtype=torch.float32, device=logits.device)
     out_pitch = _on(dev, out, f32, (b, v), "out")
     if token is not None:
         _on(dev, token, (torch.int64,), (b,), "token")

@@ -14,6 +14,7 @@ from collections import namedtuple
 import torch
 
 from . import _lib
+from ._lib import host as _host
 from .glue import _bf16, _rows_view
 
 __all__ = ["PageStep", "page_step", "page_release", "PageTables", "rope_kv_paged", "AttnPaged"]
@@ -33,9 +34,14 @@ class PageStep(namedtuple("PageStep", "cu_rows length n_free slot pos owner stat
     @classmethod
     def empty(cls, requests: int, rows: int, device, length=None, n_free=None):
         """Tensors for a step; length and n_free: existing ones to be updated in place."""
-        new = lambda n: torch.empty(n, dtype=torch.int32, device=device)  # noqa: E731
-        return cls(new(requests + 1), new(requests) if length is None else length, new(1) if n_free is None else n_free, new(rows),
-                   new(rows), new(rows), new(2))
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise ValueError("expected a CUDA device")
+        index = torch.cuda.current_device() if device.index is None else device.index
+        cu_rows, new_length, new_n_free, slot, pos, owner, status = _host().empty(
+            index, (requests + 1, "i"), (0 if length is not None else requests, "i"), (0 if n_free is not None else 1, "i"), (rows, "i"), (rows, "i"),
+            (rows, "i"), (2, "i"))
+        return cls(cu_rows, new_length if length is None else length, new_n_free if n_free is None else n_free, slot, pos, owner, status)
 
 
 def _ints(device, **tensors):
@@ -58,6 +64,8 @@ def page_step(q_len, length, table, free, n_free, page: int, rows: int, out: Pag
     the new tokens are packed into, at least as many as there are (a captured step has a fixed number).  out: tensors to
     write (``PageStep.empty``); out.length may be length and out.n_free n_free (updated in place).  All int32.
     A step that does not fit (out.status[0] != 0) takes no page and is empty: cu_rows is zero."""
+    if out is not None and _host().page_step(q_len, length, table, free, n_free, page, rows, *out):
+        return out
     _page(page)
     dev, r = q_len.get_device(), q_len.numel()
     _ints(dev, q_len=q_len, length=length, table=table, free=free, n_free=n_free)
@@ -149,6 +157,8 @@ def rope_kv_paged(q, k, v, pos, slot, k_pages, v_pages, cos, sin, hq: int, hkv: 
     """``glue.rope_kv`` for a paged cache: q [rows, >= hq*head_dim] rotated (in place, or into out [rows, hq*head_dim]); k, v [rows,
     hkv*head_dim] into the pools at slot [rows]; pos, slot: int32 [rows] as ``page_step`` gives them.  Column slices are allowed.  A
     row whose slot is outside the pools is left alone.  Between the norm and the result nothing is rounded."""
+    if _host().rope_paged(q, k, v, pos, slot, k_pages, v_pages, cos, sin, hq, hkv, head_dim, rot_dim or head_dim, q_norm, k_norm, eps, q if out is None else out):
+        return q if out is None else out
     _bf16(q_norm, k_norm)
     rows, qcols, q_pitch = _rows_view(q, "q")
     _, kcols, kv_pitch = _rows_view(k, "k")
@@ -214,6 +224,9 @@ class AttnPaged:
         cu_rows [R+1], table: int32.  Every row attends to the positions up to its own.  max_q: the most new tokens that a request has
         (1 for a step of single tokens), by which the kernels are chosen.  Returns out [rows, hq*head_dim]; rows of no request are left
         as they are (undefined without `out`), rows that see no position are zero."""
+        done = _host().attn_paged(self.hq, self.hkv, self.d, self.scratch, q, k_pages, v_pages, table, length, cu_rows, max_q, out, scale)
+        if done is not None:
+            return done
         rows, cols, pitch = _rows_view(q, "q")
         n_pages, page, k_pitch = _pool(k_pages, self.hkv, self.d, "k_pages")
         vn, vp, v_pitch = _pool(v_pages, self.hkv, self.d, "v_pages")
