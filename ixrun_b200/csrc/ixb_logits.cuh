@@ -9,22 +9,29 @@
 //   out[b][v] = x;  token[b] = the lowest v with the largest x (a NaN counts as the largest)
 // Every step is rounded to fp32 by itself, in this order.
 //
-// A cluster of eight CTAs takes a row: each holds one eighth of the vocabulary as 32-bit counters in shared memory, goes through the
-// row's tokens and counts those that fall into its part, then streams its part of the logits once.  So the counts never touch
-// memory, the arg-max of the parts meets through distributed shared memory, and nothing has to be zero between launches.
-// Bound: HBM (a bf16 logit in, an fp32 one out, a bit of mask).
+// A cluster of eight CTAs takes a row: each holds one eighth of the vocabulary as counters in shared memory, goes through the row's
+// tokens and counts those that fall into its part, then streams its part of the logits once.  So the counts never touch memory, the
+// arg-max of the parts meets through distributed shared memory, and nothing has to be zero between launches.
+// Bound: HBM (a bf16 logit in, an fp32 one out, a bit of mask) for large batches, the chain of lengths, tokens, counters and logits
+// for small ones: a thread's first logits are requested before anything else, the tokens before their number is known.  Counters
+// of 16 bits (histories of up to 16383 tokens) let all CTAs of 64 rows of 151936 be there at once: 15.7 us without a rule (9 is
+// the copy rate's time for their bytes), 18 with an empty history, 23 with 4000 tokens each, and 2 more with 300 biases.
+// Built and slower: the history shared out over the cluster with remote counting (32 us for tokens as skewed as text's), the counted
+// tokens taken from a list behind the stream (one more pass over scattered logits, 26 to 32 us).
 #pragma once
 #include "ixb_common.cuh"
 
 namespace ixb {
 
-constexpr int kLgThreads = 512;
 constexpr int kLgCtas = 8;                             // of a cluster: one row
 constexpr uint32_t kLgMaxBins = 49152;                 // of a CTA: 192 KB
-// a counter: bit 31 seen in the prompt, bits 20 .. 30 one more than the index of the bias entry, bits 0 .. 19 times generated
-constexpr uint32_t kLgPrompt = 1u << 31, kLgCount = (1u << 20) - 1u;
-constexpr int kLgBiasShift = 20;
-constexpr int64_t kLgMaxBias = 2047, kLgMaxTokens = kLgCount;
+// A counter: the top bit for a token of the prompt, the next one for a token that a bias names, the others count how often it was
+// generated.  32-bit counters are for histories that 16-bit ones cannot count.
+template <class C>
+struct LgBits {
+    static constexpr uint32_t kPrompt = 1u << (8 * sizeof(C) - 1), kBias = kPrompt >> 1, kCount = kBias - 1u;
+};
+constexpr int64_t kLgMaxBias = 2047, kLgMaxTokens = (1 << 20) - 1, kLgShortTokens = 16383;
 
 struct LogitRules {
     const void *logits;
@@ -37,7 +44,7 @@ struct LogitRules {
     float *out;
     long long *token;                                  // null: no arg-max
     size_t pitch, out_pitch;                           // elements
-    uint32_t rows, vocab, slice, hist_len, hist_pitch, n_bias, words, mask_pitch, n_masks;
+    uint32_t rows, vocab, slice, hist_vec, hist_len, hist_pitch, n_bias, n_slots, mask_pitch, n_masks;       // n_slots: of the biases' table, a power of two
 };
 
 __device__ __forceinline__ unsigned long long lg_key(float x, uint32_t v)
@@ -47,113 +54,250 @@ __device__ __forceinline__ unsigned long long lg_key(float x, uint32_t v)
     return (unsigned long long)b << 32 | (0xffffffffu - v);
 }
 
-// a counter and what hangs on it: the logit after penalties and bias
-__device__ __forceinline__ float lg_apply(float x, uint32_t bin, float rep, float pres, float freq, const float *bias)
+// A table of the row's biases for the tokens of this CTA's part: open addressing, (token + 1, its last entry: number, then value)
+__device__ __forceinline__ void lg_put(uint2 *table, uint32_t mask, uint32_t token, uint32_t entry)
 {
-    const uint32_t c = bin & kLgCount;
-    if (c || bin & kLgPrompt) x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
-    x = __fsub_rn(x, __fmul_rn(freq, (float)c));
-    if (c) x = __fsub_rn(x, pres);
-    const uint32_t e = bin >> kLgBiasShift & 2047u;
-    if (e) x = __fadd_rn(x, bias[e - 1u]);
-    return x;
+    for (uint32_t at = token * 2654435761u >> 7 & mask;; at = (at + 1u) & mask) {          // (at most half full)
+        const uint32_t was = atomicCAS(&table[at].x, 0u, token + 1u);
+        if (was == 0u || was == token + 1u) {
+            atomicMax(&table[at].y, entry);
+            return;
+        }
+    }
+}
+__device__ __forceinline__ uint2 &lg_at(uint2 *table, uint32_t mask, uint32_t token)        // (it is there)
+{
+    uint32_t at = token * 2654435761u >> 7 & mask;
+    for (uint32_t i = 0; i < mask && table[at].x != token + 1u; ++i) at = (at + 1u) & mask;
+    return table[at];
+}
+// NaN if one of them is
+__device__ __forceinline__ float lg_max(float a, float b)
+{
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+    return m;
 }
 
-// grid: rows x 8, clusters of 8.  VEC: rows of logits, out and mask start on 16 bytes (mask: 4), eight logits at a time
-template <bool F32, bool VEC>
-__global__ void __cluster_dims__(kLgCtas, 1, 1) __launch_bounds__(kLgThreads, 2)
+// grid: rows x 8, clusters of 8, of 512 threads where that fills the chip once at most, else of 256.  VEC: rows of logits and out start on 16 bytes, eight logits at a time
+template <class C, bool F32, bool VEC, int kLgThreads>
+__global__ void __cluster_dims__(kLgCtas, 1, 1) __launch_bounds__(kLgThreads, 1024 / kLgThreads)
 k_logits(LogitRules s)
 {
-    extern __shared__ __align__(16) uint32_t lg_bins[];
+    using B = LgBits<C>;
+    extern __shared__ __align__(16) unsigned char lg_smem[];
+    C *bins = (C *)lg_smem;                            // [slice], then the biases' table
+    uint2 *table = (uint2 *)(bins + s.slice);
     __shared__ unsigned long long sm_key[kLgThreads / 32], sm_part[kLgCtas];
     const uint32_t tid = threadIdx.x, row = blockIdx.x / kLgCtas, me = blockIdx.x % kLgCtas;
     const uint32_t v0 = min(s.vocab, me * s.slice), v1 = min(s.vocab, v0 + s.slice), n = v1 - v0;
     asm volatile("griddepcontrol.launch_dependents;");
     if (s.token) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // (awaited before the first remote store)
-    const bool bins = s.history || s.n_bias;           // uniform
-    if (bins)
-        for (uint32_t i = 4u * tid; i < n; i += 4u * kLgThreads) *(uint4 *)(lg_bins + i) = make_uint4(0, 0, 0, 0);      // (slice: a multiple of 32)
+    const bool count = s.history || s.n_bias;          // uniform
+    constexpr uint32_t PV = 16 / sizeof(C);            // counters of 16 bytes
+    if (count) {
+        for (uint32_t i = PV * tid; i < n; i += PV * kLgThreads) *(uint4 *)(bins + i) = make_uint4(0, 0, 0, 0);      // (slice: a multiple of 32)
+        for (uint32_t i = tid; i < s.n_slots; i += kLgThreads) table[i] = make_uint2(0, 0);
+    }
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const float rep = s.repetition ? s.repetition[row] : 1.f, pres = s.presence ? s.presence[row] : 0.f,
-                freq = s.frequency ? s.frequency[row] : 0.f;
-    const float *bias = s.n_bias ? s.bias_values + (size_t)row * s.n_bias : nullptr;
-    if (bins) __syncthreads();
-    if (s.n_bias) {
-        for (uint32_t i = tid; i < s.n_bias; i += kLgThreads) {
-            const uint32_t id = (uint32_t)s.bias_ids[(size_t)row * s.n_bias + i] - v0;
-            if (id < n) atomicMax(lg_bins + id, (i + 1u) << kLgBiasShift);     // of several entries the last
-        }
-        __syncthreads();
-    }
-    if (s.history) {
-        const uint32_t len = min((uint32_t)max(s.n_tokens[row], 0), s.hist_len), np = s.n_prompt ? min((uint32_t)max(s.n_prompt[row], 0), len) : 0u;
-        const int32_t *h = s.history + (size_t)row * s.hist_pitch;
-        constexpr int UN = 8;                          // tokens of a thread in flight
-        for (uint32_t i0 = tid; i0 < len; i0 += UN * kLgThreads) {
-            uint32_t id[UN];
-#pragma unroll
-            for (int u = 0; u < UN; ++u) id[u] = i0 + u * kLgThreads < len ? (uint32_t)h[i0 + u * kLgThreads] - v0 : 0xffffffffu;
-#pragma unroll
-            for (int u = 0; u < UN; ++u)
-                if (id[u] < n) {                       // (also: numbers outside the vocabulary fall into no part)
-                    if (i0 + u * kLgThreads < np) atomicOr(lg_bins + id[u], kLgPrompt);
-                    else atomicAdd(lg_bins + id[u], 1u);
-                }
-        }
-    }
-    if (bins) __syncthreads();
-    const int32_t mr = !s.mask ? -1 : s.mask_row ? s.mask_row[row] : (int32_t)row;
-    const uint32_t *mask = mr >= 0 && (uint32_t)mr < s.n_masks ? s.mask + (size_t)mr * s.mask_pitch : nullptr;
     float *out = s.out + (size_t)row * s.out_pitch;
     const float *lf = (const float *)s.logits + (size_t)row * s.pitch;
     const __nv_bfloat16 *lb = (const __nv_bfloat16 *)s.logits + (size_t)row * s.pitch;
-    unsigned long long best = 0;
-    float top = -INFINITY;
-    uint32_t top_v = v0;                               // of this thread: the lowest of its largest
-    bool nan = false, any = false;
-    auto finish = [&](float x, uint32_t v, bool allowed) {
-        if (bins) {
-            const uint32_t bin = lg_bins[v - v0];
-            if (bin) x = lg_apply(x, bin, rep, pres, freq, bias);
-        }
-        if (!allowed) x = -INFINITY;
-        if (!nan && (x > top || x != x || !any)) {     // (a thread's indices ascend)
-            top = x;
-            top_v = v;
-            nan = x != x;
-            any = true;
-        }
-        return x;
-    };
+    constexpr int UN = F32 ? 2 : 4;                    // vectors of a thread in flight
     const uint32_t vec_end = VEC ? v0 + (n & ~7u) : v0;
-    if (VEC) {
-        for (uint32_t v = v0 + 8u * tid; v < vec_end; v += 8u * kLgThreads) {
-            float x[8];
+    uint4 raw[UN][F32 ? 2 : 1];
+    auto request = [&](uint32_t v) {
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            const uint32_t at = v + u * 8u * kLgThreads;
+            if (at >= vec_end) continue;
             if (F32) {
-                const float4 a = __ldcs((const float4 *)(lf + v)), b = __ldcs((const float4 *)(lf + v + 4));
-                x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+                raw[u][0] = __ldcs((const uint4 *)(lf + at));
+                raw[u][F32 ? 1 : 0] = __ldcs((const uint4 *)(lf + at + 4));
             } else {
-                const uint4 a = __ldcs((const uint4 *)(lb + v));
-                const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+                raw[u][0] = __ldcs((const uint4 *)(lb + at));
+            }
+        }
+    };
+    if (VEC) request(v0 + 8u * tid);
+    constexpr int HN = 4;                              // times four tokens of a thread in flight
+    int4 id[HN];
+    const int32_t *hist = s.history + (size_t)row * s.hist_pitch;
+    auto tokens = [&](uint32_t i0) {
+#pragma unroll
+        for (int u = 0; u < HN; ++u) {
+            const uint32_t i = i0 + u * 4u * kLgThreads;
+            if (s.hist_vec && i + 3u < s.hist_len) {
+                id[u] = *(const int4 *)(hist + i);
+            } else {
+                id[u].x = i < s.hist_len ? hist[i] : -1;
+                id[u].y = i + 1u < s.hist_len ? hist[i + 1] : -1;
+                id[u].z = i + 2u < s.hist_len ? hist[i + 2] : -1;
+                id[u].w = i + 3u < s.hist_len ? hist[i + 3] : -1;
+            }
+        }
+    };
+    uint32_t len = 0, np = 0;
+    if (s.history) {
+        tokens(4u * tid);
+        len = min((uint32_t)max(s.n_tokens[row], 0), s.hist_len);
+        np = s.n_prompt ? min((uint32_t)max(s.n_prompt[row], 0), len) : 0u;
+    }
+    const float rep = s.repetition ? s.repetition[row] : 1.f, pres = s.presence ? s.presence[row] : 0.f,
+                freq = s.frequency ? s.frequency[row] : 0.f;
+    constexpr int BN = 2;                              // biases of a thread that are requested ahead
+    const int32_t *bias_ids = s.bias_ids + (size_t)row * s.n_bias;
+    const float *bias_values = s.bias_values + (size_t)row * s.n_bias;
+    uint32_t b_id[BN];
+    float b_val[BN];
+#pragma unroll
+    for (int u = 0; u < BN; ++u) {
+        const uint32_t i = tid + u * kLgThreads;
+        b_id[u] = i < s.n_bias ? (uint32_t)bias_ids[i] - v0 : 0xffffffffu;
+        b_val[u] = i < s.n_bias ? bias_values[i] : 0.f;
+    }
+    const int32_t mr = !s.mask ? -1 : s.mask_row ? s.mask_row[row] : (int32_t)row;
+    const uint32_t *mask = mr >= 0 && (uint32_t)mr < s.n_masks ? s.mask + (size_t)mr * s.mask_pitch : nullptr;
+    auto mark = [&](uint32_t i, uint32_t bits, bool add) {             // in the word that holds counter i
+        uint32_t *word = (uint32_t *)bins + i * sizeof(C) / 4;
+        const uint32_t shift = sizeof(C) == 2 ? (i & 1u) * 16u : 0u;
+        if (add) atomicAdd(word, bits << shift);
+        else atomicOr(word, bits << shift);
+    };
+    if (count) __syncthreads();
+    auto biases = [&](auto &&what) {                   // this thread's biases for tokens of this part: (token, number of the thread's, entry, value)
+#pragma unroll
+        for (int u = 0; u < BN; ++u)
+            if (b_id[u] < n) what(b_id[u], (uint32_t)u, tid + u * kLgThreads, b_val[u]);
+        for (uint32_t u = BN; tid + u * kLgThreads < s.n_bias; ++u) {
+            const uint32_t b = (uint32_t)bias_ids[tid + u * kLgThreads] - v0;
+            if (b < n) what(b, u, tid + u * kLgThreads, bias_values[tid + u * kLgThreads]);
+        }
+    };
+    if (s.n_bias)
+        biases([&](uint32_t b, uint32_t, uint32_t i, float) {
+            mark(b, B::kBias, false);
+            lg_put(table, s.n_slots - 1u, b, i);
+        });
+    if (s.history) {
+        for (uint32_t i0 = 4u * tid; i0 < len; i0 += HN * 4u * kLgThreads) {
+            if (i0 != 4u * tid) tokens(i0);
+#pragma unroll
+            for (int u = 0; u < HN; ++u) {
+                const uint32_t i = i0 + u * 4u * kLgThreads;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    x[2 * j] = __uint_as_float(w[j] << 16);
-                    x[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+                    const uint32_t at = (uint32_t)(j == 0 ? id[u].x : j == 1 ? id[u].y : j == 2 ? id[u].z : id[u].w) - v0;
+                    if (at < n && i + j < len) {       // (numbers outside the vocabulary fall into no part)
+                        const bool made = i + j >= np;
+                        mark(at, made ? 1u : B::kPrompt, made);
+                    }
                 }
             }
-            const uint32_t bits = mask ? mask[v >> 5] >> (v & 31u) : 0xffu;    // (v: a multiple of 8)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = finish(x[j], v + j, bits >> j & 1u);
-            *(float4 *)(out + v) = make_float4(x[0], x[1], x[2], x[3]);
-            *(float4 *)(out + v + 4) = make_float4(x[4], x[5], x[6], x[7]);
         }
     }
-    for (uint32_t v = vec_end + tid; v < v1; v += kLgThreads) {
-        const float x = F32 ? lf[v] : __bfloat162float(lb[v]);
-        out[v] = finish(x, v, !mask || mask[v >> 5] >> (v & 31u) & 1u);
+    if (count) __syncthreads();
+    if (s.n_bias) {                                    // the last entries' values in the place of their numbers
+        uint32_t last = 0;                             // (at most eight of a thread)
+        biases([&](uint32_t b, uint32_t u, uint32_t i, float) { last |= (lg_at(table, s.n_slots - 1u, b).y == i ? 1u : 0u) << u; });
+        __syncthreads();
+        biases([&](uint32_t b, uint32_t u, uint32_t, float value) {
+            if (last >> u & 1u) lg_at(table, s.n_slots - 1u, b).y = __float_as_uint(value);
+        });
+        __syncthreads();
+    }
+    // the logit behind its counter
+    auto rules = [&](float x, uint32_t v, uint32_t bin) {
+        const uint32_t c = bin & B::kCount;
+        if (c || bin & B::kPrompt) x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
+        x = __fsub_rn(x, __fmul_rn(freq, (float)c));
+        if (c) x = __fsub_rn(x, pres);
+        if (bin & B::kBias) x = __fadd_rn(x, __uint_as_float(lg_at(table, s.n_slots - 1u, v - v0).y));
+        return x;
+    };
+    float top = -INFINITY;
+    const bool any = VEC && v0 + 8u * tid < vec_end ? true : vec_end + tid < v1;
+    uint32_t top_v = VEC && v0 + 8u * tid < vec_end ? v0 + 8u * tid : vec_end + tid;        // the lowest of the thread's largest (its indices ascend)
+    auto keep = [&](float x, uint32_t v) {
+        if (x > top || (x != x && top == top)) {
+            top = x;
+            top_v = v;
+        }
+    };
+    if (VEC) {
+        for (uint32_t va = v0 + 8u * tid; va < vec_end; va += UN * 8u * kLgThreads) {
+            if (va != v0 + 8u * tid) request(va);
+#pragma unroll
+            for (int u = 0; u < UN; ++u) {
+                const uint32_t v = va + u * 8u * kLgThreads;
+                if (v >= vec_end) break;
+                float x[8];
+                if (F32) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint4 r = raw[u][F32 ? h : 0];
+                        x[4 * h] = __uint_as_float(r.x); x[4 * h + 1] = __uint_as_float(r.y); x[4 * h + 2] = __uint_as_float(r.z); x[4 * h + 3] = __uint_as_float(r.w);
+                    }
+                } else {
+                    const uint32_t w[4] = {raw[u][0].x, raw[u][0].y, raw[u][0].z, raw[u][0].w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        x[2 * j] = __uint_as_float(w[j] << 16);
+                        x[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+                    }
+                }
+                if (count) {
+                    uint32_t c[4 * sizeof(C) / 2], some = 0;
+#pragma unroll
+                    for (int q = 0; q < (int)sizeof(C) / 2; ++q) {
+                        const uint4 r = *(const uint4 *)(bins + (v - v0) + q * 4);
+                        c[4 * q] = r.x; c[4 * q + 1] = r.y; c[4 * q + 2] = r.z; c[4 * q + 3] = r.w;
+                        some |= r.x | r.y | r.z | r.w;
+                    }
+                    if (some) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const uint32_t bin = sizeof(C) == 4 ? c[j % (4 * sizeof(C) / 2)] : j & 1 ? c[j / 2] >> 16 : c[j / 2] & 0xffffu;
+                            if (bin) x[j] = rules(x[j], v + j, bin);
+                        }
+                    }
+                }
+                if (mask) {
+                    const uint32_t bits = mask[v >> 5] >> (v & 31u);   // (v: a multiple of 8)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[j] = bits >> j & 1u ? x[j] : -INFINITY;
+                }
+                __stcs((float4 *)(out + v), make_float4(x[0], x[1], x[2], x[3]));
+                __stcs((float4 *)(out + v + 4), make_float4(x[4], x[5], x[6], x[7]));
+                const float m = lg_max(lg_max(lg_max(x[0], x[1]), lg_max(x[2], x[3])), lg_max(lg_max(x[4], x[5]), lg_max(x[6], x[7])));
+                if (!(m <= top)) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) keep(x[j], v + j);
+                }
+            }
+        }
+    }
+    constexpr int SN = 4;                              // single logits of a thread in flight
+    for (uint32_t va = vec_end + tid; va < v1; va += SN * kLgThreads) {
+        float x[SN];
+#pragma unroll
+        for (int u = 0; u < SN; ++u) {
+            const uint32_t v = min(va + u * kLgThreads, v1 - 1u);
+            x[u] = F32 ? lf[v] : __bfloat162float(lb[v]);
+        }
+#pragma unroll
+        for (int u = 0; u < SN; ++u) {
+            const uint32_t v = va + u * kLgThreads;
+            if (v >= v1) break;
+            const uint32_t bin = count ? bins[v - v0] : 0u;
+            if (bin) x[u] = rules(x[u], v, bin);
+            if (mask && !(mask[v >> 5] >> (v & 31u) & 1u)) x[u] = -INFINITY;
+            out[v] = x[u];
+            keep(x[u], v);
+        }
     }
     if (!s.token) return;                              // uniform
-    if (any) best = lg_key(top, top_v);
+    unsigned long long best = any ? lg_key(top, top_v) : 0ull;
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, d));
     if ((tid & 31u) == 0) sm_key[tid >> 5] = best;

@@ -206,13 +206,26 @@ extern "C" int ixb_attn_paged(const void *q, const void *k_pages, const void *v_
 }
 
 // ------------------------------------------------------------------------------------------------ rules on logits
-template <bool F32, bool VEC>
+template <class C, bool F32, bool VEC, int THREADS>
 static cudaError_t launch_logits(const LogitRules &s, cudaStream_t st)
 {
     static bool attr_set[64] = {false};
-    const cudaError_t e = opt_in_smem(k_logits<F32, VEC>, attr_set, (int)kLgMaxBins * 4);
+    const cudaError_t e = opt_in_smem(k_logits<C, F32, VEC, THREADS>, attr_set, 227 * 1024 - 1024);
     if (e != cudaSuccess) return e;
-    return launch_glue_smem(k_logits<F32, VEC>, dim3(s.rows * kLgCtas), dim3(kLgThreads), s.history || s.n_bias ? (size_t)s.slice * 4 : 0, st, s);
+    return launch_glue_smem(k_logits<C, F32, VEC, THREADS>, dim3(s.rows * kLgCtas), dim3(THREADS),
+                            s.history || s.n_bias ? s.slice * sizeof(C) + s.n_slots * 8u : 0, st, s);
+}
+template <class C, bool F32, bool VEC>
+static cudaError_t launch_logits(const LogitRules &s, cudaStream_t st)
+{
+    // 512 threads while the rows' CTAs fit the chip once, two an SM: fewer vectors a thread (one row of 73448: 7.1 us, 8.1 with 256)
+    return s.rows * kLgCtas <= 2u * num_sms() ? launch_logits<C, F32, VEC, 512>(s, st) : launch_logits<C, F32, VEC, 256>(s, st);
+}
+template <class C>
+static cudaError_t launch_logits(const LogitRules &s, bool f32, bool vec, cudaStream_t st)
+{
+    return f32 ? (vec ? launch_logits<C, true, true>(s, st) : launch_logits<C, true, false>(s, st))
+               : (vec ? launch_logits<C, false, true>(s, st) : launch_logits<C, false, false>(s, st));
 }
 
 extern "C" int ixb_logits(const void *logits, int logits_f32, int64_t pitch, const int32_t *history, int64_t hist_len, int64_t hist_pitch,
@@ -228,12 +241,13 @@ extern "C" int ixb_logits(const void *logits, int logits_f32, int64_t pitch, con
     if (hist_len > kLgMaxTokens || hist_pitch > 0x7fffffffll || n_bias < 0 || n_bias > kLgMaxBias || n_masks > 0x7fffffffll || mask_pitch > 0x7fffffffll)
         return fail(IXB_E_UNSUPPORTED, "at most %lld tokens and %lld biases a row", (long long)kLgMaxTokens, (long long)kLgMaxBias);
     LogitRules s = {logits, history, n_tokens, n_prompt, repetition, presence, frequency, bias_ids, bias_values, (const uint32_t *)mask, mask_row,
-                    out, (long long *)token, (size_t)pitch, (size_t)out_pitch, (uint32_t)rows, (uint32_t)vocab, 0, (uint32_t)hist_len,
-                    (uint32_t)hist_pitch, (uint32_t)n_bias, (uint32_t)((vocab + 31) / 32), (uint32_t)mask_pitch, (uint32_t)n_masks};
+                    out, (long long *)token, (size_t)pitch, (size_t)out_pitch, (uint32_t)rows, (uint32_t)vocab, 0, 0, (uint32_t)hist_len,
+                    (uint32_t)hist_pitch, (uint32_t)n_bias, 0, (uint32_t)mask_pitch, (uint32_t)n_masks};
+    for (uint32_t slots = 2; n_bias && s.n_slots < 2 * n_bias; slots *= 2) s.n_slots = slots;      // the table stays at most half full
     s.slice = (uint32_t)((vocab + 32 * kLgCtas - 1) / (32 * kLgCtas) * 32);
     if (s.slice > kLgMaxBins) return fail(IXB_E_UNSUPPORTED, "vocabulary of %lld is too large", (long long)vocab);
+    s.hist_vec = ((uintptr_t)history & 15u) == 0 && (rows == 1 || (hist_pitch & 3) == 0);
     const cudaStream_t st = (cudaStream_t)stream;
     const bool vec = (((uintptr_t)logits | (uintptr_t)out) & 15u) == 0 && (rows == 1 || ((pitch & (logits_f32 ? 3 : 7)) == 0 && (out_pitch & 3) == 0));
-    IXB_GLUE("k_logits", logits_f32 ? (vec ? launch_logits<true, true>(s, st) : launch_logits<true, false>(s, st))
-                                    : (vec ? launch_logits<false, true>(s, st) : launch_logits<false, false>(s, st)));
+    IXB_GLUE("k_logits", hist_len > kLgShortTokens ? launch_logits<uint32_t>(s, logits_f32, vec, st) : launch_logits<uint16_t>(s, logits_f32, vec, st));
 }

@@ -173,3 +173,13 @@ def test_refusals():
         apply_rules(s["logits"][:0])
     with pytest.raises(_lib.IxbError):
         apply_rules(torch.zeros(1, 400000, device=DEV))
+
+
+@pytest.mark.parametrize("b,v,length,f32", [(3, 20000, 1537, False), (2, 151936, 9000, True), (5, 65, 3000, False), (1, 300000, 16384, False), (2, 999, 16383, True)])
+def test_long_histories(b, v, length, f32):
+    """histories that the parts of a row share among themselves, and those that 16 bits do not count"""
+    s = inputs(v + length, b, v, length, 7, 0, f32=f32)
+    s["history"][:, length // 2:] = v - 1              # one token more often than 13 bits hold, for the longest
+    s["n_tokens"].fill_(length)
+    s["n_prompt"].fill_(length // 3)
+    check(s)
