@@ -3,25 +3,27 @@
 //   row (t, g) of request r and KV head h: new token t < q_len[r], query head h * G + g, position length[r] - q_len[r] + t
 //   out = softmax(scale * q . K[0 .. position]) V[0 .. position]
 //
-// A request's rows of one KV head are packed, row t * G + g, sixteen to a group (the M of mma.sync), so a key is read once for all
-// of them.  Bound: HBM, every key and value once; mma.sync is used as an instruction that multiplies sixteen rows at a time, at a
-// fifth of its rate.
+// A request's rows of one KV head are packed, row t * G + g, eight or sixteen to a group, so a key is read once for all of them.
+// Bound: HBM, every key and value once; mma.sync is used as an instruction that multiplies eight rows at a time: keys (or
+// dimensions of values) are its M = 16, rows its N = 8, S^T = K Q^T and O^T = V^T P^T, so that a single token of a group of up to
+// eight heads wastes none of it and its sums take half the registers of rows as M.
 //
-// Work: all (KV head, request, row group) pairs' blocks of keys (16 per warp of a CTA) in one line, cut into equal ranges, one per
-// CTA, so lengths that differ cost nothing.  A warp takes its 16 keys of every block through its own ring of TMA stages (a box is 16
-// positions of a page and 64 dimensions, 128-byte swizzle) and keeps a running softmax of its own, so no barrier lies in the loop;
-// the warps' sums meet in shared memory where a pair ends.  A pair that is cut leaves its parts in the scratch, and the CTA that comes
-// last (a ticket) joins them in the order of the keys: the same bits every time.
+// Work: all (KV head, request, row group) pairs' blocks of keys in one line, cut into equal ranges, one per CTA, so lengths that differ
+// cost nothing.  A block is a slice of 16 keys per warp (32 with heads of 64, where a slice's softmax would take longer than its
+// bytes).  One warp asks for the blocks (TMA, a box per page and 64 dimensions, 128-byte swizzle) in a ring of stages K, V, K, .., across
+// pairs; eight warps take their slices and keep a running softmax each, so they meet only where a pair ends, in shared memory.  A
+// pair that is cut leaves its parts in the scratch, and the CTA that comes last (a ticket) joins them in the order of the keys: the
+// same bits every time.
 //
 // Precision: q K^T bf16 x bf16 in fp32; probabilities as two bf16 numbers whose sum they are to 17 bits; a slice's P V starts from
 // zero and joins the running sums by fp32 fused multiply-adds (the tensor core cuts low bits of what it adds to a large sum).
 //
 // Keys at and behind length are masked and their values taken as zeros, whatever lies there; a page number outside the pool is a
 // page of zeros (the copy's fill).  A value that is not finite counts for the rows that see it and for no other: it shows in the
-// sums of every row (zero times infinity is NaN), and the pair's blocks are then gone through again, slices that hold one token by
-// token.
+// sums of every row (zero times infinity is NaN), and the pair's blocks are then gone through again, straight from memory and token
+// by token.
 //
-// Every wait on an mbarrier is bounded and counts the warp's own copies; where one runs out the CTA's outputs become NaN.
+// Every wait on an mbarrier is bounded and counts the CTA's own copies; where one runs out the CTA's outputs become NaN.
 #pragma once
 #include "ixb_common.cuh"
 #include <cuda.h>
@@ -72,6 +74,13 @@ __device__ __forceinline__ void pa_ldmt(uint32_t (&r)[4], uint32_t addr)
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
+// an 8 x 8 matrix of bf16 numbers transposed
+__device__ __forceinline__ uint32_t pa_turn(uint32_t x)
+{
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
 __device__ __forceinline__ uint32_t pa_pack(float lo, float hi)
 {
     const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
@@ -81,21 +90,28 @@ __device__ __forceinline__ uint32_t pa_pack(float lo, float hi)
 __device__ __forceinline__ uint32_t pa_larger(uint32_t m, uint32_t x) { return __vmaxu2(m, x & 0x7fff7fffu); }
 __device__ __forceinline__ bool pa_wild(uint32_t m) { return (m & 0xffffu) >= 0x7f80u || m >= 0x7f800000u; }
 
+constexpr uint32_t kPaMaxRequests = 4096;
+constexpr uint32_t kPaMaxCtas = 160;                   // one per SM
+
 template <int D>
 struct PaCfg {
-    static constexpr int kWarps = D == 256 ? 4 : 8, kThreads = kWarps * 32;
-    static constexpr int kKeys = 16 * kWarps;          // of a block
-    static constexpr uint32_t kHalf = 16 * D * 2;      // K or V of a warp's slice: [64 dimensions][16 keys] of 128 bytes
-    static constexpr uint32_t kStage = 2 * kHalf;
-    static constexpr int kStages = D == 64 ? 6 : 3;
-    static constexpr uint32_t kRing = kWarps * kStages * kStage;
-    static constexpr int kPitch = D + 8;               // floats of a row in the warps' sums, (maximum, denominator) at D: 8-byte stores without conflicts
-    static constexpr uint32_t kSum = kWarps * 8 * kPitch * 4;
-    static constexpr uint32_t kSmem = kRing + kSum + kWarps * kStages * 8 + kWarps * 4 + 16;       // (no static arrays: the ring starts on 1024 bytes)
+    static constexpr int kWarps = 8;                   // that compute; one of four more asks for the blocks
+    static constexpr int kThreads = 384, kCompute = kWarps * 32;
+    static constexpr int kSub = D == 64 ? 2 : 1;       // times 16 keys of a warp's slice
+    static constexpr int kSlice = 16 * kSub;
+    static constexpr int kKeys = kSlice * kWarps;      // of a block
+    static constexpr uint32_t kPanel = 128 * 128;      // 64 dimensions of 128 keys: rows of 128 bytes
+    static constexpr uint32_t kStage = D / 64 * kSub * kPanel;     // K or V of a block: [128 keys][64 dimensions]
+    static constexpr int kStages = 196608 / kStage;
+    static constexpr uint32_t kRing = kStages * kStage;
+    static constexpr int kSumD = D < 128 ? D : 128;    // dimensions that the warps' sums are joined at a time
+    static constexpr int kPitch = kSumD + 4;           // floats of a row there, (maximum, denominator) at kSumD: stores without conflicts
+    static constexpr uint32_t kSumBytes = kWarps * 8 * kPitch * 4, kJoinBytes = kPaMaxCtas * 16 * 8;
+    static constexpr uint32_t kSum = kSumBytes > kJoinBytes ? kSumBytes : kJoinBytes;
+    static constexpr uint32_t kSmem = kRing + kSum + 2 * kStages * 8 + 64;     // (no static arrays: the ring starts on 1024 bytes)
     static constexpr uint32_t kSlot = 16 * D + 32;     // floats of a part: sums [16][D], (maximum, denominator) [16]
-    static_assert(kSmem <= 227 * 1024 && kHalf % 1024 == 0, "fits");
+    static_assert(kSmem <= 227 * 1024 && kSum >= 4 * kPaMaxRequests, "fits");
 };
-constexpr uint32_t kPaMaxRequests = 4096;
 
 constexpr uint32_t kPaWaitLimit = 1u << 20;            // polls
 __device__ __forceinline__ bool pa_wait(uint32_t mbar, uint32_t parity)
@@ -116,41 +132,89 @@ __device__ __forceinline__ float pa_exp2(float x)
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// one box of a pool's page: `keys` positions (the map's) from `row` on, 64 dimensions from d0 on, of KV head h
+__device__ __forceinline__ void pa_box(uint32_t dst, const CUtensorMap *map, uint32_t d0, uint32_t h, uint32_t row, int32_t page, uint32_t mbar)
+{
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                 :: "r"(dst), "l"(map), "r"(d0), "r"(h), "r"(row), "r"(page), "r"(mbar) : "memory");
+}
 
-template <int D>
+// the CTA's way through its pairs: blocks b0 .. b1 - 1 of row group rg of request r's rows of KV head h
+template <int D, int NT>
+struct PaWalk {
+    static constexpr uint32_t kRows = 8u * NT;         // of a group
+    PagedReq rq;
+    uint32_t r, h, rg, kb, b0, b1;                     // kb: blocks of the pair
+    unsigned long long x, x_end;                       // blocks of all pairs before block b0, and where the CTA's range ends
+    __device__ __forceinline__ static bool mine(const PagedAttn &a, const PagedReq &q) { return q.n * a.group > a.row_lo && q.n * a.group <= a.row_hi; }
+    __device__ __forceinline__ static uint32_t key_blocks(const PagedReq &q) { return max(1u, (q.len + PaCfg<D>::kKeys - 1) / PaCfg<D>::kKeys); }
+    __device__ __forceinline__ void cut() { b1 = (uint32_t)min((unsigned long long)kb, b0 + (x_end - x)); }
+    __device__ __forceinline__ uint32_t after(const PagedAttn &a) const { return r + 1u == a.requests ? 0u : r + 1u; }
+    // the next pair; ahead: what the next request has (requested earlier); false: there is none
+    __device__ __forceinline__ bool next(const PagedAttn &a, const PagedReq &ahead)
+    {
+        x += b1 - b0;
+        if (x >= x_end) return false;
+        if (++rg * kRows >= rq.n * a.group) {
+            rg = 0;
+            rq = ahead;
+            if (++r == a.requests) {
+                r = 0;
+                ++h;
+            }
+            while (!mine(a, rq) && h < a.hkv) {        // (there is one, unless the lengths change under the kernel)
+                if (++r == a.requests) {
+                    r = 0;
+                    ++h;
+                }
+                rq = paged_req(a, r);
+            }
+            if (h >= a.hkv) return false;
+            kb = key_blocks(rq);
+        }
+        b0 = 0;
+        cut();
+        return true;
+    }
+};
+
+// NT: times eight rows of a group
+template <int D, int NT>
 __global__ void __launch_bounds__(PaCfg<D>::kThreads, 1)
 k_attn_paged(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap)
 {
     using CF = PaCfg<D>;
-    constexpr int NW = CF::kWarps, ST = CF::kStages;
+    constexpr int NW = CF::kWarps, ST = CF::kStages, SUB = CF::kSub;
     extern __shared__ __align__(1024) unsigned char pa_smem[];
-    uint64_t *sm_bar = (uint64_t *)(pa_smem + CF::kRing + CF::kSum);           // [NW][ST], then:
-    uint32_t *sm_warp = (uint32_t *)(sm_bar + NW * ST), &sm_last = sm_warp[NW];
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(pa_smem), full0 = ring + CF::kRing + CF::kSum, empty0 = full0 + 8u * ST;
+    uint32_t *sm_warp = (uint32_t *)(pa_smem + CF::kRing + CF::kSum + 16 * ST), &sm_last = sm_warp[CF::kThreads / 32];
     const uint32_t tid = threadIdx.x, lane = tid & 31u, wid = __shfl_sync(0xffffffffu, tid >> 5, 0), g = lane >> 2, t = lane & 3u;
-    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(pa_smem) + wid * ST * CF::kStage;
     float *sum = (float *)(pa_smem + CF::kRing);       // [NW][8][kPitch]; before that the blocks before every request
     uint32_t *first = (uint32_t *)sum;
-    static_assert(CF::kSum >= 4 * kPaMaxRequests && CF::kRing >= 256 * 16 * 8, "fits");       // (parts of a pair: at most a CTA each)
     const uint32_t R = a.requests, G = a.group, page = 1u << a.log_page;
-    const uint32_t bar0 = (uint32_t)__cvta_generic_to_shared(sm_bar) + wid * ST * 8u;
     asm volatile("griddepcontrol.launch_dependents;");
-    if (lane == 0) {
-        for (int i = 0; i < ST; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar0 + 8u * i) : "memory");
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
     if (tid == 0) {
+        for (int i = 0; i < ST; ++i) {
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(full0 + 8u * i) : "memory");
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(empty0 + 8u * i), "r"(NW) : "memory");
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    auto key_blocks = [&](const PagedReq &q) { return max(1u, (q.len + CF::kKeys - 1) / CF::kKeys); };
-    auto mine = [&](const PagedReq &q) { return q.n * G > a.row_lo && q.n * G <= a.row_hi; };
-    auto blocks = [&](const PagedReq &q) { return mine(q) ? (q.n * G + 15u) / 16u * key_blocks(q) : 0u; };
     // ---- the blocks before every request, of one KV head
-    const uint32_t per = (R + CF::kThreads - 1) / CF::kThreads, ra = min(R, tid * per), rb = min(R, ra + per);
-    uint32_t before = 0, total = 0;
-    {
-        uint32_t own = 0;
+    uint32_t total = 0;
+    using Walk = PaWalk<D, NT>;
+    Walk s;
+    auto blocks = [&](const PagedReq &q) { return Walk::mine(a, q) ? (q.n * G + Walk::kRows - 1u) / Walk::kRows * Walk::key_blocks(q) : 0u; };
+    if (R == 1u) {
+        s.rq = paged_req(a, 0u);
+        total = blocks(s.rq);
+        __syncthreads();
+    } else {
+        const uint32_t per = (R + CF::kThreads - 1) / CF::kThreads, ra = min(R, tid * per), rb = min(R, ra + per);
+        uint32_t before = 0, own = 0;
         for (uint32_t r = ra; r < rb; ++r) {
             first[r] = own;
             own += blocks(paged_req(a, r));
@@ -164,7 +228,7 @@ k_attn_paged(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
         if (lane == 31u) sm_warp[wid] = v;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
+        for (int w = 0; w < CF::kThreads / 32; ++w) {
             if ((uint32_t)w < wid) before += sm_warp[w];
             total += sm_warp[w];
         }
@@ -175,263 +239,381 @@ k_attn_paged(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
     const unsigned long long W = (unsigned long long)total * a.hkv;
     const uint32_t N = (uint32_t)min((unsigned long long)gridDim.x, W), me = blockIdx.x;
     if (me >= N) return;
-    unsigned long long x = W * me / N;
-    const unsigned long long x_end = W * (me + 1ull) / N, x_begin = x;
-    uint32_t h = (uint32_t)(x / total), off = (uint32_t)(x - (unsigned long long)h * total), r;
-    {                                                  // the request of the first block: the last one with first[r] <= off
-        uint32_t lo = 0, hi = R;
-        while (hi - lo > 1u) {
-            const uint32_t mid = (lo + hi) / 2u;
-            if (first[mid] <= off) lo = mid;
-            else hi = mid;
+    auto part_of = [&](uint32_t c) { return W < 1u << 24 ? (unsigned long long)((uint32_t)W * c / N) : W * c / N; };     // (N at most 256)
+    auto cta_of = [&](unsigned long long y) {          // the last c with part_of(c) <= y
+        return W < 1u << 24 ? (((uint32_t)y + 1u) * N - 1u) / (uint32_t)W : (uint32_t)(((y + 1ull) * N - 1ull) / W);
+    };
+    s.x = part_of(me);
+    s.x_end = part_of(me + 1u);
+    const unsigned long long x_begin = s.x;
+    {
+        s.h = W < 1u << 24 ? (uint32_t)s.x / total : (uint32_t)(s.x / total);
+        uint32_t off = (uint32_t)(s.x - (unsigned long long)s.h * total), lo = 0;
+        if (R > 1u) {                                  // the request of the first block: the last one with first[r] <= off
+            uint32_t hi = R;
+            while (hi - lo > 1u) {
+                const uint32_t mid = (lo + hi) / 2u;
+                if (first[mid] <= off) lo = mid;
+                else hi = mid;
+            }
+            off -= first[lo];
+            s.rq = paged_req(a, lo);
         }
-        r = lo;
-        off -= first[r];
+        s.r = lo;
+        s.kb = Walk::key_blocks(s.rq);
+        s.rg = off / s.kb;
+        s.b0 = off - s.rg * s.kb;
+        s.cut();
     }
-    PagedReq rq = paged_req(a, r);
-    uint32_t kb = key_blocks(rq), rg = off / kb, b0 = off - rg * kb;           // key blocks, row group, first block
-    const float sl2 = a.scale * 1.4426950408889634f;   // scores in units of log2
-    uint32_t n = 0;                                    // stages asked for so far
     bool ok = true;
-    for (;;) {
-        // ---- blocks b0 .. b1 - 1 of row group rg of request r, KV head h
-        const uint32_t b1 = (uint32_t)min((unsigned long long)kb, b0 + (x_end - x));
-        const uint32_t rows = min(16u, rq.n * G - rg * 16u);
-        const int32_t *pages = a.table + (size_t)r * a.width;
-        int32_t page_l = -1;                           // lane l: the page of the warp's slice of block b0 + 32 i + l
-        uint32_t page_at = 0xffffffffu;
-        auto fetch = [&](uint32_t b) {                 // the warp's slice of block b into the next stage
-            const uint32_t key0 = (b * NW + wid) * 16u;
-            if (b >= b1 || key0 >= rq.len) return;     // uniform
-            const uint32_t win = (b - b0) & ~31u;
-            if (win != page_at) {
-                page_at = win;
-                const uint32_t key_l = ((b0 + win + lane) * NW + wid) * 16u;
-                page_l = key_l < rq.len ? pages[key_l >> a.log_page] : -1;
-            }
-            const int32_t p = __shfl_sync(0xffffffffu, page_l, (int)((b - b0) & 31u));
-            const uint32_t st = n % ST, bar = bar0 + 8u * st, dst = ring + st * CF::kStage;
-            ++n;
-            if (lane == 0) {
-                asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(bar), "r"(CF::kStage) : "memory");
+    if (wid >= (uint32_t)NW) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        if (wid > (uint32_t)NW) return;
+        // ---- the warp that asks for K and V of every block: boxes of (at most 128) positions of a page
+        const uint32_t bp = min(page, 128u), boxes = CF::kKeys / bp * (D / 64), bk = lane / (D / 64), panel = lane % (D / 64);
+        // (of lane < boxes, at most 32: positions bk * bp .. of a block and 64 dimensions; with D = 256 and pages of 16 a lane has just one)
+        static_assert(CF::kKeys / 16 * (D / 64) <= 32, "a box per lane");
+        const uint32_t dst = (bk * bp / 128u * (D / 64) + panel) * CF::kPanel + bk * bp % 128u * 128u;
+        uint32_t n = 0;
+        bool more = true;
+        while (more && ok) {
+            const int32_t *pages = a.table + (size_t)s.r * a.width;
+            const PagedReq ahead = paged_req(a, s.after(a));
+            auto page_of = [&](uint32_t b) {
+                const uint32_t key = b * CF::kKeys + bk * bp;
+                return lane < boxes && b < s.b1 && key < s.rq.len ? pages[key >> a.log_page] : 0;
+            };
+            int32_t p = page_of(s.b0);
+            for (uint32_t b = s.b0; b < s.b1 && ok; ++b) {
+                const uint32_t key = b * CF::kKeys + bk * bp;
+                const bool on = lane < boxes && key < s.rq.len;
+                const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, on)) * bp * 128u;
+                const int32_t p_next = page_of(b + 1u);
 #pragma unroll
-                for (uint32_t i = 0; i < 2 * D / 64; ++i)
-                    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
-                                 :: "r"(dst + i * 2048u), "l"(i < D / 64 ? &kmap : &vmap), "r"(i % (D / 64) * 64u), "r"(h), "r"(key0 & (page - 1u)), "r"(p), "r"(bar)
-                                 : "memory");
-            }
-            __syncwarp();
-        };
-        // the rows as A operands: row rg * 16 + m is token (..) / G, head (..) % G
-        uint32_t qf[D / 16][4];
-        int32_t limit[2];                              // the last position that the lane's rows g and g + 8 see
-        const uint32_t tok0 = rg * 16u / G, tok1 = (rg * 16u + rows - 1u) / G;         // the group's tokens
-        const int32_t len1 = (int32_t)rq.len - 1, all_see = min(rq.pos0 + (int32_t)tok0, len1);
-        float o[D / 8][4], m_[2], l_[2];
-        for (bool careful = false;; careful = true) {
-        uint32_t take = n;                             // the stage that comes next
-#pragma unroll
-        for (int i = 0; i < ST; ++i) fetch(b0 + i);
-        if (!careful) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint32_t m = rg * 16u + g + 8u * i, tok = m / G, gi = m - tok * G;
-                const bool on = g + 8u * i < rows;
-                limit[i] = on ? min(rq.pos0 + (int32_t)tok, len1) : -1;
-                const uint32_t *src = (const uint32_t *)(a.q + (size_t)(rq.row0 + (on ? tok : 0u)) * a.q_stride + ((size_t)h * G + (on ? gi : 0u)) * D) + t;
-#pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk) {
-                    qf[kk][i] = on ? src[kk * 8] : 0u;
-                    qf[kk][i + 2] = on ? src[kk * 8 + 4] : 0u;
+                for (int i = 0; i < 2; ++i, ++n) {
+                    const uint32_t st = n % ST, bar = full0 + 8u * st;
+                    ok = ok && pa_wait(empty0 + 8u * st, (n / ST & 1u) ^ 1u);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    if (lane == 0) asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(bar), "r"(bytes) : "memory");
+                    __syncwarp();
+                    if (on) pa_box(ring + st * CF::kStage + dst, i ? &vmap : &kmap, panel * 64u, s.h, key & (page - 1u), p, bar);
+                    __syncwarp();
                 }
+                p = p_next;
             }
+            more = s.next(a, ahead);
         }
-        m_[0] = m_[1] = -INFINITY;                     // of the raw scores
-        l_[0] = l_[1] = 0.f;
+        for (uint32_t i = n > (uint32_t)ST ? n - ST : 0u; i < n; ++i) pa_wait(full0 + 8u * (i % ST), i / ST & 1u);        // nothing is in flight behind the end
+        return;
+    }
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    const float sl2 = a.scale * 1.4426950408889634f;   // scores in units of log2
+    uint32_t take = 0;                                 // stages taken so far
+    auto landed = [&]() {                              // the next stage's slice, as an address
+        const uint32_t st = take % ST;
+        ok = ok && pa_wait(full0 + 8u * st, take / ST & 1u);
+        ok = __all_sync(0xffffffffu, ok);
+        return ring + st * CF::kStage + wid * CF::kSlice / 128u * (D / 64) * CF::kPanel + wid * CF::kSlice % 128u * 128u;
+    };
+    auto taken = [&]() {
+        __syncwarp();
+        if (lane == 0) asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.shared::cta.b64 st, [%0];\n\t}" ::"r"(empty0 + 8u * (take % ST)) : "memory");
+        ++take;
+    };
+    uint32_t qf[NT][D / 16][2];                        // the rows as B operands: row rg * kRows + m is token (..) / G, head (..) % G
+    int32_t limit[NT][2];                              // the last position that the lane's rows 8 nt + 2 t, + 1 see
+    auto rows_in = [&]() {
 #pragma unroll
-        for (int d = 0; d < D / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
-        for (uint32_t b = b0; b < b1; ++b) {
-            const int32_t key0 = (int32_t)((b * NW + wid) * 16u);
-            if ((uint32_t)key0 >= rq.len) break;       // uniform
-            const uint32_t st = take % ST, sk = ring + st * CF::kStage, sv = sk + CF::kHalf;
-            ok = ok && pa_wait(bar0 + 8u * st, take / ST & 1u);
-            ok = __all_sync(0xffffffffu, ok);
-            ++take;
-            float s[2][4];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+        for (int nt = 0; nt < NT; ++nt) {
+            const uint32_t m = s.rg * Walk::kRows + nt * 8u + g, tok = m / G, gi = m - tok * G;
+            const bool on = m < s.rq.n * G;
+            const uint32_t *src = (const uint32_t *)(a.q + (size_t)(s.rq.row0 + (on ? tok : 0u)) * a.q_stride + ((size_t)s.h * G + (on ? gi : 0u)) * D) + t;
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) {
-                uint32_t bk[4];                        // keys 0 .. 15, dimensions 16 kk .. + 15
-                const uint32_t rr = (lane & 7u) + (lane >> 4) * 8u, cc = 2u * kk + ((lane >> 3) & 1u);
-                pa_ldm(bk, sk + (cc >> 3) * 2048u + rr * 128u + ((cc ^ rr) & 7u) * 16u);
-                pa_mma(s[0], qf[kk], bk[0], bk[1]);
-                pa_mma(s[1], qf[kk], bk[2], bk[3]);
+                qf[nt][kk][0] = on ? src[kk * 8] : 0u;
+                qf[nt][kk][1] = on ? src[kk * 8 + 4] : 0u;
             }
-            if (key0 + 15 > all_see) {                 // uniform: not every row sees every key
-#pragma unroll
-                for (int c = 0; c < 2; ++c)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (key0 + c * 8 + 2 * (int32_t)t + (i & 1) > limit[i >> 1]) s[c][i] = -INFINITY;
-            }
-            float corr[2], base[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                float mx = fmaxf(fmaxf(s[0][2 * i], s[0][2 * i + 1]), fmaxf(s[1][2 * i], s[1][2 * i + 1]));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                const float mn = fmaxf(m_[i], mx);
-                base[i] = mn == -INFINITY ? 0.f : mn * sl2;            // nothing so far: sums stay zero
-                corr[i] = pa_exp2(fmaf(m_[i], sl2, -base[i]));
-                m_[i] = mn;
-                l_[i] *= corr[i];
+                const uint32_t q = s.rg * Walk::kRows + nt * 8u + 2u * t + i;
+                limit[nt][i] = q < s.rq.n * G ? min(s.rq.pos0 + (int32_t)(q / G), (int32_t)s.rq.len - 1) : -1;
             }
-            uint32_t ph[4], pl[4];                     // probabilities as A operands, leading and trailing bits
+        }
+    };
+    rows_in();
+    bool more = true;
+    while (more) {
+        const uint32_t rows = min(Walk::kRows, s.rq.n * G - s.rg * Walk::kRows);
+        const int32_t len1 = (int32_t)s.rq.len - 1, all_see = min(s.rq.pos0 + (int32_t)(s.rg * Walk::kRows / G), len1);
+        const PagedReq ahead = paged_req(a, s.after(a));               // (requested here, needed where the pair ends)
+        // sums: dimensions 16 d + g (+ 8 for elements 2 and 3) of rows 8 nt + 2 t (+ 1 for odd elements); maxima of the raw scores
+        float o[NT][D / 16][4], m_[NT][2], l_[NT][2];
+        auto zero = [&]() {
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
+            for (int nt = 0; nt < NT; ++nt) {
+                m_[nt][0] = m_[nt][1] = -INFINITY;
+                l_[nt][0] = l_[nt][1] = 0.f;
+#pragma unroll
+                for (int d = 0; d < D / 16; ++d) o[nt][d][0] = o[nt][d][1] = o[nt][d][2] = o[nt][d][3] = 0.f;
+            }
+        };
+        zero();
+        // scores of a slice (keys 16 u + g, + 8) into probabilities, as B operands of leading and trailing bits; corr: what the sums
+        // so far shrink by
+        auto softmax = [&](float (&sc)[NT][SUB][4], int32_t key0, uint32_t (&ph)[NT][SUB][2], uint32_t (&pl)[NT][SUB][2], float (&corr)[NT][2]) {
+            const bool mask = key0 + CF::kSlice - 1 > all_see;         // uniform: not every row sees every key
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                if (mask) {
+#pragma unroll
+                    for (int u = 0; u < SUB; ++u)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (key0 + u * 16 + (int32_t)g + 8 * (i >> 1) > limit[nt][i & 1]) sc[nt][u][i] = -INFINITY;
+                }
+                float base[2];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const float p0 = pa_exp2(fmaf(s[c][2 * i], sl2, -base[i])), p1 = pa_exp2(fmaf(s[c][2 * i + 1], sl2, -base[i]));
-                    l_[i] += p0 + p1;
-                    const uint32_t hi = pa_pack(p0, p1);
-                    ph[2 * c + i] = hi;
-                    pl[2 * c + i] = pa_pack(p0 - __uint_as_float(hi << 16), p1 - __uint_as_float(hi & 0xffff0000u));
+                    float mx = fmaxf(sc[nt][0][i], sc[nt][0][i + 2]);
+                    if (SUB == 2) mx = fmaxf(mx, fmaxf(sc[nt][SUB - 1][i], sc[nt][SUB - 1][i + 2]));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                    const float mn = fmaxf(m_[nt][i], mx);
+                    base[i] = mn == -INFINITY ? 0.f : mn * sl2;        // nothing so far: sums stay zero
+                    corr[nt][i] = pa_exp2(fmaf(m_[nt][i], sl2, -base[i]));
+                    m_[nt][i] = mn;
+                    l_[nt][i] *= corr[nt][i];
                 }
-            const uint32_t vrow = lane & 15u, vaddr = sv + vrow * 128u;
-            auto values = [&](uint32_t (&bv)[4], int d2) {             // keys 0 .. 15, dimensions 16 d2 .. + 15
-                const uint32_t cc = 2u * d2 + (lane >> 4);
-                pa_ldmt(bv, vaddr + (cc >> 3) * 2048u + ((cc ^ vrow) & 7u) * 16u);
-            };
-            auto cut = [&](uint32_t (&bv)[4], int32_t last) {          // without the values behind position `last`
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {          // keys 2 t, 2 t + 1 (+ 8 for odd i)
-                    const int32_t key = key0 + 2 * (int32_t)t + 8 * (i & 1);
-                    bv[i] &= key > last ? 0u : key + 1 > last ? 0xffffu : 0xffffffffu;
-                }
-            };
-            const bool tail = key0 + 15 > len1;        // uniform
-            bool wild = false;
-            if (careful) {
-                uint32_t big = 0;
-#pragma unroll 1
-                for (int d2 = 0; d2 < D / 16; ++d2) {
-                    uint32_t bv[4];
-                    values(bv, d2);
-                    cut(bv, len1);
+                for (int u = 0; u < SUB; ++u)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) big = pa_larger(big, bv[i]);
-                }
-                wild = __any_sync(0xffffffffu, pa_wild(big));
-            }
-            if (!wild) {
-#pragma unroll
-                for (int d2 = 0; d2 < D / 16; ++d2) {
-                    uint32_t bv[4];
-                    values(bv, d2);
-                    if (tail) cut(bv, len1);
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        float w[4] = {0.f, 0.f, 0.f, 0.f};
-                        pa_mma(w, pl, bv[2 * c], bv[2 * c + 1]);
-                        pa_mma(w, ph, bv[2 * c], bv[2 * c + 1]);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) o[2 * d2 + c][i] = fmaf(o[2 * d2 + c][i], corr[i >> 1], w[i]);
+                    for (int h = 0; h < 2; ++h) {      // keys g, g + 8
+                        const float p0 = pa_exp2(fmaf(sc[nt][u][2 * h], sl2, -base[0])), p1 = pa_exp2(fmaf(sc[nt][u][2 * h + 1], sl2, -base[1]));
+                        l_[nt][0] += p0;
+                        l_[nt][1] += p1;
+                        const uint32_t hi = pa_pack(p0, p1);
+                        ph[nt][u][h] = pa_turn(hi);
+                        pl[nt][u][h] = pa_turn(pa_pack(p0 - __uint_as_float(hi << 16), p1 - __uint_as_float(hi & 0xffff0000u)));
                     }
+            }
+        };
+        for (uint32_t b = s.b0; b < s.b1; ++b) {
+            const int32_t key0 = (int32_t)(b * CF::kKeys + wid * CF::kSlice);
+            const uint32_t sk = landed();
+            if (key0 > len1) {                         // uniform: nothing for this warp
+                taken();
+                landed();
+                taken();
+                continue;
+            }
+            float sc[NT][SUB][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int u = 0; u < SUB; ++u) sc[nt][u][0] = sc[nt][u][1] = sc[nt][u][2] = sc[nt][u][3] = 0.f;
+            const uint32_t krow = (lane & 7u) + ((lane >> 3) & 1u) * 8u, kaddr = sk + krow * 128u;
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+#pragma unroll
+                for (int u = 0; u < SUB; ++u) {
+                    uint32_t ak[4];                    // keys 16 u .. + 15, dimensions 16 kk .. + 15
+                    const uint32_t cc = 2u * kk + (lane >> 4);
+                    pa_ldm(ak, kaddr + (cc >> 3) * CF::kPanel + u * 2048u + ((cc ^ krow) & 7u) * 16u);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) pa_mma(sc[nt][u], ak, qf[nt][kk][0], qf[nt][kk][1]);
                 }
-            } else {
-                // one token after the other, with the values that it does not see taken out, into the rows of that token
-#pragma unroll 1
-                for (uint32_t tok = tok0; tok <= tok1; ++tok) {
-                    const int32_t last = min(rq.pos0 + (int32_t)tok, len1);
+            }
+            taken();
+            uint32_t ph[NT][SUB][2], pl[NT][SUB][2];
+            float corr[NT][2];
+            softmax(sc, key0, ph, pl, corr);
+            const uint32_t vrow = (lane & 7u) + (lane >> 4) * 8u, vaddr = landed() + vrow * 128u;
+            const bool tail = key0 + CF::kSlice - 1 > len1;            // uniform: without the values behind the last key
 #pragma unroll
-                    for (int d2 = 0; d2 < D / 16; ++d2) {
-                        uint32_t bv[4];
-                        values(bv, d2);
-                        cut(bv, last);
+            for (int d = 0; d < D / 16; ++d) {
+                float w[NT][4];
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            float w[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f};
-                            pa_mma(w, pl, bv[2 * c], bv[2 * c + 1]);
-                            pa_mma(u, ph, bv[2 * c], bv[2 * c + 1]);
-                            // (zero times infinity in the trailing bits is no reason for a NaN)
+                for (int nt = 0; nt < NT; ++nt) w[nt][0] = w[nt][1] = w[nt][2] = w[nt][3] = 0.f;
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const uint32_t m = rg * 16u + g + 8u * (i >> 1);
-                                const float add = fabsf(w[i]) < INFINITY ? u[i] + w[i] : u[i];
-                                if (m / G == tok) o[2 * d2 + c][i] = fmaf(o[2 * d2 + c][i], corr[i >> 1], add);
-                            }
+                for (int u = 0; u < SUB; ++u) {
+                    uint32_t av[4];                    // dimensions 16 d + g (+ 8 for odd registers), keys 16 u + 2 t, + 1 (+ 8 for the second two)
+                    const uint32_t cc = 2u * d + ((lane >> 3) & 1u);
+                    pa_ldmt(av, vaddr + (cc >> 3) * CF::kPanel + u * 2048u + ((cc ^ vrow) & 7u) * 16u);
+                    if (tail) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int32_t key = key0 + u * 16 + 2 * (int32_t)t + 8 * (i >> 1);
+                            av[i] &= key > len1 ? 0u : key == len1 ? 0xffffu : 0xffffffffu;
                         }
                     }
-                }
-            }
-            __syncwarp();                              // the stage is read
-            fetch(b + ST);
-        }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            l_[i] += __shfl_xor_sync(0xffffffffu, l_[i], 1);
-            l_[i] += __shfl_xor_sync(0xffffffffu, l_[i], 2);
-            if (!ok) l_[i] = __int_as_float(0x7fc00000);
+                    for (int nt = 0; nt < NT; ++nt) {
+                        pa_mma(w[nt], av, pl[nt][u][0], pl[nt][u][1]);
+                        pa_mma(w[nt], av, ph[nt][u][0], ph[nt][u][1]);
+                    }
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[nt][d][i] = fmaf(o[nt][d][i], corr[nt][i & 1], w[nt][i]);
+            }
+            taken();
         }
         float z = 0.f;
 #pragma unroll
-        for (int d = 0; d < D / 8; ++d) z = fmaf(o[d][0], 0.f, fmaf(o[d][1], 0.f, fmaf(o[d][2], 0.f, fmaf(o[d][3], 0.f, z))));
-        if (careful || !__syncthreads_or(z != 0.f)) break;             // all sums are finite
-        }
-        // ---- the warps' sums; whole: this is all of the pair
-        const bool whole = b0 == 0u && b1 == kb;
-        const unsigned long long x0 = x - b0;          // the pair's first block
-        float *dst = a.part + (size_t)(2u * me + (x == x_begin ? 0u : 1u)) * CF::kSlot;
-        auto out_row = [&](uint32_t m) {               // row m of the group
-            const uint32_t q = rg * 16u + m, tok = q / G;
-            return a.out + ((size_t)(rq.row0 + tok) * a.hq + h * G + (q - tok * G)) * D;
-        };
-        auto write_out = [&](uint32_t m, uint32_t d4, const float4 &v, float l) {
-            const uint32_t tok = (rg * 16u + m) / G;
-            const bool sees = rq.pos0 + (int32_t)tok >= 0 && rq.len > 0u;      // a row that sees nothing is zero
-            const float inv = sees ? 1.f / l : 0.f;
-            *(uint2 *)(out_row(m) + d4 * 4) = sees ? make_uint2(pa_pack(v.x * inv, v.y * inv), pa_pack(v.z * inv, v.w * inv)) : make_uint2(0u, 0u);
-        };
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {                  // rows 0 .. 7, rows 8 .. 15
-            if (rows <= 8u * i) break;                 // uniform
-            __syncthreads();
-            if (g + 8u * i < rows) {
-                float *to = sum + (wid * 8u + g) * CF::kPitch + 2u * t;
+            for (int d = 0; d < D / 16; ++d) z = fmaf(o[nt][d][0], 0.f, fmaf(o[nt][d][1], 0.f, fmaf(o[nt][d][2], 0.f, fmaf(o[nt][d][3], 0.f, z))));
+        uint32_t again;
+        asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                     : "=r"(again) : "r"((uint32_t)(z != 0.f)), "n"(CF::kCompute) : "memory");
+        if (again) {
+            // something is not finite: the same slices again, from memory, and P V for one token after the other with the values
+            // that it does not see taken out
+            const uint32_t tok0 = s.rg * Walk::kRows / G, tok1 = (s.rg * Walk::kRows + rows - 1u) / G;
+            zero();
+#pragma unroll 1
+            for (uint32_t b = s.b0; b < s.b1; ++b) {
+                const int32_t key0 = (int32_t)(b * CF::kKeys + wid * CF::kSlice);
+                if (key0 > len1) break;                // uniform
+                auto at = [&](const __nv_bfloat16 *pool, size_t stride, int32_t key) -> const __nv_bfloat16 * {        // null: zeros
+                    if (key > len1) return nullptr;
+                    const int32_t p = a.table[(size_t)s.r * a.width + ((uint32_t)key >> a.log_page)];
+                    return (uint32_t)p < a.n_pages ? pool + (size_t)p * stride + ((size_t)((uint32_t)key & (page - 1u)) * a.hkv + s.h) * D : nullptr;
+                };
+                float sc[NT][SUB][4];
 #pragma unroll
-                for (int d = 0; d < D / 8; ++d) *(float2 *)(to + d * 8) = make_float2(o[d][2 * i], o[d][2 * i + 1]);
-                if (t == 0) *(float2 *)(sum + (wid * 8u + g) * CF::kPitch + D) = make_float2(m_[i], l_[i]);
-            }
-            __syncthreads();
-            for (uint32_t it = tid; it < min(8u, rows - 8u * i) * (D / 4); it += CF::kThreads) {
-                const uint32_t row = it / (D / 4), d4 = it % (D / 4);
-                float M = -INFINITY, L = 0.f;
+                for (int u = 0; u < SUB; ++u) {
+                    const uint32_t *k0 = (const uint32_t *)at(a.k, a.k_stride, key0 + u * 16 + (int32_t)g), *k1 = (const uint32_t *)at(a.k, a.k_stride, key0 + u * 16 + 8 + (int32_t)g);
 #pragma unroll
-                for (int w = 0; w < NW; ++w) M = fmaxf(M, sum[(w * 8u + row) * CF::kPitch + D]);
-                const float mb = M == -INFINITY ? 0.f : M * sl2;
-                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (int nt = 0; nt < NT; ++nt) sc[nt][u][0] = sc[nt][u][1] = sc[nt][u][2] = sc[nt][u][3] = 0.f;
 #pragma unroll
-                for (int w = 0; w < NW; ++w) {
-                    const float2 ml = *(const float2 *)(sum + (w * 8u + row) * CF::kPitch + D);
-                    const float f = pa_exp2(fmaf(ml.x, sl2, -mb));
-                    const float4 u = *(const float4 *)(sum + (w * 8u + row) * CF::kPitch + d4 * 4);
-                    L = fmaf(ml.y, f, L);
-                    v.x = fmaf(u.x, f, v.x); v.y = fmaf(u.y, f, v.y); v.z = fmaf(u.z, f, v.z); v.w = fmaf(u.w, f, v.w);
+                    for (int kk = 0; kk < D / 16; ++kk) {
+                        const uint32_t ak[4] = {k0 ? k0[kk * 8 + t] : 0u, k1 ? k1[kk * 8 + t] : 0u, k0 ? k0[kk * 8 + 4 + t] : 0u, k1 ? k1[kk * 8 + 4 + t] : 0u};
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) pa_mma(sc[nt][u], ak, qf[nt][kk][0], qf[nt][kk][1]);
+                    }
                 }
-                const uint32_t m = row + 8u * i;
-                if (whole) {
-                    write_out(m, d4, v, L);
-                } else {
-                    *(float4 *)(dst + m * D + d4 * 4) = v;
-                    if (d4 == 0u) *(float2 *)(dst + 16 * D + 2 * m) = make_float2(M, L);
+                uint32_t ph[NT][SUB][2], pl[NT][SUB][2];
+                float corr[NT][2];
+                softmax(sc, key0, ph, pl, corr);
+#pragma unroll 1
+                for (uint32_t tok = tok0; tok <= tok1; ++tok) {
+                    const int32_t last = min(s.rq.pos0 + (int32_t)tok, len1);
+#pragma unroll
+                    for (int d = 0; d < D / 16; ++d) {
+                        float w[NT][4], v[NT][4];
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) w[nt][i] = v[nt][i] = 0.f;
+#pragma unroll
+                        for (int u = 0; u < SUB; ++u) {
+                            uint32_t av[4];
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {              // keys 2 t, 2 t + 1 (+ 8)
+                                const int32_t key = key0 + u * 16 + 2 * (int32_t)t + 8 * h;
+                                const __nv_bfloat16 *v0 = key <= last ? at(a.v, a.v_stride, key) : nullptr, *v1 = key < last ? at(a.v, a.v_stride, key + 1) : nullptr;
+#pragma unroll
+                                for (int i = 0; i < 2; ++i) {          // dimension 16 d + g (+ 8)
+                                    const uint32_t dim = d * 16 + i * 8 + g;
+                                    av[2 * h + i] = (v0 ? (uint32_t)__bfloat16_as_ushort(v0[dim]) : 0u) | (v1 ? (uint32_t)__bfloat16_as_ushort(v1[dim]) << 16 : 0u);
+                                }
+                            }
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) {
+                                pa_mma(w[nt], av, pl[nt][u][0], pl[nt][u][1]);
+                                pa_mma(v[nt], av, ph[nt][u][0], ph[nt][u][1]);
+                            }
+                        }
+                        // (zero times infinity in the trailing bits is no reason for a NaN)
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const uint32_t m = s.rg * Walk::kRows + nt * 8u + 2u * t + (i & 1);
+                                const float add = fabsf(w[nt][i]) < INFINITY ? v[nt][i] + w[nt][i] : v[nt][i];
+                                if (m / G == tok) o[nt][d][i] = fmaf(o[nt][d][i], corr[nt][i & 1], add);
+                            }
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                l_[nt][i] += __shfl_xor_sync(0xffffffffu, l_[nt][i], 4);
+                l_[nt][i] += __shfl_xor_sync(0xffffffffu, l_[nt][i], 8);
+                l_[nt][i] += __shfl_xor_sync(0xffffffffu, l_[nt][i], 16);
+                if (!ok) l_[nt][i] = __int_as_float(0x7fc00000);
+            }
+        // ---- the next pair, whose rows come while this one's sums are joined
+        const PagedReq rq = s.rq;
+        const uint32_t r_h = s.h, r_rg = s.rg, r_kb = s.kb;
+        const unsigned long long x0 = s.x - s.b0;      // the pair's first block
+        const bool whole = s.b0 == 0u && s.b1 == s.kb; // this is all of the pair
+        float *dst = a.part + (size_t)(2u * me + (s.x == x_begin ? 0u : 1u)) * CF::kSlot;
+        more = s.next(a, ahead);
+        if (more) rows_in();
+        // ---- the warps' sums
+        auto sync = [&]() { asm volatile("barrier.cta.sync 1, %0;" ::"n"(CF::kCompute) : "memory"); };
+        auto write_out = [&](uint32_t m, uint32_t d4, const float4 &v, float l) {      // row m of the group
+            const uint32_t q = r_rg * Walk::kRows + m, tok = q / G;
+            const bool sees = rq.pos0 + (int32_t)tok >= 0 && rq.len > 0u;              // a row that sees nothing is zero
+            const float inv = 1.f / l;
+            *(uint2 *)(a.out + ((size_t)(rq.row0 + tok) * a.hq + r_h * G + (q - tok * G)) * D + d4 * 4) =
+                sees ? make_uint2(pa_pack(v.x * inv, v.y * inv), pa_pack(v.z * inv, v.w * inv)) : make_uint2(0u, 0u);
+        };
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            if (rows <= 8u * nt) break;                // uniform
+#pragma unroll
+            for (int d0 = 0; d0 < D; d0 += CF::kSumD) {
+                if (nt || d0) sync();                  // (the first time the barrier above has been passed since the sums were read)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    float *to = sum + (wid * 8u + 2u * t + i) * CF::kPitch;
+                    if (8u * nt + 2u * t + i >= rows) continue;
+#pragma unroll
+                    for (int d = 0; d < CF::kSumD / 16; ++d) {
+                        to[d * 16 + g] = o[nt][d0 / 16 + d][i];
+                        to[d * 16 + 8 + g] = o[nt][d0 / 16 + d][2 + i];
+                    }
+                    if (g == 0) *(float2 *)(to + CF::kSumD) = make_float2(m_[nt][i], l_[nt][i]);
+                }
+                sync();
+                for (uint32_t it = tid; it < min(8u, rows - 8u * nt) * (CF::kSumD / 4); it += CF::kCompute) {
+                    const uint32_t row = it / (CF::kSumD / 4), d4 = it % (CF::kSumD / 4);
+                    const float *from = sum + row * CF::kPitch;
+                    float M = -INFINITY, L = 0.f;
+#pragma unroll
+                    for (int w = 0; w < NW; ++w) M = fmaxf(M, from[w * 8 * CF::kPitch + CF::kSumD]);
+                    const float mb = M == -INFINITY ? 0.f : M * sl2;
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                    for (int w = 0; w < NW; ++w) {
+                        const float2 ml = *(const float2 *)(from + w * 8 * CF::kPitch + CF::kSumD);
+                        const float f = pa_exp2(fmaf(ml.x, sl2, -mb));
+                        const float4 u = *(const float4 *)(from + w * 8 * CF::kPitch + d4 * 4);
+                        L = fmaf(ml.y, f, L);
+                        v.x = fmaf(u.x, f, v.x); v.y = fmaf(u.y, f, v.y); v.z = fmaf(u.z, f, v.z); v.w = fmaf(u.w, f, v.w);
+                    }
+                    const uint32_t m = row + 8u * nt;
+                    if (whole) {
+                        write_out(m, d0 / 4 + d4, v, L);
+                    } else {
+                        *(float4 *)(dst + m * D + d0 + d4 * 4) = v;
+                        if (d0 == 0 && d4 == 0u) *(float2 *)(dst + 16 * D + 2 * m) = make_float2(M, L);
+                    }
                 }
             }
         }
         if (!whole) {
-            // the CTA of block y is the last c with W c / N <= y
-            const uint32_t c0 = (uint32_t)(((x0 + 1ull) * N - 1ull) / W), c1 = (uint32_t)(((x0 + kb) * N - 1ull) / W), parts = c1 - c0 + 1u;
-            __syncthreads();
+            const uint32_t c0 = cta_of(x0), parts = cta_of(x0 + r_kb - 1u) - c0 + 1u;
+            sync();
             // numbers whose sum is zero, so the ticket is zero again when all have come
             if (tid == 0) {
                 const uint32_t add = me == c0 ? 1u - parts : 1u;
@@ -439,15 +621,15 @@ k_attn_paged(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
                 sm_last = atomicAdd(a.tickets + c0, add) + add == 0u;
                 __threadfence();
             }
-            __syncthreads();
+            sync();
             if (sm_last) {
-                const uint32_t behind = W * c0 / N != x0 ? 1u : 0u;
-                auto slot_of = [&](uint32_t c) { return a.part + (size_t)(2u * c + (c == c0 ? behind : 0u)) * CF::kSlot; };
+                const uint32_t behind = part_of(c0) != x0 ? 1u : 0u;
+                auto slot_of = [&](uint32_t q) { return a.part + (size_t)(2u * q + (q == c0 ? behind : 0u)) * CF::kSlot; };
                 // what every part counts, for every row: all of the parts' numbers are requested at once
-                float2 *ml = (float2 *)pa_smem;        // [parts][rows] (maximum, denominator): nothing is on its way into the ring
-                for (uint32_t i = tid; i < parts * rows; i += CF::kThreads) ml[i] = __ldcg((const float2 *)(slot_of(c0 + i / rows) + 16 * D) + i % rows);
-                __syncthreads();
-                for (uint32_t it = tid; it < rows * (D / 4); it += CF::kThreads) {
+                float2 *ml = (float2 *)sum;            // [parts][rows] (maximum, denominator)
+                for (uint32_t i = tid; i < parts * rows; i += CF::kCompute) ml[i] = __ldcg((const float2 *)(slot_of(c0 + i / rows) + 16 * D) + i % rows);
+                sync();
+                for (uint32_t it = tid; it < rows * (D / 4); it += CF::kCompute) {
                     const uint32_t m = it / (D / 4), d4 = it % (D / 4);
                     float M = -INFINITY, L = 0.f;
                     for (uint32_t p = 0; p < parts; ++p) M = fmaxf(M, ml[p * rows + m].x);
@@ -463,29 +645,9 @@ k_attn_paged(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
                     }
                     write_out(m, d4, v, L);
                 }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncthreads();                       // the ring is free again
             }
         }
-        x += b1 - b0;
-        if (x >= x_end) break;
-        // ---- the next pair: row group, request, KV head
-        if (++rg * 16u >= rq.n * G) {
-            rg = 0;
-            do {
-                if (++r == R) {
-                    r = 0;
-                    ++h;
-                }
-                rq = paged_req(a, r);
-            } while (!mine(rq) && h < a.hkv);          // (there is one, unless the lengths change under the kernel)
-            if (h >= a.hkv) break;
-            kb = key_blocks(rq);
-        }
-        b0 = 0;
     }
-    if (!ok)                                           // (otherwise every copy has been waited for)
-        for (uint32_t i = n > (uint32_t)ST ? n - ST : 0u; i < n; ++i) pa_wait(bar0 + 8u * (i % ST), i / ST & 1u);
 }
 
 }  // namespace ixb

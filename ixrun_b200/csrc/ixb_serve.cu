@@ -97,9 +97,10 @@ extern "C" int ixb_rope_paged(const void *q, const void *k, const void *v, const
 }
 
 // ------------------------------------------------------------------------------------------------ attention over pages
-// Requests with at most this many rows (new tokens times query heads of a KV head) go through k_attn_paged, one group of rows; the
-// others through k_attn_chunk.
-constexpr uint32_t kAttnFewRows = 16;
+// Requests with at most this many rows (new tokens times query heads of a KV head) go through k_attn_paged in one group of rows, the
+// others through k_attn_chunk.  (Sixteen rows of 256 dimensions do not fit its registers.)
+template <int D>
+constexpr uint32_t few_rows() { return D == 256 ? 8 : 16; }
 constexpr size_t kPaTicketBytes = 4096, kPaCutBytes = 8192;       // a word, a PcCut per CTA; the tickets are zero between launches
 
 template <int D>
@@ -113,41 +114,43 @@ extern "C" size_t ixb_attn_paged_scratch_bytes(int64_t head_dim)
     return kPaTicketBytes + kPaCutBytes + (head_dim == 64 ? attn_part_bytes<64>() : head_dim == 128 ? attn_part_bytes<128>() : attn_part_bytes<256>());
 }
 
-// a pool as a tensor of [pages][page][kv heads][D]: boxes of 64 dimensions of one head of `keys` positions of a page
-static CUresult pool_map(CUtensorMap *map, const __nv_bfloat16 *pool, size_t page_stride, const PagedAttn &a, uint32_t D, uint32_t keys)
+// a pool as a tensor of [pages][page][kv heads][D]: boxes of 64 dimensions of one head of (at most 128) positions of a page
+static CUresult pool_map(CUtensorMap *map, const __nv_bfloat16 *pool, size_t page_stride, const PagedAttn &a, uint32_t D)
 {
     const cuuint64_t dims[4] = {D, a.hkv, 1ull << a.log_page, a.n_pages}, strides[3] = {D * 2ull, (cuuint64_t)a.hkv * D * 2, (cuuint64_t)page_stride * 2};
-    const cuuint32_t box[4] = {64, 1, keys, 1}, one[4] = {1, 1, 1, 1};
+    const cuuint32_t box[4] = {64, 1, std::min(1u << a.log_page, kPcKeys), 1}, one[4] = {1, 1, 1, 1};
     return tensor_map_encoder()(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<__nv_bfloat16 *>(pool), dims, strides, box, one,
                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+}
+
+template <int D, int NT>
+static int launch_attn_few(const PagedAttn &a, const CUtensorMap &kmap, const CUtensorMap &vmap, cudaStream_t st)
+{
+    static bool attr_set[64] = {false};
+    IXB_CUDA(opt_in_smem(k_attn_paged<D, NT>, attr_set, (int)PaCfg<D>::kSmem));
+    IXB_CUDA(launch_glue_smem(k_attn_paged<D, NT>, dim3((unsigned)num_sms()), dim3(PaCfg<D>::kThreads), PaCfg<D>::kSmem, st, a, kmap, vmap));
+    return launch_check("k_attn_paged");
 }
 
 template <int D>
 static int attn_paged_run(PagedAttn a, PcCut *cuts, int64_t max_q, cudaStream_t st)
 {
     const unsigned sms = (unsigned)num_sms();
-    const bool few = max_q * a.group <= kAttnFewRows, both = !few && a.requests > 1u;
+    const bool few = max_q * a.group <= few_rows<D>(), both = !few && a.requests > 1u;
     if (!tensor_map_encoder()) return fail(IXB_E_UNSUPPORTED, "the driver has no cuTensorMapEncodeTiled");
     CUtensorMap kmap, vmap;
-    auto maps = [&](uint32_t keys) {
-        CUresult r = pool_map(&kmap, a.k, a.k_stride, a, D, keys);
-        if (r == CUDA_SUCCESS) r = pool_map(&vmap, a.v, a.v_stride, a, D, keys);
-        return r == CUDA_SUCCESS ? IXB_OK : fail(IXB_E_CUDA, "tensor map of a pool: error %d", (int)r);
-    };
+    CUresult r = pool_map(&kmap, a.k, a.k_stride, a, D);
+    if (r == CUDA_SUCCESS) r = pool_map(&vmap, a.v, a.v_stride, a, D);
+    if (r != CUDA_SUCCESS) return fail(IXB_E_CUDA, "tensor map of a pool: error %d", (int)r);
     int rc;
     if (few || both) {
-        if (both) a.row_hi = kAttnFewRows;
-        if ((rc = maps(16))) return rc;
-        static bool attr_set[64] = {false};
-        IXB_CUDA(opt_in_smem(k_attn_paged<D>, attr_set, (int)PaCfg<D>::kSmem));
-        IXB_CUDA(launch_glue_smem(k_attn_paged<D>, dim3(sms), dim3(PaCfg<D>::kThreads), PaCfg<D>::kSmem, st, a, kmap, vmap));
-        rc = launch_check("k_attn_paged");
+        if (both) a.row_hi = few_rows<D>();
+        rc = D == 256 || (few && max_q * a.group <= 8) ? launch_attn_few<D, 1>(a, kmap, vmap, st) : launch_attn_few<D, D == 256 ? 1 : 2>(a, kmap, vmap, st);
         if (rc || few) return rc;
-        a.row_lo = kAttnFewRows;
+        a.row_lo = few_rows<D>();
         a.row_hi = 0xffffffffu;
     }
-    if ((rc = maps(std::min(1u << a.log_page, kPcKeys)))) return rc;
     static bool attr_set[64] = {false};
     IXB_CUDA(opt_in_smem(k_attn_chunk<D>, attr_set, (int)PcCfg<D>::kSmem));
     IXB_CUDA(launch_glue_smem(k_attn_chunk<D>, dim3(sms), dim3(PcCfg<D>::kThreads), PcCfg<D>::kSmem, st, a, kmap, vmap, cuts));
@@ -171,7 +174,7 @@ extern "C" int ixb_attn_paged(const void *q, const void *k_pages, const void *v_
         return fail(IXB_E_ARG, "bad strides");
     if (((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)out | (uintptr_t)scratch) & 15u)
         return fail(IXB_E_ARG, "q, pages, output or scratch are not 16-byte aligned");
-    if (num_sms() > 256 || (size_t)num_sms() * sizeof(PcCut) > kPaCutBytes)
+    if (num_sms() > (int)kPaMaxCtas || (size_t)num_sms() * sizeof(PcCut) > kPaCutBytes)
         return fail(IXB_E_UNSUPPORTED, "a device of %d SMs", num_sms());
     if (scratch_bytes < ixb_attn_paged_scratch_bytes(head_dim)) return fail(IXB_E_SCRATCH, "attention scratch too small");
     PagedAttn a = {};
