@@ -43,9 +43,9 @@ static cudaError_t opt_in_smem(K kernel, bool (&done)[64], int bytes)
     return cudaSuccess;
 }
 
-// one launch with the programmatic-stream-serialization attribute when ixb_set_pdl is on
+// one launch, with the programmatic-stream-serialization attribute if `overlap`
 template <class... KArgs, class... Args>
-static cudaError_t launch_glue_smem(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args... args)
+static cudaError_t launch_overlapped(bool overlap, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args... args)
 {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
@@ -56,8 +56,14 @@ static cudaError_t launch_glue_smem(void (*kernel)(KArgs...), dim3 grid, dim3 bl
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = pdl_on() ? 1 : 0;
+    cfg.numAttrs = overlap ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+// the same when ixb_set_pdl is on
+template <class... KArgs, class... Args>
+static cudaError_t launch_glue_smem(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args... args)
+{
+    return launch_overlapped(pdl_on(), kernel, grid, block, smem, st, args...);
 }
 
 }  // namespace ixb

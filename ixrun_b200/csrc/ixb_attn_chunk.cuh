@@ -9,8 +9,9 @@
 //            of a unit; or, with one row tile, even and odd key tiles (each with an accumulator and a softmax of its own; heads of 256
 //            leave room for one accumulator, there they share it).
 //   warps    0 .. 3, 4 .. 7  softmax of the two slots (heads of 256: 0 .. 3); they also bring Q and write the results
-//            then            (of four) one that issues the MMAs, one that asks for K and V (TMA, a box per page and 64 dimensions, 128-byte
-//                            swizzle), in a ring of [128 keys][128 dimensions] (64 with heads of 64)
+//            then four       one that issues the MMAs, one that asks for K and V (TMA, a box per page and 64 dimensions, 128-byte
+//                            swizzle) in a ring of [128 keys][128 dimensions] (64 with heads of 64), two that look for values that are
+//                            not finite
 //
 // The accumulator is rescaled only when a row's maximum has grown by more than 2^8 (a running maximum that lags changes no ratio).
 // Precision: scores and sums fp32, probabilities bf16 for P V (half a step 2^-9 of each, as the result's own rounding; the tensor
@@ -18,7 +19,7 @@
 //
 // Keys that no row of the unit sees are not read; the rows of V behind the last key are zeroed up to a multiple of 16 and not
 // multiplied beyond.  A value that is not finite counts for the rows that see it and for no other: where a key tile is not
-// seen by all rows, the softmax warps look for such values and take the tile's P V themselves if there is one.
+// seen by all rows, two warps look for such values, and the softmax warps take the tile's P V themselves if there is one.
 //
 // Every wait on an mbarrier is bounded and counts this CTA's own copies and products; where one runs out the CTA's outputs
 // become NaN, and it carries on to its end with nothing in flight and tensor memory released.
@@ -44,9 +45,9 @@ struct PcCfg {
     static constexpr uint32_t kStages = D == 64 ? 8 : 5;
     static constexpr uint32_t kRingOff = kTiles * kQTile;
     static constexpr uint32_t kBarOff = kRingOff + kStages * kUnit;
-    static constexpr uint32_t kBars = 2 * kStages + 12;
+    static constexpr uint32_t kBars = 2 * kStages + 20;
     static constexpr uint32_t kSmem = kBarOff + kBars * 8 + 1024 + 128;        // and a few words; no static arrays: stages start on 1024 bytes
-    static constexpr int kSoftWarps = 4 * kGroups, kMmaWarp = kSoftWarps, kLoadWarp = kSoftWarps + 1, kThreads = (kSoftWarps + 4) * 32;
+    static constexpr int kSoftWarps = 4 * kGroups, kMmaWarp = kSoftWarps, kLoadWarp = kSoftWarps + 1, kScanWarp = kSoftWarps + 2, kThreads = (kSoftWarps + 4) * 32;
     // Registers of a thread: a softmax thread keeps a row of 128 scores.  With two groups of them the launch's 168 are dealt out
     // again (256 x 216 + 128 x 72 = 384 x 168); with one 255 are left for everybody.
     static constexpr bool kDeal = kGroups == 2;
@@ -179,6 +180,14 @@ struct PcWalk {
         const unsigned long long left = x_end - x;     // tiles whose first cost unit lies before x_end
         kt1 = (uint32_t)min((unsigned long long)u.tiles, kt0 + (left + u.weight - 1u) / u.weight);
     }
+    // Key tiles from this one on hold keys that not all of the unit's rows see, and are looked through.  (The position that its first row
+    // has is the last one that all of them see.)
+    __device__ __forceinline__ uint32_t looked(const PagedAttn &a) const
+    {
+        const int32_t low = rq.pos0 + (int32_t)(tile * PcCfg<D>::kUnitRows / a.group);
+        if ((int32_t)u.keys - 1 <= low) return u.tiles;
+        return low < (int32_t)kPcKeys - 1 ? 0u : (uint32_t)(low - (int32_t)kPcKeys + 1) / kPcKeys + 1u;
+    }
     // the next segment; false: there is none
     __device__ __forceinline__ bool next(const PagedAttn &a)
     {
@@ -214,10 +223,11 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
     const int warp = __shfl_sync(0xffffffffu, (int)(tid >> 5), 0);
     const uint32_t ring = s0 + CF::kRingOff, full0 = s0 + CF::kBarOff, empty0 = full0 + 8u * CF::kStages, q_full = empty0 + 8u * CF::kStages,
                    q_free = q_full + 8u, s_full0 = q_free + 8u, p_full0 = s_full0 + 16u, p_half0 = p_full0 + 16u, o_full0 = p_half0 + 16u, pv_done = o_full0 + 16u,
-                   done_bar = pv_done + 8u;
+                   done_bar = pv_done + 8u, w_full0 = done_bar + 8u, v_go0 = w_full0 + 32u;
     float2 *sm_ml = (float2 *)(smem + CF::kBarOff + CF::kBars * 8);            // [128]
     uint32_t *tmem_slot = (uint32_t *)(sm_ml + 128), &sm_units = tmem_slot[1], &sm_two = tmem_slot[2], *sm_warp = tmem_slot + 8;
     volatile uint32_t *wild_s = tmem_slot + 4;         // [2]: the slot's P V is done by its softmax warps
+    volatile uint32_t *found = tmem_slot + 24;         // [4][2]: what the two warps found in the values of a key tile
     asm volatile("griddepcontrol.launch_dependents;");
     if (tid == 0) {
         auto init = [&](uint32_t bar, uint32_t n, uint32_t count) {
@@ -230,6 +240,8 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
         init(p_full0, 4u, 4u);                         // (and p_half0)
         init(o_full0, 2u, 1u);
         init(pv_done, 2u, 1u);
+        init(w_full0, 4u, 2u);
+        init(v_go0, 4u, 1u);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
@@ -409,10 +421,10 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
         if (CF::kDeal) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         uint32_t el;
         asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(el));
-        uint32_t n0 = 0, seg = 0, p0 = 0, p1 = 0;      // before this segment: ring units, segments, steps of the two slots
+        uint32_t n0 = 0, seg = 0, p0 = 0, p1 = 0, n_look = 0;      // before this segment: ring units, segments, steps of the two slots, tiles looked through
         for (bool more = work; more && ok; more = w.next(a), ++seg) {
             const bool two = w.u.weight == 2u;         // two row tiles: a key tile is two steps
-            const uint32_t tiles = w.kt1 - w.kt0, steps = two ? 2u * tiles : tiles;
+            const uint32_t tiles = w.kt1 - w.kt0, steps = two ? 2u * tiles : tiles, look0 = max(w.looked(a), w.kt0);
             auto wait = [&](uint32_t bar, uint32_t parity) {
                 ok = ok && pa_wait(bar, parity);
                 ok = __all_sync(0xffffffffu, ok);
@@ -437,76 +449,119 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
                 if (st + 1u == steps) pc_commit(el, q_free);
             };
             wait(q_full, seg & 1u);
-            if (ok) qk(0u);
-            if (ok && steps > 1u) qk(1u);
-            for (uint32_t st = 0; st < steps && ok; ++st) {
-                const uint32_t slot = st & 1u, j = two ? st >> 1 : st, kt = w.kt0 + j;
-                const bool last_use = !two || slot;
-                const uint32_t valid = w.u.keys > kt * kPcKeys ? min(kPcKeys, w.u.keys - kt * kPcKeys) : 0u;
-                const uint32_t p_par = ((slot ? p1 : p0) + (st >> 1)) & 1u;
-                wait(p_half0 + 8u * slot, p_par);      // the first 64 keys' probabilities
-                if (!ok) break;
-                const bool wild = wild_s[slot] != 0u;
-                const uint32_t o = tmem + CF::kO + (CF::kTiles == 2 ? slot * 128u : 0u);
-                const uint32_t acc = (CF::kTiles == 2 ? st >= 2u : st >= 1u) ? 1u : 0u;
+            // Q K^T of a step two steps ahead of its P V
+            for (uint32_t it = 0; it < steps + 2u && ok; ++it) {
+                if (it >= 2u) {
+                    const uint32_t st = it - 2u, slot = st & 1u, j = two ? st >> 1 : st, kt = w.kt0 + j;
+                    const bool last_use = !two || slot;
+                    const uint32_t valid = w.u.keys > kt * kPcKeys ? min(kPcKeys, w.u.keys - kt * kPcKeys) : 0u;
+                    const uint32_t p_par = ((slot ? p1 : p0) + (st >> 1)) & 1u;
+                    if (kt >= look0 && (!two || !slot)) {              // the values are there: they may be looked through
 #pragma unroll
-                for (int c = 0; c < CF::kNU; ++c) {
-                    const uint32_t n = unit(j, 1u) + c, rs = n % CF::kStages, base = ring + rs * CF::kUnit;
-                    wait(full0 + 8u * rs, n / CF::kStages & 1u);
-                    if (!ok) break;
-                    if (valid & 15u) {                 // (both steps of a tile do it: the same zeros)
-                        const uint32_t z0 = valid, z1 = (valid + 15u) & ~15u;
-                        for (uint32_t i = lane; i < (z1 - z0) * (CF::kUD / 8); i += 32u) {
-                            const uint32_t row = z0 + i / (CF::kUD / 8), p = i % (CF::kUD / 8);
-                            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(base + (p >> 3) * CF::kPanel + row * 128u + (p & 7u) * 16u), "r"(0u) : "memory");
-                        }
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        for (int c = 0; c < CF::kNU; ++c) wait(full0 + 8u * ((unit(j, 1u) + c) % CF::kStages), (unit(j, 1u) + c) / CF::kStages & 1u);
+                        if (!ok) break;
+                        if (el) pc_arrive(v_go0 + 8u * ((n_look + kt - look0) & 3u));
                         __syncwarp();
                     }
-                    auto pv = [&](uint32_t kk) {
-                        pc_mma_ts(el, o + c * CF::kUD, tmem + slot * 128u + kk * 8u, pc_desc(base + kk * 2048u, CF::kPanel, 1024u), pc_idesc(CF::kUD, 1u), kk ? 1u : acc);
-                    };
-                    const uint32_t steps16 = wild ? 0u : (valid + 15u) / 16u;
-                    if (steps16 >= 4u) {
+                    wait(p_half0 + 8u * slot, p_par);      // the first 64 keys' probabilities
+                    if (!ok) break;
+                    const bool wild = wild_s[slot] != 0u;
+                    const uint32_t o = tmem + CF::kO + (CF::kTiles == 2 ? slot * 128u : 0u);
+                    const uint32_t acc = (CF::kTiles == 2 ? st >= 2u : st >= 1u) ? 1u : 0u;
 #pragma unroll
-                        for (uint32_t kk = 0; kk < 4u; ++kk) pv(kk);
-                    } else {
-                        for (uint32_t kk = 0; kk < steps16; ++kk) pv(kk);
-                    }
-                    if (c == 0) {
-                        wait(p_full0 + 8u * slot, p_par);
+                    for (int c = 0; c < CF::kNU; ++c) {
+                        const uint32_t n = unit(j, 1u) + c, rs = n % CF::kStages, base = ring + rs * CF::kUnit;
+                        wait(full0 + 8u * rs, n / CF::kStages & 1u);
                         if (!ok) break;
-                    }
-                    if (steps16 == 8u) {
+                        if (valid & 15u) {                 // (both steps of a tile do it: the same zeros)
+                            const uint32_t z0 = valid, z1 = (valid + 15u) & ~15u;
+                            for (uint32_t i = lane; i < (z1 - z0) * (CF::kUD / 8); i += 32u) {
+                                const uint32_t row = z0 + i / (CF::kUD / 8), p = i % (CF::kUD / 8);
+                                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(base + (p >> 3) * CF::kPanel + row * 128u + (p & 7u) * 16u), "r"(0u) : "memory");
+                            }
+                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                            __syncwarp();
+                        }
+                        auto pv = [&](uint32_t kk) {
+                            pc_mma_ts(el, o + c * CF::kUD, tmem + slot * 128u + kk * 8u, pc_desc(base + kk * 2048u, CF::kPanel, 1024u), pc_idesc(CF::kUD, 1u), kk ? 1u : acc);
+                        };
+                        const uint32_t steps16 = wild ? 0u : (valid + 15u) / 16u;
+                        if (steps16 >= 4u) {
 #pragma unroll
-                        for (uint32_t kk = 4; kk < 8u; ++kk) pv(kk);
-                    } else {
-                        for (uint32_t kk = 4; kk < steps16; ++kk) pv(kk);
+                            for (uint32_t kk = 0; kk < 4u; ++kk) pv(kk);
+                        } else {
+                            for (uint32_t kk = 0; kk < steps16; ++kk) pv(kk);
+                        }
+                        if (c == 0) {
+                            wait(p_full0 + 8u * slot, p_par);
+                            if (!ok) break;
+                        }
+                        if (steps16 == 8u) {
+#pragma unroll
+                            for (uint32_t kk = 4; kk < 8u; ++kk) pv(kk);
+                        } else {
+                            for (uint32_t kk = 4; kk < steps16; ++kk) pv(kk);
+                        }
+                        if (last_use) pc_commit(el, empty0 + 8u * rs);
                     }
-                    if (last_use) pc_commit(el, empty0 + 8u * rs);
+                    if (!ok) break;
+                    if (CF::kTiles == 1) pc_commit(el, pv_done);
+                    if (st + 1u == steps || (CF::kTiles == 2 && st + 2u == steps)) pc_commit(el, o_full0 + 8u * (CF::kTiles == 2 ? slot : 0u));
+                    if (CF::kTiles == 2 && steps == 1u) pc_commit(el, o_full0 + 8u);       // (the other slot has no step)
                 }
-                if (!ok) break;
-                if (CF::kTiles == 1) pc_commit(el, pv_done);
-                if (st + 1u == steps || (CF::kTiles == 2 && st + 2u == steps)) pc_commit(el, o_full0 + 8u * (CF::kTiles == 2 ? slot : 0u));
-                if (CF::kTiles == 2 && steps == 1u) pc_commit(el, o_full0 + 8u);       // (the other slot has no step)
-                if (st + 2u < steps) qk(st + 2u);
+                if (it < steps) qk(it);
             }
             n0 += 2u * tiles * CF::kNU;
             p0 += (steps + 1u) >> 1;
             p1 += steps >> 1;
+            n_look += w.kt1 - min(w.kt1, look0);
         }
         pc_commit(el, done_bar);
-    } else if (warp < CF::kSoftWarps) {
+    } else if (warp >= CF::kScanWarp) {
+        if (CF::kDeal) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        // ---- values that are not finite, in the key tiles that not all rows see
+        const uint32_t half = (uint32_t)(warp - CF::kScanWarp);
+        uint32_t n0 = 0, n_look = 0;
+        for (bool more = work; more && ok; more = w.next(a)) {
+            for (uint32_t kt = max(w.looked(a), w.kt0); kt < w.kt1 && ok; ++kt, ++n_look) {
+                const uint32_t keys = min(kPcKeys, w.u.keys - kt * kPcKeys);
+                uint32_t big = 0;
+                // (a parity of the ring's barriers alone does not tell a stage that is still to come from one two rounds before it: the
+                // warp that goes through all of them says when)
+                ok = ok && pa_wait(v_go0 + 8u * (n_look & 3u), n_look >> 2 & 1u);
+#pragma unroll
+                for (int c = 0; c < CF::kNU; ++c) {
+                    const uint32_t n = n0 + (2u * (kt - w.kt0) + 1u) * CF::kNU + c, rs = n % CF::kStages;
+                    ok = ok && pa_wait(full0 + 8u * rs, n / CF::kStages & 1u);
+#pragma unroll 8
+                    for (uint32_t i = half * 32u + lane; i < keys * (CF::kUD / 8); i += 64u) {
+                        uint4 v;
+                        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                                     : "r"(ring + rs * CF::kUnit + (i & 7u) * 16u + (i >> 3) / (CF::kUD / 64) * 128u + (i >> 3) % (CF::kUD / 64) * CF::kPanel) : "memory");
+                        big = pa_larger(pa_larger(pa_larger(pa_larger(big, v.x), v.y), v.z), v.w);
+                    }
+                }
+                ok = __all_sync(0xffffffffu, ok);
+                const bool any = __any_sync(0xffffffffu, pa_wild(big));
+                if (lane == 0) {
+                    found[(n_look & 3u) * 2u + half] = any;
+                    pc_arrive(w_full0 + 8u * (n_look & 3u));
+                }
+                __syncwarp();
+            }
+            n0 += 2u * (w.kt1 - w.kt0) * CF::kNU;
+        }
+    } else {
         if (CF::kDeal) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         // ---- softmax: group gr of four warps has a slot (heads of 256: both); a thread is a row
         const uint32_t gr = (uint32_t)warp >> 2, row_t = tid & 127u, lanes = ((uint32_t)warp & 3u) << 21;
         const float sl2 = a.scale * 1.4426950408889634f;
-        uint32_t c0s = 0, c1s = 0, pv_cnt = 0, seg = 0, n0 = 0;       // before this segment: steps of the slots, of both, segments, ring units
+        uint32_t c0s = 0, c1s = 0, pv_cnt = 0, seg = 0, n0 = 0, n_look = 0;       // before this segment: steps of the slots, of both, segments, ring units, tiles looked through
         uint32_t cut_parts = 0, cut_r = 0, cut_tile = 0, cut_h = 0, cut_slot = 0;
         for (bool more = work; more; more = w.next(a), ++seg) {
             const bool two = w.u.weight == 2u;
             const uint32_t tiles = w.kt1 - w.kt0, steps = two ? 2u * tiles : tiles;
-            // ---- Q: rows of the unit into [tile][64 dimensions][128 rows], swizzled; rows behind the last are zero
+            // ---- Q: rows of the unit into [tile][64 dimensions][128 rows], swizzled
             if (seg) ok = ok && pa_wait(q_free, (seg - 1u) & 1u);
             const uint32_t m0 = w.tile * CF::kUnitRows, tok0 = m0 / G, rem0 = m0 - tok0 * G;
             {
@@ -514,12 +569,11 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
                 const uint32_t ch = tid % CH;
                 const __nv_bfloat16 *src = a.q + (size_t)(w.rq.row0 + tok0) * a.q_stride + (size_t)w.h * G * D + ch * 8u;
 #pragma unroll 4
-                for (uint32_t m = tid / CH; m < (two ? 256u : 128u); m += STEP) {
+                for (uint32_t m = tid / CH; m < w.u.rows; m += STEP) {       // (what lies in rows behind the last one stays in them)
                     const uint32_t q = rem0 + m, tok = G == 1u ? q : __umulhi(q, a.group_magic), rr = m & 127u;
-                    const bool on = m < w.u.rows;
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
                                  ::"r"(s0 + (m >> 7) * CF::kQTile + (ch >> 3) * CF::kPanel + rr * 128u + ((ch ^ rr) & 7u) * 16u),
-                                 "l"(src + (on ? tok * a.q_stride + (size_t)(q - tok * G) * D : 0)), "r"(on ? 16u : 0u) : "memory");
+                                 "l"(src + tok * a.q_stride + (size_t)(q - tok * G) * D) : "memory");
                 }
                 cp_async_commit();
                 cp_async_wait<0>();
@@ -532,35 +586,18 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             const bool valid = m < w.u.rows;
             const int32_t limit = valid ? w.rq.pos0 + (int32_t)((m0 + m) / G) : -1;
             const bool warp_on = (m & ~31u) < w.u.rows;                        // (warp uniform) some row is there
-            const int32_t low_warp = w.rq.pos0 + (int32_t)((m0 + (m & ~31u)) / G), low_tile = w.rq.pos0 + (int32_t)((m0 + (m & ~127u)) / G);
+            const int32_t low_warp = w.rq.pos0 + (int32_t)((m0 + (m & ~31u)) / G);
+            const uint32_t look0 = max(w.looked(a), w.kt0);
             const uint32_t o_at = tmem + lanes + CF::kO + (CF::kTiles == 2 ? gr * 128u : 0u);
             float mb = -INFINITY, l = 0.f;             // the maximum that the sums are relative to (in units of log2), the denominator
             bool any = false;                          // (group uniform) the accumulator holds something
             const uint32_t stride = CF::kTiles == 2 ? 2u : 1u;
             for (uint32_t st = CF::kTiles == 2 ? gr : 0u; st < steps; st += stride) {
                 const uint32_t slot = st & 1u, j = two ? st >> 1 : st, kt = w.kt0 + j, s_at = tmem + lanes + slot * 128u;
-                const int32_t key0 = (int32_t)(kt * kPcKeys), key_last = min(key0 + (int32_t)kPcKeys, (int32_t)w.u.keys) - 1;
+                const int32_t key0 = (int32_t)(kt * kPcKeys);
                 ok = ok && pa_wait(s_full0 + 8u * slot, ((slot ? c1s : c0s) + (st >> 1)) & 1u);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 bool wild = false;
-                if (key_last > low_tile) {             // (group uniform) not every row sees every key: is there a value that is not finite?
-                    uint32_t big = 0;
-                    for (int c = 0; c < CF::kNU; ++c) {
-                        const uint32_t n = n0 + (2u * j + 1u) * CF::kNU + c, rs = n % CF::kStages;
-                        ok = ok && pa_wait(full0 + 8u * rs, n / CF::kStages & 1u);
-                        for (uint32_t i = row_t; i < (uint32_t)(key_last - key0 + 1) * (CF::kUD / 8); i += 128u) {
-                            uint4 v;
-                            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                                         : "r"(ring + rs * CF::kUnit + (i & 7u) * 16u + (i >> 3) / (CF::kUD / 64) * 128u + (i >> 3) % (CF::kUD / 64) * CF::kPanel) : "memory");
-                            big = pa_larger(pa_larger(pa_larger(pa_larger(big, v.x), v.y), v.z), v.w);
-                        }
-                    }
-                    uint32_t found;
-                    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-                                 : "=r"(found) : "r"((uint32_t)pa_wild(big)), "r"(1u + gr) : "memory");
-                    wild = found != 0u;
-                }
-                if (row_t == 0) wild_s[slot] = wild;
                 ok = __all_sync(0xffffffffu, ok);
                 if (warp_on && ok) {
                     uint32_t s[128];
@@ -582,7 +619,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
                         ok = ok && pa_wait(pv_done, (pv_cnt + st - 1u) & 1u);
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     }
-                    if (__any_sync(0xffffffffu, top > mb + 8.f)) {             // (false for -inf; the first maximum of a row is larger than -inf)
+                    if (__any_sync(0xffffffffu, valid && top > mb + 8.f)) {    // (false for -inf; the first maximum of a row is larger than -inf)
                         const float mn = fmaxf(mb, top), f = pa_exp2(mb - (mn == -INFINITY ? 0.f : mn));
                         mb = mn;
                         l *= f;
@@ -616,6 +653,12 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
                         pc_st32(s_at + 32u * half, s + 32 * half);
                         pc_wait_st();
                         if (half == 0) {
+                            if (kt >= look0) {         // (group uniform)
+                                const uint32_t k = n_look + kt - look0;
+                                ok = ok && pa_wait(w_full0 + 8u * (k & 3u), k >> 2 & 1u);
+                                wild = found[(k & 3u) * 2u] | found[(k & 3u) * 2u + 1u];
+                            }
+                            if (row_t == 0) wild_s[slot] = wild;
                             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                             __syncwarp();
                             if (lane == 0) pc_arrive(p_half0 + 8u * slot);
@@ -678,6 +721,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             c0s += (steps + 1u) >> 1;
             c1s += steps >> 1;
             n0 += 2u * tiles * CF::kNU;
+            n_look += w.kt1 - min(w.kt1, look0);
             // ---- the unit's sums
             ok = ok && pa_wait(o_full0 + 8u * gr, seg & 1u);
             if (CF::kTiles == 1) ok = ok && pa_wait(pv_done, (pv_cnt - 1u) & 1u);
@@ -695,7 +739,8 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
                 cut_h = w.h;
                 cut_slot = slot_n;
             }
-            const bool merge = CF::kTiles == 2 && !two;                        // both groups have a part of the same rows
+            const bool merge = CF::kTiles == 2 && !two && steps > 1u;          // both groups have a part of the same rows
+            const bool mine = two || gr == 0u;                                 // writes this row's result or part
             float other_l = 0.f, f_own = 1.f, f_other = 0.f;
             const uint32_t xbuf = s0 + CF::kQTile;                             // [columns][128 rows] floats: the second row tile's Q, unused here
             constexpr int XC = CF::kQTile / 512 < D ? (int)(CF::kQTile / 512) : D;     // columns that fit
@@ -716,7 +761,6 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
                     other_l = o.y;
                     mb = mn;
                     l = l * f_own + other_l * f_other;
-                    if (steps < 2u) f_other = 0.f;
                 }
             }
             const float inv = 1.f / l;
@@ -724,7 +768,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             for (int c0 = 0; c0 < D; c0 += merge ? XC : D) {
                 const int c1 = merge ? min(D, c0 + XC) : D;
                 if (merge) {
-                    if (gr == 1u && steps > 1u && warp_on) {
+                    if (gr == 1u && warp_on) {
 #pragma unroll 1
                         for (int c = c0; c < c1; c += 32) {
                             uint32_t o[32];
@@ -737,7 +781,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
                     }
                     asm volatile("barrier.cta.sync 3, 256;" ::: "memory");
                 }
-                if (warp_on && (!merge || gr == 0u)) {
+                if (warp_on && mine) {
 #pragma unroll 1
                     for (int c = c0; c < c1; c += 32) {
                         uint32_t o[32];
@@ -748,11 +792,9 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
 #pragma unroll
                             for (int i = 0; i < 32; ++i) {
                                 float v = __uint_as_float(o[i]) * f_own;
-                                if (steps > 1u) {
-                                    uint32_t u;
-                                    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(u) : "r"(xbuf + ((c - c0 + i) * 128u + row_t) * 4u) : "memory");
-                                    v = fmaf(__uint_as_float(u), f_other, v);
-                                }
+                                uint32_t u;
+                                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(u) : "r"(xbuf + ((c - c0 + i) * 128u + row_t) * 4u) : "memory");
+                                v = fmaf(__uint_as_float(u), f_other, v);
                                 o[i] = __float_as_uint(v);
                             }
                         }
@@ -776,7 +818,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
                 }
                 if (merge) asm volatile("barrier.cta.sync 3, 256;" ::: "memory");
             }
-            if (!whole && valid && (!merge || gr == 0u)) *(float2 *)(part + CF::kUnitRows * D + 2u * m) = make_float2(mb, l);
+            if (!whole && valid && mine) *(float2 *)(part + CF::kUnitRows * D + 2u * m) = make_float2(mb, l);
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");   // (the accumulators are read: the next unit's may be written)
         }
         if (tid == 0) {
@@ -786,8 +828,6 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             cuts[me].first_slot = cut_slot;
             cuts[me].parts = cut_parts;
         }
-    } else {
-        if (CF::kDeal) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     }
     __syncwarp();
     ok = pa_wait(done_bar, 0u) && ok;                  // (the MMAs that were issued are done, whoever gave up)

@@ -117,10 +117,12 @@ extern "C" size_t ixb_attn_paged_scratch_bytes(int64_t head_dim)
 // a pool as a tensor of [pages][page][kv heads][D]: boxes of 64 dimensions of one head of (at most 128) positions of a page
 static CUresult pool_map(CUtensorMap *map, const __nv_bfloat16 *pool, size_t page_stride, const PagedAttn &a, uint32_t D)
 {
+    // (heads of 64 with 128-byte lines: of a larger piece the half would be another head's, 64 requests behind 4000 128 us instead of 100)
     const cuuint64_t dims[4] = {D, a.hkv, 1ull << a.log_page, a.n_pages}, strides[3] = {D * 2ull, (cuuint64_t)a.hkv * D * 2, (cuuint64_t)page_stride * 2};
     const cuuint32_t box[4] = {64, 1, std::min(1u << a.log_page, kPcKeys), 1}, one[4] = {1, 1, 1, 1};
     return tensor_map_encoder()(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<__nv_bfloat16 *>(pool), dims, strides, box, one,
-                                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                D == 64 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
@@ -153,9 +155,10 @@ static int attn_paged_run(PagedAttn a, PcCut *cuts, int64_t max_q, cudaStream_t 
     }
     static bool attr_set[64] = {false};
     IXB_CUDA(opt_in_smem(k_attn_chunk<D>, attr_set, (int)PcCfg<D>::kSmem));
-    IXB_CUDA(launch_glue_smem(k_attn_chunk<D>, dim3(sms), dim3(PcCfg<D>::kThreads), PcCfg<D>::kSmem, st, a, kmap, vmap, cuts));
+    // (a launch behind another one of this call may begin while that ends: it waits for it before it reads or writes anything)
+    IXB_CUDA(launch_overlapped(both || pdl_on(), k_attn_chunk<D>, dim3(sms), dim3(PcCfg<D>::kThreads), PcCfg<D>::kSmem, st, a, kmap, vmap, cuts));
     if ((rc = launch_check("k_attn_chunk"))) return rc;
-    IXB_GLUE("k_attn_chunk_join", launch_glue_smem(k_attn_chunk_join<D>, dim3(sms, PcCfg<D>::kTiles * (D / 32)), dim3(128), 0, st, a, (const PcCut *)cuts));
+    IXB_GLUE("k_attn_chunk_join", launch_overlapped(true, k_attn_chunk_join<D>, dim3(sms, PcCfg<D>::kTiles * (D / 32)), dim3(128), 0, st, a, (const PcCut *)cuts));
 }
 
 extern "C" int ixb_attn_paged(const void *q, const void *k_pages, const void *v_pages, const int32_t *table, const int32_t *length,
