@@ -31,6 +31,7 @@ namespace ixb {
 
 constexpr uint32_t kPcKeys = 128;
 constexpr uint32_t kPcMinCost = 4;                     // key tiles of a CTA, unless there are more units than that makes CTAs
+constexpr uint32_t kPcShortUnit = 12;                  // cost of a unit (key tiles times row tiles), on average, up to which it is not cut
 
 template <int D>
 struct PcCfg {
@@ -53,14 +54,16 @@ struct PcCfg {
     static constexpr bool kDeal = kGroups == 2;
     static constexpr uint32_t kPart = kUnitRows * (D + 2);                     // floats: sums [tile][D / 4][128][4], (maximum, denominator) [rows]
     static constexpr uint32_t kO = 256;                // tensor memory: S or P of the slots at 0 and 128, accumulators from here
-    static_assert(kSmem <= 227 * 1024 && kStages * kUnit >= 4 * (kPaMaxRequests + 1) && kUnit % 1024 == 0, "fits");
+    static_assert(kSmem <= 227 * 1024 && kStages * kUnit >= 8 * kPaMaxRequests && kUnit % 1024 == 0, "fits");
 };
 
 // a unit that was cut, under the number of the CTA that has its first key tile; parts 0: none
 struct PcCut {
-    uint32_t parts, request, tile, head, first_slot;
+    uint32_t parts, first_slot;
+    uint32_t row0, m0, rows, head;                     // the request's first row; the unit's rows m0 .. m0 + rows - 1 of its packed ones, KV head
+    int32_t pos0;                                      // position of the request's first new token
+    uint32_t keys;                                     // that any row sees
 };
-
 __device__ __forceinline__ void pc_arrive(uint32_t mbar)
 {
     asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.shared::cta.b64 st, [%0];\n\t}" ::"r"(mbar) : "memory");
@@ -154,13 +157,13 @@ struct PcUnit {
     uint32_t rows, keys, tiles, weight;
 };
 template <int D>
-__device__ __forceinline__ PcUnit pc_unit(const PagedReq &q, uint32_t G, uint32_t tile)
+__device__ __forceinline__ PcUnit pc_unit(const PagedAttn &a, const PagedReq &q, uint32_t tile)
 {
     constexpr uint32_t TR = PcCfg<D>::kUnitRows;
     PcUnit u;
-    const uint32_t all = q.n * G, m0 = tile * TR;
+    const uint32_t all = q.n * a.group, m0 = tile * TR;
     u.rows = min(TR, all - m0);
-    const int32_t last = q.pos0 + (int32_t)((m0 + u.rows - 1u) / G);
+    const int32_t last = q.pos0 + (int32_t)a.by_group(m0 + u.rows - 1u);
     u.keys = last < 0 ? 0u : min((uint32_t)last + 1u, q.len);
     u.tiles = max(1u, (u.keys + kPcKeys - 1u) / kPcKeys);
     u.weight = u.rows > 128u ? 2u : 1u;
@@ -172,26 +175,27 @@ template <int D>
 struct PcWalk {
     unsigned long long x, x_end;                       // cost before the next key tile, and where the CTA's range ends
     uint32_t h, r, tile, kt0, kt1;                     // this segment: key tiles kt0 .. kt1 - 1 of the unit
+    bool by_unit;                                      // the line's parts are whole units, not key tiles
     PagedReq rq;
     PcUnit u;
     __device__ __forceinline__ static bool mine(const PagedAttn &a, const PagedReq &q) { return q.n * a.group > a.row_lo && q.n * a.group <= a.row_hi; }
     __device__ __forceinline__ void cut()
     {
         const unsigned long long left = x_end - x;     // tiles whose first cost unit lies before x_end
-        kt1 = (uint32_t)min((unsigned long long)u.tiles, kt0 + (left + u.weight - 1u) / u.weight);
+        kt1 = by_unit ? u.tiles : (uint32_t)min((unsigned long long)u.tiles, kt0 + (left + u.weight - 1u) / u.weight);
     }
     // Key tiles from this one on hold keys that not all of the unit's rows see, and are looked through.  (The position that its first row
     // has is the last one that all of them see.)
     __device__ __forceinline__ uint32_t looked(const PagedAttn &a) const
     {
-        const int32_t low = rq.pos0 + (int32_t)(tile * PcCfg<D>::kUnitRows / a.group);
+        const int32_t low = rq.pos0 + (int32_t)a.by_group(tile * PcCfg<D>::kUnitRows);
         if ((int32_t)u.keys - 1 <= low) return u.tiles;
         return low < (int32_t)kPcKeys - 1 ? 0u : (uint32_t)(low - (int32_t)kPcKeys + 1) / kPcKeys + 1u;
     }
     // the next segment; false: there is none
     __device__ __forceinline__ bool next(const PagedAttn &a)
     {
-        x += (unsigned long long)(kt1 - kt0) * u.weight;
+        x += by_unit ? 1ull : (unsigned long long)(kt1 - kt0) * u.weight;
         if (x >= x_end) return false;
         kt0 = 0;
         if (++tile * PcCfg<D>::kUnitRows >= rq.n * a.group) {
@@ -205,7 +209,7 @@ struct PcWalk {
             } while (!mine(a, rq) && h < a.hkv);       // (there is one, unless the lengths change under the kernel)
             if (h >= a.hkv) return false;
         }
-        u = pc_unit<D>(rq, a.group, tile);
+        u = pc_unit<D>(a, rq, tile);
         cut();
         return true;
     }
@@ -225,7 +229,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
                    q_free = q_full + 8u, s_full0 = q_free + 8u, p_full0 = s_full0 + 16u, p_half0 = p_full0 + 16u, o_full0 = p_half0 + 16u, pv_done = o_full0 + 16u,
                    done_bar = pv_done + 8u, w_full0 = done_bar + 8u, v_go0 = w_full0 + 32u;
     float2 *sm_ml = (float2 *)(smem + CF::kBarOff + CF::kBars * 8);            // [128]
-    uint32_t *tmem_slot = (uint32_t *)(sm_ml + 128), &sm_units = tmem_slot[1], &sm_two = tmem_slot[2], *sm_warp = tmem_slot + 8;
+    uint32_t *tmem_slot = (uint32_t *)(sm_ml + 128), &sm_units = tmem_slot[1], &sm_two = tmem_slot[2], &sm_cost = tmem_slot[3], *sm_warp = tmem_slot + 8;
     volatile uint32_t *wild_s = tmem_slot + 4;         // [2]: the slot's P V is done by its softmax warps
     volatile uint32_t *found = tmem_slot + 24;         // [4][2]: what the two warps found in the values of a key tile
     asm volatile("griddepcontrol.launch_dependents;");
@@ -245,7 +249,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
-        sm_units = sm_two = 0u;
+        sm_units = sm_two = sm_cost = 0u;
     }
     if (warp == CF::kMmaWarp) {
         const uint32_t slot_addr = (uint32_t)__cvta_generic_to_shared(tmem_slot);
@@ -254,20 +258,24 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
     }
     __syncthreads();
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    // ---- the cost before every request, of one KV head (over the ring, which is empty)
-    uint32_t *first = (uint32_t *)(smem + CF::kRingOff);
+    // ---- every request's cost and units, of one KV head (over the ring, which is empty)
+    uint32_t *first = (uint32_t *)(smem + CF::kRingOff), *units = first + kPaMaxRequests;
     const uint32_t R = a.requests, G = a.group, me = blockIdx.x;
     auto cost_of = [&](const PagedReq &q, uint32_t t) {
         if (t * CF::kUnitRows >= q.n * G) return 0u;
-        const PcUnit u = pc_unit<D>(q, G, t);
+        const PcUnit u = pc_unit<D>(a, q, t);
         return u.tiles * u.weight;
     };
-    auto count = [&](const PagedReq &q) {
-        atomicAdd(&sm_units, (q.n * G + CF::kUnitRows - 1u) / CF::kUnitRows);
+    auto note = [&](uint32_t r, const PagedReq &q, uint32_t cost) {
+        const uint32_t n = cost ? (q.n * G + CF::kUnitRows - 1u) / CF::kUnitRows : 0u;
+        first[r] = cost;
+        units[r] = n;
+        if (!n) return;
+        atomicAdd(&sm_cost, cost);
+        atomicAdd(&sm_units, n);
         if (CF::kTiles == 2 && q.n * G > 128u) sm_two = 1u;
     };
     const uint32_t per = (R + CF::kThreads - 1) / CF::kThreads, ra = min(R, tid * per), rb = min(R, ra + per);
-    uint32_t total = 0;
     if (R <= 2u * CF::kThreads / 32u) {                // few requests, perhaps of many tiles: a warp each
         for (uint32_t r = (uint32_t)warp; r < R; r += CF::kThreads / 32) {
             const PagedReq q = paged_req(a, r);
@@ -275,10 +283,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             if (PcWalk<D>::mine(a, q))
                 for (uint32_t t = lane; t * CF::kUnitRows < q.n * G; t += 32u) own += cost_of(q, t);
             own = __reduce_add_sync(0xffffffffu, own);
-            if (lane == 0) {
-                first[r] = own;
-                if (own) count(q);
-            }
+            if (lane == 0) note(r, q, own);
         }
     } else {
         for (uint32_t r = ra; r < rb; ++r) {
@@ -286,14 +291,18 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             uint32_t own = 0;
             if (PcWalk<D>::mine(a, q))
                 for (uint32_t t = 0; t * CF::kUnitRows < q.n * G; ++t) own += cost_of(q, t);
-            first[r] = own;
-            if (own) count(q);
+            note(r, q, own);
         }
     }
     __syncthreads();
+    // What the line is cut into: key tiles; or whole units where there is room for one per CTA and they are short, so that cutting them
+    // would cost more than it saves (300 rows of a prompt, 16 / 8 heads of 128: 24 us cut, FIG whole)
+    const bool by_unit = (unsigned long long)sm_units * a.hkv <= gridDim.x && sm_cost <= kPcShortUnit * sm_units;
+    const uint32_t total = by_unit ? sm_units : sm_cost;
     {
+        const uint32_t *const own_of = by_unit ? units : first;
         uint32_t own = 0, before = 0;
-        for (uint32_t r = ra; r < rb; ++r) own += first[r];
+        for (uint32_t r = ra; r < rb; ++r) own += own_of[r];
         uint32_t v = own;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -303,13 +312,11 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
         if (lane == 31u) sm_warp[warp] = v;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < CF::kThreads / 32; ++w) {
+        for (int w = 0; w < CF::kThreads / 32; ++w)
             if (w < warp) before += sm_warp[w];
-            total += sm_warp[w];
-        }
         before += v - own;
         for (uint32_t r = ra; r < rb; ++r) {
-            const uint32_t c = first[r];
+            const uint32_t c = own_of[r];
             first[r] = before;
             before += c;
         }
@@ -318,8 +325,8 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
     const unsigned long long W = (unsigned long long)total * a.hkv;
     // CTAs: one for every four key tiles, or every unit if that is more; with units of two row tiles a range is at least as long as a
     // key tile's cost, so that every CTA between the first and the last of a unit has a key tile of it
-    unsigned long long n_max = max((unsigned long long)sm_units * a.hkv, (W + kPcMinCost - 1u) / kPcMinCost);
-    if (sm_two) n_max = min(n_max, max(W / 2u, 1ull));
+    unsigned long long n_max = by_unit ? W : max((unsigned long long)sm_units * a.hkv, (W + kPcMinCost - 1u) / kPcMinCost);
+    if (sm_two && !by_unit) n_max = min(n_max, max(W / 2u, 1ull));
     const uint32_t N = (uint32_t)min((unsigned long long)gridDim.x, n_max);
     auto part_of = [&](uint32_t c) { return W < 1u << 24 ? (unsigned long long)((uint32_t)W * c / N) : W * c / N; };      // (N at most 256)
     auto cta_of = [&](unsigned long long y) {          // the last c with part_of(c) <= y
@@ -331,6 +338,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
         return;
     }
     PcWalk<D> w;
+    w.by_unit = by_unit;
     w.x = part_of(me);
     w.x_end = part_of(me + 1u);
     {
@@ -344,7 +352,12 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
         w.r = lo;
         off -= first[lo];
         w.rq = paged_req(a, lo);
-        for (w.tile = 0;; w.tile += 32u) {             // its tile: 32 at a time (off is less than the request's cost)
+        w.tile = 0;
+        if (by_unit) {
+            w.tile = off;
+            off = 0;
+        }
+        for (; !by_unit; w.tile += 32u) {              // its tile: 32 at a time (off is less than the request's cost)
             const uint32_t c = cost_of(w.rq, w.tile + lane);
             uint32_t v = c;
 #pragma unroll
@@ -362,7 +375,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             if ((w.tile + 32u) * CF::kUnitRows >= w.rq.n * G) break;           // (not so, unless the lengths change under the kernel)
             off -= __shfl_sync(0xffffffffu, v, 31);
         }
-        w.u = pc_unit<D>(w.rq, G, w.tile);
+        w.u = pc_unit<D>(a, w.rq, w.tile);
         w.kt0 = (off + w.u.weight - 1u) / w.u.weight;  // a tile that began before this range is its predecessor's
         w.x += w.kt0 * w.u.weight - off;
         w.kt1 = w.kt0;
@@ -557,20 +570,20 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
         const uint32_t gr = (uint32_t)warp >> 2, row_t = tid & 127u, lanes = ((uint32_t)warp & 3u) << 21;
         const float sl2 = a.scale * 1.4426950408889634f;
         uint32_t c0s = 0, c1s = 0, pv_cnt = 0, seg = 0, n0 = 0, n_look = 0;       // before this segment: steps of the slots, of both, segments, ring units, tiles looked through
-        uint32_t cut_parts = 0, cut_r = 0, cut_tile = 0, cut_h = 0, cut_slot = 0;
+        if (tid == 0) cuts[me].parts = 0u;
         for (bool more = work; more; more = w.next(a), ++seg) {
             const bool two = w.u.weight == 2u;
             const uint32_t tiles = w.kt1 - w.kt0, steps = two ? 2u * tiles : tiles;
             // ---- Q: rows of the unit into [tile][64 dimensions][128 rows], swizzled
             if (seg) ok = ok && pa_wait(q_free, (seg - 1u) & 1u);
-            const uint32_t m0 = w.tile * CF::kUnitRows, tok0 = m0 / G, rem0 = m0 - tok0 * G;
+            const uint32_t m0 = w.tile * CF::kUnitRows, tok0 = a.by_group(m0), rem0 = m0 - tok0 * G;
             {
                 constexpr uint32_t CH = D / 8, STEP = CF::kSoftWarps * 32 / CH;        // 16-byte pieces of a row, rows at a time
                 const uint32_t ch = tid % CH;
                 const __nv_bfloat16 *src = a.q + (size_t)(w.rq.row0 + tok0) * a.q_stride + (size_t)w.h * G * D + ch * 8u;
 #pragma unroll 4
                 for (uint32_t m = tid / CH; m < w.u.rows; m += STEP) {       // (what lies in rows behind the last one stays in them)
-                    const uint32_t q = rem0 + m, tok = G == 1u ? q : __umulhi(q, a.group_magic), rr = m & 127u;
+                    const uint32_t q = rem0 + m, tok = a.by_group(q), rr = m & 127u;
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
                                  ::"r"(s0 + (m >> 7) * CF::kQTile + (ch >> 3) * CF::kPanel + rr * 128u + ((ch ^ rr) & 7u) * 16u),
                                  "l"(src + tok * a.q_stride + (size_t)(q - tok * G) * D) : "memory");
@@ -584,9 +597,9 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             // ---- this thread's row
             const uint32_t m = (two ? gr * 128u : 0u) + row_t;                 // in the unit
             const bool valid = m < w.u.rows;
-            const int32_t limit = valid ? w.rq.pos0 + (int32_t)((m0 + m) / G) : -1;
+            const int32_t limit = valid ? w.rq.pos0 + (int32_t)a.by_group(m0 + m) : -1;
             const bool warp_on = (m & ~31u) < w.u.rows;                        // (warp uniform) some row is there
-            const int32_t low_warp = w.rq.pos0 + (int32_t)((m0 + (m & ~31u)) / G);
+            const int32_t low_warp = w.rq.pos0 + (int32_t)a.by_group(m0 + (m & ~31u));
             const uint32_t look0 = max(w.looked(a), w.kt0);
             const uint32_t o_at = tmem + lanes + CF::kO + (CF::kTiles == 2 ? gr * 128u : 0u);
             float mb = -INFINITY, l = 0.f;             // the maximum that the sums are relative to (in units of log2), the denominator
@@ -733,11 +746,8 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             const uint32_t slot_n = 2u * me + (w.kt0 ? 0u : 1u);               // a unit's first part is this CTA's last segment
             float *part = a.part + (size_t)slot_n * CF::kPart;
             if (!whole && w.kt0 == 0u) {
-                cut_parts = cta_of(x0 + (unsigned long long)(w.u.tiles - 1u) * w.u.weight) - me + 1u;
-                cut_r = w.r;
-                cut_tile = w.tile;
-                cut_h = w.h;
-                cut_slot = slot_n;
+                if (tid == 0)                          // (at most one of a CTA: its last)
+                    cuts[me] = {cta_of(x0 + (unsigned long long)(w.u.tiles - 1u) * w.u.weight) - me + 1u, slot_n, w.rq.row0, m0, w.u.rows, w.h, w.rq.pos0, w.u.keys};
             }
             const bool merge = CF::kTiles == 2 && !two && steps > 1u;          // both groups have a part of the same rows
             const bool mine = two || gr == 0u;                                 // writes this row's result or part
@@ -746,7 +756,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             constexpr int XC = CF::kQTile / 512 < D ? (int)(CF::kQTile / 512) : D;     // columns that fit
             __nv_bfloat16 *dst = a.out;
             if (valid) {
-                const uint32_t q = m0 + m, tok = q / G;
+                const uint32_t q = m0 + m, tok = a.by_group(q);
                 dst = a.out + ((size_t)(w.rq.row0 + tok) * a.hq + (size_t)w.h * G + (q - tok * G)) * D;
             }
             if (merge) {
@@ -821,13 +831,6 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             if (!whole && valid && mine) *(float2 *)(part + CF::kUnitRows * D + 2u * m) = make_float2(mb, l);
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");   // (the accumulators are read: the next unit's may be written)
         }
-        if (tid == 0) {
-            cuts[me].request = cut_r;
-            cuts[me].tile = cut_tile;
-            cuts[me].head = cut_h;
-            cuts[me].first_slot = cut_slot;
-            cuts[me].parts = cut_parts;
-        }
     }
     __syncwarp();
     ok = pa_wait(done_bar, 0u) && ok;                  // (the MMAs that were issued are done, whoever gave up)
@@ -839,7 +842,8 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
     }
 }
 
-// The parts of the units that were cut.  grid (CTAs of k_attn_chunk, row tiles x groups of 32 dimensions), a thread per row.
+// The parts of the units that were cut.  grid (CTAs of k_attn_chunk, row tiles x groups of 16 dimensions), a thread per row; four parts
+// of a row are requested at once.
 template <int D>
 __global__ void __launch_bounds__(128)
 k_attn_chunk_join(PagedAttn a, const PcCut *cuts)
@@ -848,35 +852,51 @@ k_attn_chunk_join(PagedAttn a, const PcCut *cuts)
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const PcCut cut = cuts[blockIdx.x];
-    if (cut.parts == 0u) return;
-    const PagedReq rq = paged_req(a, cut.request);
-    const PcUnit u = pc_unit<D>(rq, a.group, cut.tile);
-    const uint32_t tile = blockIdx.y / (D / 32), c0 = blockIdx.y % (D / 32) * 8u, row = threadIdx.x, m = tile * 128u + row;
-    if (m >= u.rows) return;
+    const uint32_t tile = blockIdx.y / (D / 16), c0 = blockIdx.y % (D / 16) * 4u, row = threadIdx.x, m = tile * 128u + row;
+    if (cut.parts == 0u || m >= cut.rows) return;
+    constexpr uint32_t UN = 4;
     auto part = [&](uint32_t p) { return a.part + (size_t)(p ? 2u * (blockIdx.x + p) : cut.first_slot) * CF::kPart; };
     float M = -INFINITY, L = 0.f;
-    for (uint32_t p = 0; p < cut.parts; ++p) M = fmaxf(M, ((const float2 *)(part(p) + CF::kUnitRows * D))[m].x);
-    const float mz = M == -INFINITY ? 0.f : M;
-    float4 v[8];
+    float4 v[4];
 #pragma unroll
-    for (int c = 0; c < 8; ++c) v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (uint32_t p = 0; p < cut.parts; ++p) {
-        const float2 ml = ((const float2 *)(part(p) + CF::kUnitRows * D))[m];
-        const float f = pa_exp2(ml.x - mz);
-        L = fmaf(ml.y, f, L);
-        const float4 *src = (const float4 *)part(p) + (size_t)(tile * (D / 4) + c0) * 128u + row;
+    for (int c = 0; c < 4; ++c) v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (uint32_t p0 = 0; p0 < cut.parts; p0 += UN) {
+        float2 ml[UN];
+        float4 s[UN][4];
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-            const float4 s = src[c * 128];
-            v[c].x = fmaf(s.x, f, v[c].x); v[c].y = fmaf(s.y, f, v[c].y); v[c].z = fmaf(s.z, f, v[c].z); v[c].w = fmaf(s.w, f, v[c].w);
+        for (uint32_t i = 0; i < UN; ++i) {
+            const float *src = part(min(p0 + i, cut.parts - 1u));
+            ml[i] = p0 + i < cut.parts ? ((const float2 *)(src + CF::kUnitRows * D))[m] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) s[i][c] = ((const float4 *)src)[(size_t)(tile * (D / 4) + c0 + c) * 128u + row];
+        }
+        float mn = M;
+#pragma unroll
+        for (uint32_t i = 0; i < UN; ++i) mn = fmaxf(mn, ml[i].x);
+        const float mz = mn == -INFINITY ? 0.f : mn, shrink = pa_exp2(M - mz);
+        M = mn;
+        L *= shrink;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            v[c].x *= shrink; v[c].y *= shrink; v[c].z *= shrink; v[c].w *= shrink;
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < UN; ++i) {
+            if (p0 + i >= cut.parts) break;
+            const float f = pa_exp2(ml[i].x - mz);
+            L = fmaf(ml[i].y, f, L);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                v[c].x = fmaf(s[i][c].x, f, v[c].x); v[c].y = fmaf(s[i][c].y, f, v[c].y); v[c].z = fmaf(s[i][c].z, f, v[c].z); v[c].w = fmaf(s[i][c].w, f, v[c].w);
+            }
         }
     }
-    const uint32_t q = cut.tile * CF::kUnitRows + m, tok = q / a.group;
-    const bool sees = rq.pos0 + (int32_t)tok >= 0 && u.keys > 0u;
+    const uint32_t q = cut.m0 + m, tok = a.by_group(q);
+    const bool sees = cut.pos0 + (int32_t)tok >= 0 && cut.keys > 0u;
     const float inv = 1.f / L;
-    __nv_bfloat16 *dst = a.out + ((size_t)(rq.row0 + tok) * a.hq + (size_t)cut.head * a.group + (q - tok * a.group)) * D + c0 * 4u;
+    __nv_bfloat16 *dst = a.out + ((size_t)(cut.row0 + tok) * a.hq + (size_t)cut.head * a.group + (q - tok * a.group)) * D + c0 * 4u;
 #pragma unroll
-    for (int c = 0; c < 8; c += 2)
+    for (int c = 0; c < 4; c += 2)
         *(uint4 *)(dst + c * 4) = sees ? make_uint4(pa_pack(v[c].x * inv, v[c].y * inv), pa_pack(v[c].z * inv, v[c].w * inv),
                                                     pa_pack(v[c + 1].x * inv, v[c + 1].y * inv), pa_pack(v[c + 1].z * inv, v[c + 1].w * inv))
                                        : make_uint4(0u, 0u, 0u, 0u);

@@ -38,9 +38,10 @@ struct PagedAttn {
     uint32_t *tickets;
     size_t k_stride, v_stride, q_stride;               // elements: page to page, row to row
     uint32_t requests, width, n_pages, log_page, rows, hq, hkv, group;
-    uint32_t group_magic;                              // ceil(2^32 / group): x / group = umulhi(x, magic) for x * group < 2^32, group > 1
+    uint32_t group_magic;                              // ceil(2^32 / group)
     uint32_t row_lo, row_hi;                           // requests with row_lo < q_len * group <= row_hi are taken
     float scale;
+    __device__ __forceinline__ uint32_t by_group(uint32_t m) const { return group == 1u ? m : __umulhi(m, group_magic); }      // m / group, m * group < 2^32
 };
 
 // what a request has: the row of its first new token, new tokens, its positions in the pages, the position of the first new token
@@ -326,7 +327,7 @@ k_attn_paged(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
     auto rows_in = [&]() {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const uint32_t m = s.rg * Walk::kRows + nt * 8u + g, tok = m / G, gi = m - tok * G;
+            const uint32_t m = s.rg * Walk::kRows + nt * 8u + g, tok = a.by_group(m), gi = m - tok * G;
             const bool on = m < s.rq.n * G;
             const uint32_t *src = (const uint32_t *)(a.q + (size_t)(s.rq.row0 + (on ? tok : 0u)) * a.q_stride + ((size_t)s.h * G + (on ? gi : 0u)) * D) + t;
 #pragma unroll
@@ -337,7 +338,7 @@ k_attn_paged(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const uint32_t q = s.rg * Walk::kRows + nt * 8u + 2u * t + i;
-                limit[nt][i] = q < s.rq.n * G ? min(s.rq.pos0 + (int32_t)(q / G), (int32_t)s.rq.len - 1) : -1;
+                limit[nt][i] = q < s.rq.n * G ? min(s.rq.pos0 + (int32_t)a.by_group(q), (int32_t)s.rq.len - 1) : -1;
             }
         }
     };
@@ -345,7 +346,7 @@ k_attn_paged(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
     bool more = true;
     while (more) {
         const uint32_t rows = min(Walk::kRows, s.rq.n * G - s.rg * Walk::kRows);
-        const int32_t len1 = (int32_t)s.rq.len - 1, all_see = min(s.rq.pos0 + (int32_t)(s.rg * Walk::kRows / G), len1);
+        const int32_t len1 = (int32_t)s.rq.len - 1, all_see = min(s.rq.pos0 + (int32_t)a.by_group(s.rg * Walk::kRows), len1);
         const PagedReq ahead = paged_req(a, s.after(a));               // (requested here, needed where the pair ends)
         // sums: dimensions 16 d + g (+ 8 for elements 2 and 3) of rows 8 nt + 2 t (+ 1 for odd elements); maxima of the raw scores
         float o[NT][D / 16][4], m_[NT][2], l_[NT][2];
@@ -472,7 +473,7 @@ k_attn_paged(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
         if (again) {
             // something is not finite: the same slices again, from memory, and P V for one token after the other with the values
             // that it does not see taken out
-            const uint32_t tok0 = s.rg * Walk::kRows / G, tok1 = (s.rg * Walk::kRows + rows - 1u) / G;
+            const uint32_t tok0 = a.by_group(s.rg * Walk::kRows), tok1 = a.by_group(s.rg * Walk::kRows + rows - 1u);
             zero();
 #pragma unroll 1
             for (uint32_t b = s.b0; b < s.b1; ++b) {
@@ -535,7 +536,7 @@ k_attn_paged(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
                             for (int i = 0; i < 4; ++i) {
                                 const uint32_t m = s.rg * Walk::kRows + nt * 8u + 2u * t + (i & 1);
                                 const float add = fabsf(w[nt][i]) < INFINITY ? v[nt][i] + w[nt][i] : v[nt][i];
-                                if (m / G == tok) o[nt][d][i] = fmaf(o[nt][d][i], corr[nt][i & 1], add);
+                                if (a.by_group(m) == tok) o[nt][d][i] = fmaf(o[nt][d][i], corr[nt][i & 1], add);
                             }
                     }
                 }
@@ -561,7 +562,7 @@ k_attn_paged(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
         // ---- the warps' sums
         auto sync = [&]() { asm volatile("barrier.cta.sync 1, %0;" ::"n"(CF::kCompute) : "memory"); };
         auto write_out = [&](uint32_t m, uint32_t d4, const float4 &v, float l) {      // row m of the group
-            const uint32_t q = r_rg * Walk::kRows + m, tok = q / G;
+            const uint32_t q = r_rg * Walk::kRows + m, tok = a.by_group(q);
             const bool sees = rq.pos0 + (int32_t)tok >= 0 && rq.len > 0u;              // a row that sees nothing is zero
             const float inv = 1.f / l;
             *(uint2 *)(a.out + ((size_t)(rq.row0 + tok) * a.hq + r_h * G + (q - tok * G)) * D + d4 * 4) =

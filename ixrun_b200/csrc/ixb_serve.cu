@@ -158,7 +158,7 @@ static int attn_paged_run(PagedAttn a, PcCut *cuts, int64_t max_q, cudaStream_t 
     // (a launch behind another one of this call may begin while that ends: it waits for it before it reads or writes anything)
     IXB_CUDA(launch_overlapped(both || pdl_on(), k_attn_chunk<D>, dim3(sms), dim3(PcCfg<D>::kThreads), PcCfg<D>::kSmem, st, a, kmap, vmap, cuts));
     if ((rc = launch_check("k_attn_chunk"))) return rc;
-    IXB_GLUE("k_attn_chunk_join", launch_overlapped(true, k_attn_chunk_join<D>, dim3(sms, PcCfg<D>::kTiles * (D / 32)), dim3(128), 0, st, a, (const PcCut *)cuts));
+    IXB_GLUE("k_attn_chunk_join", launch_overlapped(true, k_attn_chunk_join<D>, dim3(sms, PcCfg<D>::kTiles * (D / 16)), dim3(128), 0, st, a, (const PcCut *)cuts));
 }
 
 extern "C" int ixb_attn_paged(const void *q, const void *k_pages, const void *v_pages, const int32_t *table, const int32_t *length,
@@ -172,6 +172,7 @@ extern "C" int ixb_attn_paged(const void *q, const void *k_pages, const void *v_
     if (hq <= 0 || hkv <= 0 || hq > 65535 || hq % hkv) return fail(IXB_E_ARG, "query heads must be a multiple of KV heads");
     if (head_dim != 64 && head_dim != 128 && head_dim != 256) return fail(IXB_E_UNSUPPORTED, "head_dim=%lld: 64, 128 or 256", (long long)head_dim);
     if (rows <= 0 || rows > 0x7fffffffll / hq || max_q <= 0) return fail(IXB_E_ARG, "bad rows");
+    if (rows * (hq / hkv) > 0xfffffff0ll / (hq / hkv)) return fail(IXB_E_UNSUPPORTED, "%lld rows of groups of %lld heads", (long long)rows, (long long)(hq / hkv));
     if (q_stride < hq * head_dim || (q_stride & 7) || k_page_stride < page * hkv * head_dim || v_page_stride < page * hkv * head_dim ||
         ((k_page_stride | v_page_stride) & 7))
         return fail(IXB_E_ARG, "bad strides");
