@@ -47,7 +47,8 @@ struct PcCfg {
     static constexpr uint32_t kRingOff = kTiles * kQTile;
     static constexpr uint32_t kBarOff = kRingOff + kStages * kUnit;
     static constexpr uint32_t kBars = 2 * kStages + 20;
-    static constexpr uint32_t kSmem = kBarOff + kBars * 8 + 1024 + 128;        // and a few words; no static arrays: stages start on 1024 bytes
+    static constexpr uint32_t kWalkOff = kBarOff + kBars * 8 + 1024 + 128;
+    static constexpr uint32_t kSmem = kWalkOff + kGroups * 4 * 80;             // no static arrays: stages start on 1024 bytes
     static constexpr int kSoftWarps = 4 * kGroups, kMmaWarp = kSoftWarps, kLoadWarp = kSoftWarps + 1, kScanWarp = kSoftWarps + 2, kThreads = (kSoftWarps + 4) * 32;
     // Registers of a thread: a softmax thread keeps a row of 128 scores.  With two groups of them the launch's 168 are dealt out
     // again (256 x 216 + 128 x 72 = 384 x 168); with one 255 are left for everybody.
@@ -215,6 +216,8 @@ struct PcWalk {
     }
 };
 
+static_assert(sizeof(PcWalk<64>) <= 80, "fits");
+
 template <int D>
 __global__ void __launch_bounds__(PcCfg<D>::kThreads, 1)
 k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, PcCut *cuts)
@@ -296,7 +299,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
     }
     __syncthreads();
     // What the line is cut into: key tiles; or whole units where there is room for one per CTA and they are short, so that cutting them
-    // would cost more than it saves (300 rows of a prompt, 16 / 8 heads of 128: 24 us cut, FIG whole)
+    // would cost more than it saves (300 rows of a prompt, 16 / 8 heads of 128: 24 us cut, 16.8 whole)
     const bool by_unit = (unsigned long long)sm_units * a.hkv <= gridDim.x && sm_cost <= kPcShortUnit * sm_units;
     const uint32_t total = by_unit ? sm_units : sm_cost;
     {
@@ -571,9 +574,14 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
         const float sl2 = a.scale * 1.4426950408889634f;
         uint32_t c0s = 0, c1s = 0, pv_cnt = 0, seg = 0, n0 = 0, n_look = 0;       // before this segment: steps of the slots, of both, segments, ring units, tiles looked through
         if (tid == 0) cuts[me].parts = 0u;
-        for (bool more = work; more; more = w.next(a), ++seg) {
+        // (the way through the units lies in shared memory between segments: beside a row of scores there is no room for it)
+        PcWalk<D> *const kept = (PcWalk<D> *)(smem + CF::kWalkOff) + warp;
+        if (lane == 0) *kept = w;
+        __syncwarp();
+        for (bool more = work; more; ++seg) {
+            PcWalk<D> w = *kept;
             const bool two = w.u.weight == 2u;
-            const uint32_t tiles = w.kt1 - w.kt0, steps = two ? 2u * tiles : tiles;
+            const uint32_t kt0 = w.kt0, tiles = w.kt1 - kt0, steps = two ? 2u * tiles : tiles;
             // ---- Q: rows of the unit into [tile][64 dimensions][128 rows], swizzled
             if (seg) ok = ok && pa_wait(q_free, (seg - 1u) & 1u);
             const uint32_t m0 = w.tile * CF::kUnitRows, tok0 = a.by_group(m0), rem0 = m0 - tok0 * G;
@@ -606,7 +614,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             bool any = false;                          // (group uniform) the accumulator holds something
             const uint32_t stride = CF::kTiles == 2 ? 2u : 1u;
             for (uint32_t st = CF::kTiles == 2 ? gr : 0u; st < steps; st += stride) {
-                const uint32_t slot = st & 1u, j = two ? st >> 1 : st, kt = w.kt0 + j, s_at = tmem + lanes + slot * 128u;
+                const uint32_t slot = st & 1u, j = two ? st >> 1 : st, kt = kt0 + j, s_at = tmem + lanes + slot * 128u;
                 const int32_t key0 = (int32_t)(kt * kPcKeys);
                 ok = ok && pa_wait(s_full0 + 8u * slot, ((slot ? c1s : c0s) + (st >> 1)) & 1u);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -734,8 +742,10 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             c0s += (steps + 1u) >> 1;
             c1s += steps >> 1;
             n0 += 2u * tiles * CF::kNU;
-            n_look += w.kt1 - min(w.kt1, look0);
+            n_look += kt0 + tiles - min(kt0 + tiles, look0);
             // ---- the unit's sums
+            asm volatile("" ::: "memory");
+            w = *kept;
             ok = ok && pa_wait(o_full0 + 8u * gr, seg & 1u);
             if (CF::kTiles == 1) ok = ok && pa_wait(pv_done, (pv_cnt - 1u) & 1u);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -830,6 +840,10 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             }
             if (!whole && valid && mine) *(float2 *)(part + CF::kUnitRows * D + 2u * m) = make_float2(mb, l);
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");   // (the accumulators are read: the next unit's may be written)
+            more = w.next(a);
+            __syncwarp();
+            if (lane == 0) *kept = w;
+            __syncwarp();
         }
     }
     __syncwarp();
