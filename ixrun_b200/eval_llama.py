@@ -29,6 +29,8 @@ def main():
     ap.add_argument("--batched", default="",
                     help="comma-separated batch sizes: also time lock-step decoding of B sequences (BatchedGreedyDecoder; "
                          "B <= 8 on the fused GEMV, up to 64 on the tensor-core GEMM) and report tokens per second")
+    ap.add_argument("--paged", default="",
+                    help="comma-separated numbers of requests (1..64): the same for requests over a paged cache (PagedDecoder)")
     ap.add_argument("--no-pdl", action="store_true",
                     help="launch the packed GEMVs without programmatic dependent launch")
     args = ap.parse_args()
@@ -106,6 +108,30 @@ def main():
                             "linears": "fused GEMV" if b <= 8 else "fused GEMM"})
             del dec
             torch.cuda.empty_cache()
+    paged = None
+    if args.paged:
+        from .llama_runner import PagedDecoder
+
+        paged = []
+        g = torch.Generator().manual_seed(2)
+        for b in (int(v) for v in args.paged.split(",")):
+            dec = PagedDecoder(packed, b, b * (-(-cfg.max_seq // 64))).capture()
+            for _ in range(b):
+                dec.add(torch.randint(0, cfg.vocab, (128,), generator=g))
+            for _ in range(4):
+                dec.step()
+            torch.cuda.synchronize()
+            e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            steps = 32
+            e0.record()
+            for _ in range(steps):
+                dec.step()
+            e1.record()
+            torch.cuda.synchronize()
+            ms = e0.elapsed_time(e1) / steps
+            paged.append({"requests": b, "ms_per_step": round(ms, 4), "tokens_per_s": round(b / ms * 1e3, 1)})
+            del dec
+            torch.cuda.empty_cache()
     print(json.dumps({
         "model": f"llama-style {args.layers}L h{cfg.hidden} ffn{cfg.intermediate} {cfg.n_heads}q/{cfg.n_kv_heads}kv vocab{cfg.vocab}",
         "packed_linears": len(layers) * 7, "packed_weights": n_weights, "packed_MB": packed_bytes / 1e6,
@@ -116,6 +142,7 @@ def main():
         "free_running_prefix_match": int((toks_packed == toks_dense).long().cumprod(0).sum().item()),
         "min_top1_top2_margin_at_mismatch": None if agree == args.new else min_margin,
         "setup_s": setup_s, "batched_decode_128_token_prompts": batched,
+        "paged_decode_128_token_prompts": paged,
     }), flush=True)
 
 

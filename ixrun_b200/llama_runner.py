@@ -561,6 +561,244 @@ class BatchedGreedyDecoder:
         return torch.stack(out, dim=1)
 
 
+class PagedDecoder:
+    """Requests that come and go, decoded together on a packed model over a paged KV cache: what the reference's batched
+    generator does with one static cache row per sequence (ixrun/batching.py:88-234), for requests of different lengths in
+    memory for the tokens that there are.  A step feeds every request the tokens that it has and the model has not seen: the
+    next piece of its prompt, or its last token.  Steps of single tokens are one CUDA graph (``capture``).  Per request:
+    penalties, biases and a mask of allowed tokens; the token is the arg-max behind them."""
+
+    def __init__(self, model: PackedLlama, requests: int, n_pages: int, page: int = 64, max_bias: int = 64):
+        from .paged import AttnPaged, PageTables
+
+        if model.weights != "packed" or model.glue != "kernels":
+            raise ValueError("the paged decoder runs on packed weights and the glue kernels")
+        if not 1 <= requests <= 64:
+            raise ValueError("1..64 requests")
+        if max_bias < 0:
+            raise ValueError("max_bias must not be negative")
+        self.m, self.b = model, int(requests)
+        cfg, dev, b = model.cfg, model.embed.device, self.b
+        self._attn = AttnPaged(cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, dev)
+        self.pages = PageTables(b, n_pages, page, -(-cfg.max_seq // page), dev)
+        self.k_pages = torch.zeros(cfg.n_layers, n_pages, page, cfg.n_kv_heads, cfg.head_dim, dtype=torch.bfloat16, device=dev)
+        self.v_pages = torch.zeros_like(self.k_pages)
+        # what is known of every request: its tokens (prompt and answer), how many, and its rules
+        ints = dict(dtype=torch.int32, device=dev)
+        self.history = torch.zeros(b, cfg.max_seq + 1, **ints)
+        self.n_tokens, self.n_prompt, self.q_len = (torch.zeros(b, **ints) for _ in range(3))
+        self.repetition, self.presence, self.frequency = (torch.zeros(b, dtype=torch.float32, device=dev) for _ in range(3))
+        self.repetition.fill_(1.0)
+        self.bias_ids = torch.full((b, max_bias), -1, **ints)
+        self.bias_values = torch.zeros(b, max_bias, dtype=torch.float32, device=dev)
+        self.mask = torch.zeros(b, -(-cfg.vocab // 32), **ints)
+        self.mask_row = torch.full((b,), -1, **ints)
+        # results of a step: logits behind the rules, and the token of every request (-1: none in this step)
+        self.logits = torch.zeros(b, cfg.vocab, dtype=torch.float32, device=dev)
+        self.token = torch.full((b,), -1, dtype=torch.long, device=dev)
+        self._best = torch.zeros(b, dtype=torch.long, device=dev)
+        # the host's account of the same: tokens known and tokens in the cache (None: no request), pages left
+        self._known, self._cached = [None] * b, [0] * b
+        self._pages_left, self._fed = n_pages, [0] * b
+        self._step, self._bufs = self.pages.new_step(b), self._buffers(b)
+        self.graph = None
+
+    def _buffers(self, rows):
+        cfg, first = self.m.cfg, self.m.layers[0]
+        new = lambda n: torch.zeros(rows, n, dtype=torch.bfloat16, device=self.m.embed.device)  # noqa: E731
+        return dict(h=new(cfg.hidden), xn=new(cfg.hidden), d=new(cfg.hidden), qkv=new(first["qkv"].res.out_f), gu=new(first["gate_up"].res.out_f),
+                    a=new(cfg.n_heads * cfg.head_dim), act=new(cfg.intermediate))
+
+    def _lin(self, res, x, out):
+        if x.shape[0] <= 8:
+            return res.gemv(x, out=out)
+        if x.shape[0] <= 64:
+            return res.gemm(x, out=out)
+        return torch.matmul(x, res.decode(out=self.m._shared[:res.N], kind="bf16").t(), out=out)
+
+    def _forward(self, step, bufs, max_q):
+        """One pass of the rows that `step` says through the model; logits, tokens and what is known of the requests."""
+        from . import glue as G
+        from .logits import apply_rules
+        from .paged import rope_kv_paged
+
+        m, cfg = self.m, self.m.cfg
+        self.pages.step(self.q_len, step.slot.numel(), out=step)
+        h, xn, d, a, act = (bufs[n] for n in ("h", "xn", "d", "a", "act"))
+        q, k, v = (bufs["qkv"][:, o:o + n] for o, n in m.layers[0]["qkv"].res.sections)
+        g, u = (bufs["gu"][:, o:o + n] for o, n in m.layers[0]["gate_up"].res.sections)
+        at = step.owner.clamp(min=0).long() * self.history.shape[1] + step.pos     # (rows behind the last token: any token)
+        torch.index_select(m.embed, 0, self.history.view(-1).index_select(0, at).long(), out=h)
+        delta = None
+        for li, L in enumerate(m.layers):
+            G.add_rmsnorm(h, delta, m.ln1[li], cfg.rms_eps, out=xn)
+            self._lin(L["qkv"].res, xn, bufs["qkv"])
+            rope_kv_paged(q, k, v, step.pos, step.slot, self.k_pages[li], self.v_pages[li], m.cos, m.sin, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim)
+            self._attn(q, self.k_pages[li], self.v_pages[li], self.pages.table, step.length, step.cu_rows, max_q=max_q, out=a)
+            self._lin(L["o_proj"]._res, a, d)
+            G.add_rmsnorm(h, d, m.ln2[li], cfg.rms_eps, out=xn)
+            self._lin(L["gate_up"].res, xn, bufs["gu"])
+            G.swiglu(g, u, out=act)
+            self._lin(L["down_proj"]._res, act, d)
+            delta = d
+        last = (step.cu_rows[1:] - 1).clamp(min=0)                                 # (requests without a row: any row)
+        x = G.add_rmsnorm(h.index_select(0, last), delta.index_select(0, last), m.ln_f, cfg.rms_eps)
+        apply_rules(F.linear(x, m.lm_head), self.history, self.n_tokens, self.n_prompt, self.repetition, self.presence, self.frequency,
+                    self.bias_ids if self.bias_ids.shape[1] else None, self.bias_values if self.bias_ids.shape[1] else None, self.mask,
+                    self.mask_row, out=self.logits, token=self._best)
+        # a request whose known tokens are all in the cache has a new one
+        new = (self.q_len > 0) & (step.length == self.n_tokens)
+        end = self.n_tokens.long().clamp(max=self.history.shape[1] - 1)[:, None]   # (of a full request: rewritten as it is)
+        self.history.scatter_(1, end, torch.where(new[:, None], self._best[:, None].int(), self.history.gather(1, end)))
+        self.n_tokens += new
+        self.token.copy_(torch.where(new, self._best, -1))
+
+    # ------------------------------------------------------------------- API
+    def _request(self, r):
+        if not 0 <= r < self.b or self._known[r] is None:
+            raise ValueError(f"no request {r}")
+        return r
+
+    @torch.no_grad()
+    def add(self, prompt: torch.Tensor, repetition: float = 1.0, presence: float = 0.0, frequency: float = 0.0, bias: dict | None = None,
+            allowed: torch.Tensor | None = None) -> int:
+        """Takes a request in; returns its number (a free one).  The rules are those of ``logits.apply_rules``; bias: {token:
+        value}; allowed: a bool tensor [vocab]."""
+        n = prompt.numel()
+        if None not in self._known:
+            raise RuntimeError("all requests are taken")
+        if not 1 <= n <= self.m.cfg.max_seq:
+            raise ValueError(f"a prompt of 1..{self.m.cfg.max_seq} tokens")
+        if prompt.is_floating_point() or prompt.min() < 0 or prompt.max() >= self.m.cfg.vocab:
+            raise ValueError(f"tokens are whole numbers of 0..{self.m.cfg.vocab - 1}")
+        if not repetition > 0.0:
+            raise ValueError("repetition must be positive")
+        bias = bias or {}
+        if len(bias) > self.bias_ids.shape[1]:
+            raise ValueError(f"at most {self.bias_ids.shape[1]} biases")
+        r = self._known.index(None)
+        self._allow(r, allowed)
+        dev = self.history.device
+        self.history[r, :n].copy_(prompt.reshape(-1))
+        for t, x in ((self.n_tokens, n), (self.n_prompt, n), (self.repetition, repetition), (self.presence, presence), (self.frequency, frequency)):
+            t[r].fill_(x)
+        if self.bias_ids.shape[1]:
+            self.bias_ids[r].fill_(-1)
+        if bias:
+            self.bias_ids[r, :len(bias)].copy_(torch.tensor(list(bias), dtype=torch.int32, device=dev))
+            self.bias_values[r, :len(bias)].copy_(torch.tensor(list(bias.values()), dtype=torch.float32, device=dev))
+        self._known[r], self._cached[r] = n, 0
+        return r
+
+    def allow(self, r: int, allowed: torch.Tensor | None):
+        """The tokens that request r may have from now on (a bool tensor [vocab]; None: all), as a grammar moves on."""
+        self._allow(self._request(r), allowed)
+
+    @torch.no_grad()
+    def _allow(self, r, allowed):
+        if allowed is None:
+            self.mask_row[r].fill_(-1)
+            return
+        if allowed.dtype != torch.bool or allowed.shape != (self.m.cfg.vocab,):
+            raise ValueError("allowed: a bool tensor [vocab]")
+        bits = F.pad(allowed.to(self.mask.device), (0, self.mask.shape[1] * 32 - allowed.numel())).view(-1, 32).long()
+        words = (bits << torch.arange(32, device=bits.device)).sum(1)
+        self.mask[r].copy_(torch.where(words >= 2**31, words - 2**32, words))
+        self.mask_row[r].fill_(r)
+
+    @torch.no_grad()
+    def remove(self, r: int):
+        """The request's pages go back to the pool, and its number may be taken by the next one."""
+        self._request(r)
+        done = torch.zeros(self.b, dtype=torch.bool, device=self.history.device)
+        done[r].fill_(True)
+        self.pages.release(done)
+        self.n_tokens[r].fill_(0)
+        self._pages_left += self._n_pages(self._cached[r])
+        self._known[r], self._cached[r] = None, 0
+
+    def _n_pages(self, tokens):
+        return -(-tokens // self.pages.page)
+
+    @torch.no_grad()
+    def step(self, max_rows: int = PackedLlama.PREFILL_ROWS) -> torch.Tensor:
+        """Feeds the requests what they have, at most max_rows rows in all: single tokens first, then prompts in the order of
+        their numbers.  Returns tokens int64 [requests], -1 for those without a new one (a static tensor)."""
+        left, q_len = int(max_rows), [0] * self.b
+        todo = {r: n - self._cached[r] for r, n in enumerate(self._known) if n is not None}
+        for r in sorted(todo, key=lambda r: (todo[r] > 1, r)):
+            q_len[r] = min(todo[r], left)
+            left -= q_len[r]
+        if not any(q_len):
+            raise RuntimeError("no request to feed")
+        if any(self._cached[r] + n > self.m.cfg.max_seq for r, n in enumerate(q_len)):
+            raise RuntimeError(f"a request has all {self.m.cfg.max_seq} tokens that fit: remove it")
+        need = sum(self._n_pages(c + n) - self._n_pages(c) for c, n in zip(self._cached, q_len))
+        if need > self._pages_left:
+            raise RuntimeError(f"the step needs {need} pages, {self._pages_left} are left: remove a request")
+        if q_len != self._fed:
+            self.q_len.copy_(torch.tensor(q_len, dtype=torch.int32))
+            self._fed = q_len
+        if max(q_len) == 1:
+            if self.graph is not None:
+                self.graph.replay()
+            else:
+                self._forward(self._step, self._bufs, 1)
+        else:
+            self._forward(self.pages.new_step(sum(q_len)), self._buffers(sum(q_len)), max(q_len))
+        self._pages_left -= need
+        for r, n in enumerate(q_len):
+            self._cached[r] += n
+            if n and self._cached[r] == self._known[r]:
+                self._known[r] += 1
+        return self.token
+
+    @torch.no_grad()
+    def capture(self):
+        """Captures the step of single tokens."""
+        self.q_len.zero_()                     # (the warm-up feeds nothing)
+        self._fed = [0] * self.b
+        side = torch.cuda.Stream(self.q_len.device)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _ in range(2):
+                self._forward(self._step, self._bufs, 1)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        self.graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(self.graph):
+            self._forward(self._step, self._bufs, 1)
+        return self
+
+    @torch.no_grad()
+    def generate(self, prompts: list, n_new: int, eos: int | None = None, max_rows: int = PackedLlama.PREFILL_ROWS, **rules) -> list:
+        """n_new tokens for every prompt (fewer for one that ends with eos or has all max_seq tokens), as lists; a prompt waits
+        until a number and the pages for its whole answer are free."""
+        if n_new < 1:
+            raise ValueError("n_new must be positive")
+        if any(n is not None for n in self._known):
+            raise RuntimeError("generate wants the decoder for itself: remove the requests that are there")
+        whole = [self._n_pages(min(ids.numel() + n_new - 1, self.m.cfg.max_seq)) for ids in prompts]
+        if whole and max(whole) > self._pages_left:
+            raise RuntimeError(f"a prompt and its answer need {max(whole)} pages, there are {self._pages_left}")
+        out, waiting, running, free = [[] for _ in prompts], list(range(len(prompts))), {}, self._pages_left
+        while waiting or running:
+            while waiting and None in self._known and whole[waiting[0]] <= free:
+                i = waiting.pop(0)
+                running[self.add(prompts[i], **rules)] = i
+                free -= whole[i]
+            tokens = self.step(max_rows).tolist()
+            for r, i in list(running.items()):
+                if tokens[r] < 0:
+                    continue
+                out[i].append(tokens[r])
+                if len(out[i]) == n_new or tokens[r] == eos or self._known[r] > self.m.cfg.max_seq:
+                    self.remove(r)
+                    del running[r]
+                    free += whole[i]
+        return out
+
+
 def synthetic_llama(cfg: LlamaConfig, seed: int = 0, distinct_layers: bool = True):
     """Random-init weights of the config: Laplace codes for every linear (one
     tensor per linear type and layer when distinct_layers, else one per type
