@@ -105,6 +105,7 @@ struct PaCfg {
     static constexpr uint32_t kStage = D / 64 * kSub * kPanel;     // K or V of a block: [128 keys][64 dimensions]
     static constexpr int kStages = 196608 / kStage;
     static constexpr uint32_t kRing = kStages * kStage;
+    static constexpr uint32_t kWhole = 4 * 65536 / (2 * kStage);       // blocks of a pair that is never cut (256 KB)
     static constexpr int kSumD = D < 128 ? D : 128;    // dimensions that the warps' sums are joined at a time
     static constexpr int kPitch = kSumD + 4;           // floats of a row there, (maximum, denominator) at kSumD: stores without conflicts
     static constexpr uint32_t kSumBytes = kWarps * 8 * kPitch * 4, kJoinBytes = kPaMaxCtas * 16 * 8;
@@ -146,10 +147,12 @@ struct PaWalk {
     static constexpr uint32_t kRows = 8u * NT;         // of a group
     PagedReq rq;
     uint32_t r, h, rg, kb, b0, b1;                     // kb: blocks of the pair
+    uint32_t longest;                                  // pair that is not cut
     unsigned long long x, x_end;                       // blocks of all pairs before block b0, and where the CTA's range ends
     __device__ __forceinline__ static bool mine(const PagedAttn &a, const PagedReq &q) { return q.n * a.group > a.row_lo && q.n * a.group <= a.row_hi; }
     __device__ __forceinline__ static uint32_t key_blocks(const PagedReq &q) { return max(1u, (q.len + PaCfg<D>::kKeys - 1) / PaCfg<D>::kKeys); }
-    __device__ __forceinline__ void cut() { b1 = (uint32_t)min((unsigned long long)kb, b0 + (x_end - x)); }
+    __device__ __forceinline__ bool whole() const { return kb <= longest; }
+    __device__ __forceinline__ void cut() { b1 = whole() ? kb : (uint32_t)min((unsigned long long)kb, b0 + (x_end - x)); }
     __device__ __forceinline__ uint32_t after(const PagedAttn &a) const { return r + 1u == a.requests ? 0u : r + 1u; }
     // the next pair; ahead: what the next request has (requested earlier); false: there is none
     __device__ __forceinline__ bool next(const PagedAttn &a, const PagedReq &ahead)
@@ -244,6 +247,7 @@ k_attn_paged(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
     auto cta_of = [&](unsigned long long y) {          // the last c with part_of(c) <= y
         return W < 1u << 24 ? (((uint32_t)y + 1u) * N - 1u) / (uint32_t)W : (uint32_t)(((y + 1ull) * N - 1ull) / W);
     };
+    s.longest = W >= 3u * PaCfg<D>::kWhole * N ? 2u * PaCfg<D>::kWhole : max(PaCfg<D>::kWhole, 2u * (uint32_t)W / (3u * N));
     s.x = part_of(me);
     s.x_end = part_of(me + 1u);
     const unsigned long long x_begin = s.x;
@@ -264,7 +268,12 @@ k_attn_paged(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
         s.kb = Walk::key_blocks(s.rq);
         s.rg = off / s.kb;
         s.b0 = off - s.rg * s.kb;
-        s.cut();
+        if (s.b0 && s.whole()) {                       // the CTA before has all of it
+            s.b1 = s.kb;
+            if (!s.next(a, paged_req(a, s.after(a)))) return;
+        } else {
+            s.cut();
+        }
     }
     bool ok = true;
     if (wid >= (uint32_t)NW) {
@@ -626,23 +635,37 @@ k_attn_paged(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             if (sm_last) {
                 const uint32_t behind = part_of(c0) != x0 ? 1u : 0u;
                 auto slot_of = [&](uint32_t q) { return a.part + (size_t)(2u * q + (q == c0 ? behind : 0u)) * CF::kSlot; };
-                // what every part counts, for every row: all of the parts' numbers are requested at once
-                float2 *ml = (float2 *)sum;            // [parts][rows] (maximum, denominator)
-                for (uint32_t i = tid; i < parts * rows; i += CF::kCompute) ml[i] = __ldcg((const float2 *)(slot_of(c0 + i / rows) + 16 * D) + i % rows);
-                sync();
                 for (uint32_t it = tid; it < rows * (D / 4); it += CF::kCompute) {
                     const uint32_t m = it / (D / 4), d4 = it % (D / 4);
                     float M = -INFINITY, L = 0.f;
-                    for (uint32_t p = 0; p < parts; ++p) M = fmaxf(M, ml[p * rows + m].x);
-                    const float mb = M == -INFINITY ? 0.f : M * sl2;
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-                    for (uint32_t p = 0; p < parts; ++p) {
-                        const float4 u = __ldcg((const float4 *)(slot_of(c0 + p) + m * D) + d4);
-                        const float2 e = ml[p * rows + m];
-                        const float f = pa_exp2(fmaf(e.x, sl2, -mb));
-                        L = fmaf(e.y, f, L);
-                        v.x = fmaf(u.x, f, v.x); v.y = fmaf(u.y, f, v.y); v.z = fmaf(u.z, f, v.z); v.w = fmaf(u.w, f, v.w);
+                    constexpr uint32_t AT = 16;        // parts whose numbers are requested at once
+                    for (uint32_t p0 = 0; p0 < parts; p0 += AT) {
+                        float2 e[AT];
+                        float4 u[AT];
+                        float mx = M;
+#pragma unroll
+                        for (uint32_t i = 0; i < AT; ++i) {
+                            const float *from = slot_of(c0 + p0 + i);
+                            e[i] = make_float2(-INFINITY, 0.f);
+                            u[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (p0 + i < parts) {
+                                e[i] = __ldcg((const float2 *)(from + 16 * D) + m);
+                                u[i] = __ldcg((const float4 *)(from + m * D) + d4);
+                            }
+                        }
+#pragma unroll
+                        for (uint32_t i = 0; i < AT; ++i) mx = fmaxf(mx, e[i].x);
+                        const float mb = mx == -INFINITY ? 0.f : mx * sl2, f0 = pa_exp2(fmaf(M, sl2, -mb));
+                        M = mx;
+                        L *= f0;
+                        v.x *= f0; v.y *= f0; v.z *= f0; v.w *= f0;
+#pragma unroll
+                        for (uint32_t i = 0; i < AT; ++i) {
+                            const float f = pa_exp2(fmaf(e[i].x, sl2, -mb));
+                            L = fmaf(e[i].y, f, L);
+                            v.x = fmaf(u[i].x, f, v.x); v.y = fmaf(u[i].y, f, v.y); v.z = fmaf(u[i].z, f, v.z); v.w = fmaf(u[i].w, f, v.w);
+                        }
                     }
                     write_out(m, d4, v, L);
                 }
