@@ -260,7 +260,10 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     __syncthreads();
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    // Behind k_attn_paged this does not wait for it: the two share inputs only, and the other lets this one start when its own
+    // predecessors are complete.  CTAs come as the others leave (three chunks of prompts beside 29 single tokens: FIG us, 75 before);
+    // the wait is at the end, for those who rely on both.
+    if (!a.second) asm volatile("griddepcontrol.wait;" ::: "memory");
     // ---- every request's cost and units, of one KV head (over the ring, which is empty)
     uint32_t *first = (uint32_t *)(smem + CF::kRingOff), *units = first + kPaMaxRequests;
     const uint32_t R = a.requests, G = a.group, me = blockIdx.x;
@@ -338,6 +341,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
     if (me >= N) {
         if (tid == 0) cuts[me].parts = 0u;
         if (warp == CF::kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*tmem_slot), "r"(512u) : "memory");
+        if (a.second) asm volatile("griddepcontrol.wait;" ::: "memory");
         return;
     }
     PcWalk<D> w;
@@ -854,6 +858,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     }
+    if (a.second) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // The parts of the units that were cut.  grid (CTAs of k_attn_chunk, row tiles x groups of 16 dimensions), a thread per row; four parts

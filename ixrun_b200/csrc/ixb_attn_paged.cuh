@@ -40,6 +40,7 @@ struct PagedAttn {
     uint32_t requests, width, n_pages, log_page, rows, hq, hkv, group;
     uint32_t group_magic;                              // ceil(2^32 / group)
     uint32_t row_lo, row_hi;                           // requests with row_lo < q_len * group <= row_hi are taken
+    uint32_t second;                                   // behind the form for few rows, in one call
     float scale;
     __device__ __forceinline__ uint32_t by_group(uint32_t m) const { return group == 1u ? m : __umulhi(m, group_magic); }      // m / group, m * group < 2^32
 };
@@ -196,7 +197,6 @@ k_attn_paged(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
     float *sum = (float *)(pa_smem + CF::kRing);       // [NW][8][kPitch]; before that the blocks before every request
     uint32_t *first = (uint32_t *)sum;
     const uint32_t R = a.requests, G = a.group, page = 1u << a.log_page;
-    asm volatile("griddepcontrol.launch_dependents;");
     if (tid == 0) {
         for (int i = 0; i < ST; ++i) {
             asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(full0 + 8u * i) : "memory");
@@ -206,7 +206,9 @@ k_attn_paged(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
         asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
     }
+    // (in this order: what starts behind this launch may rely on what came before it, see k_attn_chunk)
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     // ---- the blocks before every request, of one KV head
     uint32_t total = 0;
     using Walk = PaWalk<D, NT>;
@@ -247,7 +249,7 @@ k_attn_paged(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
     auto cta_of = [&](unsigned long long y) {          // the last c with part_of(c) <= y
         return W < 1u << 24 ? (((uint32_t)y + 1u) * N - 1u) / (uint32_t)W : (uint32_t)(((y + 1ull) * N - 1ull) / W);
     };
-    s.longest = W >= 3u * PaCfg<D>::kWhole * N ? 2u * PaCfg<D>::kWhole : max(PaCfg<D>::kWhole, 2u * (uint32_t)W / (3u * N));
+    s.longest = PaCfg<D>::kWhole;
     s.x = part_of(me);
     s.x_end = part_of(me + 1u);
     const unsigned long long x_begin = s.x;

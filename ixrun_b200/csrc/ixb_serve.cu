@@ -104,9 +104,11 @@ constexpr uint32_t few_rows() { return D == 256 ? 8 : 16; }
 constexpr size_t kPaTicketBytes = 4096, kPaCutBytes = 8192;       // a word, a PcCut per CTA; the tickets are zero between launches
 
 template <int D>
-static size_t attn_part_bytes()                        // the two kernels run one after the other
+static size_t few_part_floats() { return (size_t)num_sms() * 2 * PaCfg<D>::kSlot; }
+template <int D>
+static size_t attn_part_bytes()                        // (the two kernels of a call overlap)
 {
-    return (size_t)num_sms() * 2 * 4 * std::max<size_t>(PaCfg<D>::kSlot, PcCfg<D>::kPart);
+    return 4 * (few_part_floats<D>() + (size_t)num_sms() * 2 * PcCfg<D>::kPart);
 }
 extern "C" size_t ixb_attn_paged_scratch_bytes(int64_t head_dim)
 {
@@ -152,10 +154,12 @@ static int attn_paged_run(PagedAttn a, PcCut *cuts, int64_t max_q, cudaStream_t 
         if (rc || few) return rc;
         a.row_lo = few_rows<D>();
         a.row_hi = 0xffffffffu;
+        a.part += few_part_floats<D>();
+        a.second = 1u;
     }
     static bool attr_set[64] = {false};
     IXB_CUDA(opt_in_smem(k_attn_chunk<D>, attr_set, (int)PcCfg<D>::kSmem));
-    // (a launch behind another one of this call may begin while that ends: it waits for it before it reads or writes anything)
+    // (launches of one call may begin while the one before ends)
     IXB_CUDA(launch_overlapped(both || pdl_on(), k_attn_chunk<D>, dim3(sms), dim3(PcCfg<D>::kThreads), PcCfg<D>::kSmem, st, a, kmap, vmap, cuts));
     if ((rc = launch_check("k_attn_chunk"))) return rc;
     IXB_GLUE("k_attn_chunk_join", launch_overlapped(true, k_attn_chunk_join<D>, dim3(sms, PcCfg<D>::kTiles * (D / 16)), dim3(128), 0, st, a, (const PcCut *)cuts));
