@@ -261,7 +261,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
     }
     __syncthreads();
     // Behind k_attn_paged this does not wait for it: the two share inputs only, and the other lets this one start when its own
-    // predecessors are complete.  CTAs come as the others leave (three chunks of prompts beside 29 single tokens: FIG us, 75 before);
+    // predecessors are complete.  CTAs come as the others leave (three chunks of prompts beside 29 single tokens: 64 us, 75 before);
     // the wait is at the end, for those who rely on both.
     if (!a.second) asm volatile("griddepcontrol.wait;" ::: "memory");
     // ---- every request's cost and units, of one KV head (over the ring, which is empty)

@@ -224,13 +224,29 @@ k_rope_paged(RopePaged s)
     const uint32_t row = blockIdx.x, part = threadIdx.x % PT, hl = threadIdx.x / PT;
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int32_t slot = s.slot[row];
-    const uint32_t p = min((uint32_t)max(s.pos[row], 0), s.max_seq - 1u);
-    if (slot < 0 || (size_t)slot >= s.n_slots) return;
     const uint32_t heads = s.hq + 2u * s.hkv, turned = s.rot / 16u;            // threads whose pieces are rotated
     const bool rot = part < turned;
     // elements a .. a + 7 and b .. b + 7 of a head
     const uint32_t a = rot ? 8u * part : s.rot + 16u * (part - turned), b = rot ? a + s.rot / 2u : a + 8u;
+    constexpr int UN = 4;                              // heads of a thread in flight
+    uint4 ra[UN], rb[UN];
+    auto fetch = [&](uint32_t h0) {
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            const uint32_t h = h0 + u * HL + hl;
+            ra[u] = rb[u] = make_uint4(0, 0, 0, 0);
+            if (h < heads) {
+                const __nv_bfloat16 *src = h < s.hq ? s.q + (size_t)row * s.q_stride + (size_t)h * D
+                                                    : (h < s.hq + s.hkv ? s.k + (size_t)(h - s.hq) * D : s.v + (size_t)(h - s.hq - s.hkv) * D) + (size_t)row * s.kv_stride;
+                ra[u] = *(const uint4 *)(src + a);
+                rb[u] = *(const uint4 *)(src + b);
+            }
+        }
+    };
+    fetch(0u);                                         // (beside the slot and the position: one trip to memory less)
+    const int32_t slot = s.slot[row];
+    const uint32_t p = min((uint32_t)max(s.pos[row], 0), s.max_seq - 1u);
+    if (slot < 0 || (size_t)slot >= s.n_slots) return;
     float c[8], sn[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -262,20 +278,8 @@ k_rope_paged(RopePaged s)
         }
         return make_uint4(w[0], w[1], w[2], w[3]);
     };
-    constexpr int UN = 4;                              // heads of a thread in flight
     for (uint32_t h0 = 0; h0 < heads; h0 += UN * HL) { // (the bound is the same for all threads: shuffles below)
-        uint4 ra[UN], rb[UN];
-#pragma unroll
-        for (int u = 0; u < UN; ++u) {
-            const uint32_t h = h0 + u * HL + hl;
-            ra[u] = rb[u] = make_uint4(0, 0, 0, 0);
-            if (h < heads) {
-                const __nv_bfloat16 *src = h < s.hq ? s.q + (size_t)row * s.q_stride + (size_t)h * D
-                                                    : (h < s.hq + s.hkv ? s.k + (size_t)(h - s.hq) * D : s.v + (size_t)(h - s.hq - s.hkv) * D) + (size_t)row * s.kv_stride;
-                ra[u] = *(const uint4 *)(src + a);
-                rb[u] = *(const uint4 *)(src + b);
-            }
-        }
+        if (h0) fetch(h0);
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
             const uint32_t h = h0 + u * HL + hl;
