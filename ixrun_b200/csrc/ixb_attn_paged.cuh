@@ -637,39 +637,51 @@ k_attn_paged(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             if (sm_last) {
                 const uint32_t behind = part_of(c0) != x0 ? 1u : 0u;
                 auto slot_of = [&](uint32_t q) { return a.part + (size_t)(2u * q + (q == c0 ? behind : 0u)) * CF::kSlot; };
-                for (uint32_t it = tid; it < rows * (D / 4); it += CF::kCompute) {
-                    const uint32_t m = it / (D / 4), d4 = it % (D / 4);
+                // Few rows: up to four threads share four dimensions' parts, four of which a thread requests at once.  (Short
+                // code: this is its first run in the launch, and it comes from memory.)
+                const uint32_t items = rows * (D / 4), split = 4u * items <= CF::kCompute ? 2u : 2u * items <= CF::kCompute ? 1u : 0u;
+#pragma unroll 1
+                for (uint32_t at = tid; at >> split < items; at += CF::kCompute) {     // (a warp's threads are in or out together)
+                    const uint32_t it = at >> split, m = it / (D / 4), d4 = it % (D / 4);
                     float M = -INFINITY, L = 0.f;
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                    constexpr uint32_t AT = 16;        // parts whose numbers are requested at once
-                    for (uint32_t p0 = 0; p0 < parts; p0 += AT) {
-                        float2 e[AT];
-                        float4 u[AT];
-                        float mx = M;
+#pragma unroll 1
+                    for (uint32_t p0 = at & ((1u << split) - 1u); p0 < parts; p0 += 4u << split) {
+                        float2 e[4];
+                        float4 u[4];
 #pragma unroll
-                        for (uint32_t i = 0; i < AT; ++i) {
-                            const float *from = slot_of(c0 + p0 + i);
-                            e[i] = make_float2(-INFINITY, 0.f);
-                            u[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                            if (p0 + i < parts) {
-                                e[i] = __ldcg((const float2 *)(from + 16 * D) + m);
-                                u[i] = __ldcg((const float4 *)(from + m * D) + d4);
+                        for (uint32_t i = 0; i < 4u; ++i) {
+                            const uint32_t p = p0 + (i << split);
+                            const float *from = slot_of(c0 + min(p, parts - 1u));
+                            e[i] = __ldcg((const float2 *)(from + 16 * D) + m);
+                            u[i] = __ldcg((const float4 *)(from + m * D) + d4);
+                            if (p >= parts) {
+                                e[i] = make_float2(-INFINITY, 0.f);
+                                u[i] = make_float4(0.f, 0.f, 0.f, 0.f);
                             }
                         }
-#pragma unroll
-                        for (uint32_t i = 0; i < AT; ++i) mx = fmaxf(mx, e[i].x);
-                        const float mb = mx == -INFINITY ? 0.f : mx * sl2, f0 = pa_exp2(fmaf(M, sl2, -mb));
+                        const float mx = fmaxf(fmaxf(fmaxf(e[0].x, e[1].x), fmaxf(e[2].x, e[3].x)), M), mb = mx == -INFINITY ? 0.f : mx * sl2;
+                        const float f0 = pa_exp2(fmaf(M, sl2, -mb));
                         M = mx;
                         L *= f0;
                         v.x *= f0; v.y *= f0; v.z *= f0; v.w *= f0;
 #pragma unroll
-                        for (uint32_t i = 0; i < AT; ++i) {
+                        for (uint32_t i = 0; i < 4u; ++i) {
                             const float f = pa_exp2(fmaf(e[i].x, sl2, -mb));
                             L = fmaf(e[i].y, f, L);
                             v.x = fmaf(u[i].x, f, v.x); v.y = fmaf(u[i].y, f, v.y); v.z = fmaf(u[i].z, f, v.z); v.w = fmaf(u[i].w, f, v.w);
                         }
                     }
-                    write_out(m, d4, v, L);
+#pragma unroll 1
+                    for (uint32_t d = 1u; d < 1u << split; d <<= 1) {
+                        const float mo = __shfl_xor_sync(0xffffffffu, M, d), mx = fmaxf(M, mo), mb = mx == -INFINITY ? 0.f : mx * sl2;
+                        const float f = pa_exp2(fmaf(M, sl2, -mb));
+                        M = mx;
+                        auto both = [&](float x) { x *= f; return x + __shfl_xor_sync(0xffffffffu, x, d); };
+                        L = both(L);
+                        v.x = both(v.x); v.y = both(v.y); v.z = both(v.z); v.w = both(v.w);
+                    }
+                    if ((at & ((1u << split) - 1u)) == 0u) write_out(m, d4, v, L);
                 }
             }
         }
