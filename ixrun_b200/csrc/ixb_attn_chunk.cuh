@@ -131,14 +131,14 @@ __device__ __forceinline__ uint64_t pc_pair(float lo, float hi)
 }
 __device__ __forceinline__ float pc_lo(uint64_t v)
 {
-    float lo, hi;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+    float lo;
+    asm("{\n\t.reg .f32 hi;\n\tmov.b64 {%0, hi}, %1;\n\t}" : "=f"(lo) : "l"(v));
     return lo;
 }
 __device__ __forceinline__ float pc_hi(uint64_t v)
 {
-    float lo, hi;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+    float hi;
+    asm("{\n\t.reg .f32 lo;\n\tmov.b64 {lo, %0}, %1;\n\t}" : "=f"(hi) : "l"(v));
     return hi;
 }
 __device__ __forceinline__ uint64_t pc_fma2(uint64_t a, uint64_t b, uint64_t c)
@@ -206,7 +206,7 @@ struct PcWalk {
                     r = 0;
                     ++h;
                 }
-                rq = paged_req(a, r);
+                rq = paged_req<true>(a, r);
             } while (!mine(a, rq) && h < a.hkv);       // (there is one, unless the lengths change under the kernel)
             if (h >= a.hkv) return false;
         }
@@ -284,7 +284,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
     const uint32_t per = (R + CF::kThreads - 1) / CF::kThreads, ra = min(R, tid * per), rb = min(R, ra + per);
     if (R <= 2u * CF::kThreads / 32u) {                // few requests, perhaps of many tiles: a warp each
         for (uint32_t r = (uint32_t)warp; r < R; r += CF::kThreads / 32) {
-            const PagedReq q = paged_req(a, r);
+            const PagedReq q = paged_req<true>(a, r);
             uint32_t own = 0;
             if (PcWalk<D>::mine(a, q))
                 for (uint32_t t = lane; t * CF::kUnitRows < q.n * G; t += 32u) own += cost_of(q, t);
@@ -293,7 +293,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
         }
     } else {
         for (uint32_t r = ra; r < rb; ++r) {
-            const PagedReq q = paged_req(a, r);
+            const PagedReq q = paged_req<true>(a, r);
             uint32_t own = 0;
             if (PcWalk<D>::mine(a, q))
                 for (uint32_t t = 0; t * CF::kUnitRows < q.n * G; ++t) own += cost_of(q, t);
@@ -358,7 +358,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
         }
         w.r = lo;
         off -= first[lo];
-        w.rq = paged_req(a, lo);
+        w.rq = paged_req<true>(a, lo);
         w.tile = 0;
         if (by_unit) {
             w.tile = off;
@@ -407,7 +407,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             const int32_t *pages = a.table + (size_t)w.r * a.width;
             auto page_of = [&](uint32_t kt) {
                 const uint32_t key = kt * kPcKeys + bk * bp;
-                return lane < boxes && kt < w.kt1 && key < w.u.keys ? pages[key >> a.log_page] : 0;
+                return lane < boxes && kt < w.kt1 && key < w.u.keys ? __ldcg(pages + (key >> a.log_page)) : 0;
             };
             int32_t page = page_of(w.kt0);
             for (uint32_t kt = w.kt0; kt < w.kt1 && ok; ++kt) {

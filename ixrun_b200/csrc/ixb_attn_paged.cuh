@@ -9,10 +9,10 @@
 // eight heads wastes none of it and its sums take half the registers of rows as M.
 //
 // Work: all (KV head, request, row group) pairs' blocks of keys in one line, cut into equal ranges, one per CTA, so lengths that differ
-// cost nothing.  A block is a slice of 16 keys per warp (32 with heads of 64, where a slice's softmax would take longer than its
+// cost nothing; a short pair is the CTA's that has its first block.  A block is a slice of 16 keys per warp (32 with heads of 64, where a slice's softmax would take longer than its
 // bytes).  One warp asks for the blocks (TMA, a box per page and 64 dimensions, 128-byte swizzle) in a ring of stages K, V, K, .., across
 // pairs; eight warps take their slices and keep a running softmax each, so they meet only where a pair ends, in shared memory.  A
-// pair that is cut leaves its parts in the scratch, and the CTA that comes last (a ticket) joins them in the order of the keys: the
+// long pair that is cut leaves its parts in the scratch, and the CTA that comes last (a ticket) joins them in the order of the keys: the
 // same bits every time.
 //
 // Precision: q K^T bf16 x bf16 in fp32; probabilities as two bf16 numbers whose sum they are to 17 bits; a slice's P V starts from
@@ -50,9 +50,12 @@ struct PagedReq {
     uint32_t row0, n, len;
     int32_t pos0;
 };
+// L2: from there, for k_attn_chunk, which may begin without a wait of its own
+template <bool L2 = false>
 __device__ __forceinline__ PagedReq paged_req(const PagedAttn &a, uint32_t r)
 {
-    const int32_t c0 = min(max(a.cu_rows[r], 0), (int32_t)a.rows), c1 = min(max(a.cu_rows[r + 1], 0), (int32_t)a.rows), l = a.length[r];
+    auto at = [](const int32_t *p) { return L2 ? __ldcg(p) : *p; };
+    const int32_t c0 = min(max(at(a.cu_rows + r), 0), (int32_t)a.rows), c1 = min(max(at(a.cu_rows + r + 1), 0), (int32_t)a.rows), l = at(a.length + r);
     PagedReq q;
     q.row0 = (uint32_t)c0;
     q.n = (uint32_t)max(c1 - c0, 0);
@@ -106,11 +109,13 @@ struct PaCfg {
     static constexpr uint32_t kStage = D / 64 * kSub * kPanel;     // K or V of a block: [128 keys][64 dimensions]
     static constexpr int kStages = 196608 / kStage;
     static constexpr uint32_t kRing = kStages * kStage;
-    static constexpr uint32_t kWhole = 4 * 65536 / (2 * kStage);       // blocks of a pair that is never cut (256 KB)
+    // Blocks of a pair that is not cut: 256 KB of keys and values.  A join is a CTA's 3 us and a CTA takes 64 KB in 0.45 us: 32 single
+    // tokens behind 300 keys 17.2 us cut, 11.4 whole; one behind 700 (six blocks) 7.3 cut, 8.6 whole.  A limit that grows with
+    // the call's size: 36.5 instead of 39 us for 64 tokens behind 700 keys, 65.4 instead of 64 for requests of unequal lengths.
+    static constexpr uint32_t kWhole = 4 * 65536 / (2 * kStage);
     static constexpr int kSumD = D < 128 ? D : 128;    // dimensions that the warps' sums are joined at a time
     static constexpr int kPitch = kSumD + 4;           // floats of a row there, (maximum, denominator) at kSumD: stores without conflicts
-    static constexpr uint32_t kSumBytes = kWarps * 8 * kPitch * 4, kJoinBytes = kPaMaxCtas * 16 * 8;
-    static constexpr uint32_t kSum = kSumBytes > kJoinBytes ? kSumBytes : kJoinBytes;
+    static constexpr uint32_t kSum = kWarps * 8 * kPitch * 4;
     static constexpr uint32_t kSmem = kRing + kSum + 2 * kStages * 8 + 64;     // (no static arrays: the ring starts on 1024 bytes)
     static constexpr uint32_t kSlot = 16 * D + 32;     // floats of a part: sums [16][D], (maximum, denominator) [16]
     static_assert(kSmem <= 227 * 1024 && kSum >= 4 * kPaMaxRequests, "fits");
@@ -148,11 +153,10 @@ struct PaWalk {
     static constexpr uint32_t kRows = 8u * NT;         // of a group
     PagedReq rq;
     uint32_t r, h, rg, kb, b0, b1;                     // kb: blocks of the pair
-    uint32_t longest;                                  // pair that is not cut
     unsigned long long x, x_end;                       // blocks of all pairs before block b0, and where the CTA's range ends
     __device__ __forceinline__ static bool mine(const PagedAttn &a, const PagedReq &q) { return q.n * a.group > a.row_lo && q.n * a.group <= a.row_hi; }
     __device__ __forceinline__ static uint32_t key_blocks(const PagedReq &q) { return max(1u, (q.len + PaCfg<D>::kKeys - 1) / PaCfg<D>::kKeys); }
-    __device__ __forceinline__ bool whole() const { return kb <= longest; }
+    __device__ __forceinline__ bool whole() const { return kb <= PaCfg<D>::kWhole; }
     __device__ __forceinline__ void cut() { b1 = whole() ? kb : (uint32_t)min((unsigned long long)kb, b0 + (x_end - x)); }
     __device__ __forceinline__ uint32_t after(const PagedAttn &a) const { return r + 1u == a.requests ? 0u : r + 1u; }
     // the next pair; ahead: what the next request has (requested earlier); false: there is none
@@ -249,7 +253,6 @@ k_attn_paged(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
     auto cta_of = [&](unsigned long long y) {          // the last c with part_of(c) <= y
         return W < 1u << 24 ? (((uint32_t)y + 1u) * N - 1u) / (uint32_t)W : (uint32_t)(((y + 1ull) * N - 1ull) / W);
     };
-    s.longest = PaCfg<D>::kWhole;
     s.x = part_of(me);
     s.x_end = part_of(me + 1u);
     const unsigned long long x_begin = s.x;
