@@ -46,8 +46,10 @@ struct PcCfg {
     static constexpr uint32_t kStages = D == 64 ? 8 : 5;
     static constexpr uint32_t kRingOff = kTiles * kQTile;
     static constexpr uint32_t kBarOff = kRingOff + kStages * kUnit;
-    static constexpr uint32_t kBars = 2 * kStages + 20;
-    static constexpr uint32_t kWalkOff = kBarOff + kBars * 8 + 1024 + 128;
+    static constexpr uint32_t kLook = 8;               // key tiles that may be looked through ahead
+    static constexpr uint32_t kBars = 2 * kStages + 13 + 2 * kLook;
+    static_assert(kStages / (2 * kNU) < kLook, "a barrier is not used again before its last phase was seen");
+    static constexpr uint32_t kWalkOff = kBarOff + kBars * 8 + 1024 + 192;
     static constexpr uint32_t kSmem = kWalkOff + kGroups * 4 * 80;             // no static arrays: stages start on 1024 bytes
     static constexpr int kSoftWarps = 4 * kGroups, kMmaWarp = kSoftWarps, kLoadWarp = kSoftWarps + 1, kScanWarp = kSoftWarps + 2, kThreads = (kSoftWarps + 4) * 32;
     // Registers of a thread: a softmax thread keeps a row of 128 scores.  With two groups of them the launch's 168 are dealt out
@@ -121,6 +123,12 @@ __device__ __forceinline__ void pc_pin(uint32_t *r)
 {
 #pragma unroll
     for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(r[i]));
+}
+__device__ __forceinline__ float pc_max3(float a, float b, float c)
+{
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 // two fp32 numbers in a register pair
 __device__ __forceinline__ uint64_t pc_pair(float lo, float hi)
@@ -229,12 +237,12 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
     const uint32_t tid = threadIdx.x, lane = tid & 31u;
     const int warp = __shfl_sync(0xffffffffu, (int)(tid >> 5), 0);
     const uint32_t ring = s0 + CF::kRingOff, full0 = s0 + CF::kBarOff, empty0 = full0 + 8u * CF::kStages, q_full = empty0 + 8u * CF::kStages,
-                   q_free = q_full + 8u, s_full0 = q_free + 8u, p_full0 = s_full0 + 16u, p_half0 = p_full0 + 16u, o_full0 = p_half0 + 16u, pv_done = o_full0 + 16u,
-                   done_bar = pv_done + 8u, w_full0 = done_bar + 8u, v_go0 = w_full0 + 32u;
+                   q_free = q_full + 8u, s_full0 = q_free + 8u, p_full0 = s_full0 + 16u, p_half0 = p_full0 + 16u, o_full0 = p_half0 + 16u, pv_done0 = o_full0 + 16u,
+                   done_bar = pv_done0 + 16u, w_full0 = done_bar + 8u, v_go0 = w_full0 + 8u * CF::kLook;
     float2 *sm_ml = (float2 *)(smem + CF::kBarOff + CF::kBars * 8);            // [128]
     uint32_t *tmem_slot = (uint32_t *)(sm_ml + 128), &sm_units = tmem_slot[1], &sm_two = tmem_slot[2], &sm_cost = tmem_slot[3], *sm_warp = tmem_slot + 8;
     volatile uint32_t *wild_s = tmem_slot + 4;         // [2]: the slot's P V is done by its softmax warps
-    volatile uint32_t *found = tmem_slot + 24;         // [4][2]: what the two warps found in the values of a key tile
+    volatile uint32_t *found = tmem_slot + 24;         // [kLook][2]: what the two warps found in the values of a key tile
     asm volatile("griddepcontrol.launch_dependents;");
     if (tid == 0) {
         auto init = [&](uint32_t bar, uint32_t n, uint32_t count) {
@@ -246,9 +254,9 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
         init(s_full0, 2u, 1u);
         init(p_full0, 4u, 4u);                         // (and p_half0)
         init(o_full0, 2u, 1u);
-        init(pv_done, 2u, 1u);
-        init(w_full0, 4u, 2u);
-        init(v_go0, 4u, 1u);
+        init(pv_done0, 3u, 1u);                        // (and done_bar)
+        init(w_full0, CF::kLook, 2u);
+        init(v_go0, CF::kLook, 1u);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
@@ -402,8 +410,9 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
         // ---- K and V of every key tile, in the order K0 V0 K1 V1 ..; a box is a page's (at most 128) keys and 64 dimensions
         const uint32_t bp = min(1u << a.log_page, kPcKeys), boxes = kPcKeys / bp * (CF::kUD / 64);
         const uint32_t bk = lane / (CF::kUD / 64), panel = lane % (CF::kUD / 64);      // of lane < boxes: keys bk * bp .., 64 dimensions
-        uint32_t n = 0;
+        uint32_t n = 0, n_look = 0;
         for (bool more = work; more && ok; more = w.next(a)) {
+            const uint32_t look0 = max(w.looked(a), w.kt0);
             const int32_t *pages = a.table + (size_t)w.r * a.width;
             auto page_of = [&](uint32_t kt) {
                 const uint32_t key = kt * kPcKeys + bk * bp;
@@ -429,6 +438,12 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
                                         "r"((i % CF::kNU) * CF::kUD + panel * 64u), "r"(w.h), "r"(row), "r"(page), "r"(bar) : "memory");
                     __syncwarp();
                 }
+                // (a parity of the ring's barriers alone does not tell a stage that is still to come from one two rounds before it: the
+                // warp that goes through all of them says when)
+                if (kt >= look0) {
+                    if (lane == 0 && ok) pc_arrive(v_go0 + 8u * (n_look % CF::kLook));
+                    ++n_look;
+                }
                 page = page_n;
             }
         }
@@ -441,10 +456,10 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
         if (CF::kDeal) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         uint32_t el;
         asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(el));
-        uint32_t n0 = 0, seg = 0, p0 = 0, p1 = 0, n_look = 0;      // before this segment: ring units, segments, steps of the two slots, tiles looked through
+        uint32_t n0 = 0, seg = 0, p0 = 0, p1 = 0;      // before this segment: ring units, segments, steps of the two slots
         for (bool more = work; more && ok; more = w.next(a), ++seg) {
             const bool two = w.u.weight == 2u;         // two row tiles: a key tile is two steps
-            const uint32_t tiles = w.kt1 - w.kt0, steps = two ? 2u * tiles : tiles, look0 = max(w.looked(a), w.kt0);
+            const uint32_t tiles = w.kt1 - w.kt0, steps = two ? 2u * tiles : tiles;
             auto wait = [&](uint32_t bar, uint32_t parity) {
                 ok = ok && pa_wait(bar, parity);
                 ok = __all_sync(0xffffffffu, ok);
@@ -476,13 +491,6 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
                     const bool last_use = !two || slot;
                     const uint32_t valid = w.u.keys > kt * kPcKeys ? min(kPcKeys, w.u.keys - kt * kPcKeys) : 0u;
                     const uint32_t p_par = ((slot ? p1 : p0) + (st >> 1)) & 1u;
-                    if (kt >= look0 && (!two || !slot)) {              // the values are there: they may be looked through
-#pragma unroll
-                        for (int c = 0; c < CF::kNU; ++c) wait(full0 + 8u * ((unit(j, 1u) + c) % CF::kStages), (unit(j, 1u) + c) / CF::kStages & 1u);
-                        if (!ok) break;
-                        if (el) pc_arrive(v_go0 + 8u * ((n_look + kt - look0) & 3u));
-                        __syncwarp();
-                    }
                     wait(p_half0 + 8u * slot, p_par);      // the first 64 keys' probabilities
                     if (!ok) break;
                     const bool wild = wild_s[slot] != 0u;
@@ -525,7 +533,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
                         if (last_use) pc_commit(el, empty0 + 8u * rs);
                     }
                     if (!ok) break;
-                    if (CF::kTiles == 1) pc_commit(el, pv_done);
+                    if (CF::kTiles == 1) pc_commit(el, pv_done0 + 8u * slot);
                     if (st + 1u == steps || (CF::kTiles == 2 && st + 2u == steps)) pc_commit(el, o_full0 + 8u * (CF::kTiles == 2 ? slot : 0u));
                     if (CF::kTiles == 2 && steps == 1u) pc_commit(el, o_full0 + 8u);       // (the other slot has no step)
                 }
@@ -534,7 +542,6 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             n0 += 2u * tiles * CF::kNU;
             p0 += (steps + 1u) >> 1;
             p1 += steps >> 1;
-            n_look += w.kt1 - min(w.kt1, look0);
         }
         pc_commit(el, done_bar);
     } else if (warp >= CF::kScanWarp) {
@@ -546,9 +553,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             for (uint32_t kt = max(w.looked(a), w.kt0); kt < w.kt1 && ok; ++kt, ++n_look) {
                 const uint32_t keys = min(kPcKeys, w.u.keys - kt * kPcKeys);
                 uint32_t big = 0;
-                // (a parity of the ring's barriers alone does not tell a stage that is still to come from one two rounds before it: the
-                // warp that goes through all of them says when)
-                ok = ok && pa_wait(v_go0 + 8u * (n_look & 3u), n_look >> 2 & 1u);
+                ok = ok && pa_wait(v_go0 + 8u * (n_look % CF::kLook), n_look / CF::kLook & 1u);
 #pragma unroll
                 for (int c = 0; c < CF::kNU; ++c) {
                     const uint32_t n = n0 + (2u * (kt - w.kt0) + 1u) * CF::kNU + c, rs = n % CF::kStages;
@@ -564,8 +569,8 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
                 ok = __all_sync(0xffffffffu, ok);
                 const bool any = __any_sync(0xffffffffu, pa_wild(big));
                 if (lane == 0) {
-                    found[(n_look & 3u) * 2u + half] = any;
-                    pc_arrive(w_full0 + 8u * (n_look & 3u));
+                    found[n_look % CF::kLook * 2u + half] = any;
+                    pc_arrive(w_full0 + 8u * (n_look % CF::kLook));
                 }
                 __syncwarp();
             }
@@ -576,7 +581,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
         // ---- softmax: group gr of four warps has a slot (heads of 256: both); a thread is a row
         const uint32_t gr = (uint32_t)warp >> 2, row_t = tid & 127u, lanes = ((uint32_t)warp & 3u) << 21;
         const float sl2 = a.scale * 1.4426950408889634f;
-        uint32_t c0s = 0, c1s = 0, pv_cnt = 0, seg = 0, n0 = 0, n_look = 0;       // before this segment: steps of the slots, of both, segments, ring units, tiles looked through
+        uint32_t c0s = 0, c1s = 0, seg = 0, n0 = 0, n_look = 0;   // before this segment: steps of the slots, segments, ring units, tiles looked through
         if (tid == 0) cuts[me].parts = 0u;
         // (the way through the units lies in shared memory between segments: beside a row of scores there is no room for it)
         PcWalk<D> *const kept = (PcWalk<D> *)(smem + CF::kWalkOff) + warp;
@@ -617,9 +622,17 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             float mb = -INFINITY, l = 0.f;             // the maximum that the sums are relative to (in units of log2), the denominator
             bool any = false;                          // (group uniform) the accumulator holds something
             const uint32_t stride = CF::kTiles == 2 ? 2u : 1u;
+            // One accumulator for both slots: the P V of the step before, done.  (Its slot's P V before that is: the scores that this warp
+            // has seen came behind it, so the parity tells.)
+            auto pv_of = [&](uint32_t of) { ok = ok && pa_wait(pv_done0 + 8u * (of & 1u), ((of & 1u ? c1s : c0s) + (of >> 1)) & 1u); };
             for (uint32_t st = CF::kTiles == 2 ? gr : 0u; st < steps; st += stride) {
                 const uint32_t slot = st & 1u, j = two ? st >> 1 : st, kt = kt0 + j, s_at = tmem + lanes + slot * 128u;
                 const int32_t key0 = (int32_t)(kt * kPcKeys);
+                auto before = [&]() {
+                    if (CF::kTiles == 2) return;
+                    pv_of(st - 1u);
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                };
                 ok = ok && pa_wait(s_full0 + 8u * slot, ((slot ? c1s : c0s) + (st >> 1)) & 1u);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 bool wild = false;
@@ -638,17 +651,14 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
                     }
                     float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int c = 0; c < 128; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(s[c]));
-                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
-                    if (CF::kTiles == 1 && st) {       // the accumulator is the step before's too
-                        ok = ok && pa_wait(pv_done, (pv_cnt + st - 1u) & 1u);
-                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    }
+                    for (int c = 0; c < 128; c += 2) mx[c / 2 & 3] = pc_max3(mx[c / 2 & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+                    const float top = pc_max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * sl2;
                     if (__any_sync(0xffffffffu, valid && top > mb + 8.f)) {    // (false for -inf; the first maximum of a row is larger than -inf)
                         const float mn = fmaxf(mb, top), f = pa_exp2(mb - (mn == -INFINITY ? 0.f : mn));
                         mb = mn;
                         l *= f;
                         if (any) {
+                            before();
 #pragma unroll 1
                             for (int c = 0; c < D / 32; ++c) {
                                 uint32_t o[32];
@@ -680,8 +690,8 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
                         if (half == 0) {
                             if (kt >= look0) {         // (group uniform)
                                 const uint32_t k = n_look + kt - look0;
-                                ok = ok && pa_wait(w_full0 + 8u * (k & 3u), k >> 2 & 1u);
-                                wild = found[(k & 3u) * 2u] | found[(k & 3u) * 2u + 1u];
+                                ok = ok && pa_wait(w_full0 + 8u * (k % CF::kLook), k / CF::kLook & 1u);
+                                wild = found[k % CF::kLook * 2u] | found[k % CF::kLook * 2u + 1u];
                             }
                             if (row_t == 0) wild_s[slot] = wild;
                             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -692,6 +702,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
                     la = pc_add2(la, lb);
                     l += pc_lo(la) + pc_hi(la);
                     if (wild) {
+                        if (any) before();
                         // P V of this tile for this thread's row: what the row does not see is left out
 #pragma unroll 1
                         for (int c = 0; c < D / 32; ++c) {
@@ -733,7 +744,6 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
                         pc_wait_st();
                     }
                 } else {
-                    if (CF::kTiles == 1 && st) ok = ok && pa_wait(pv_done, (pv_cnt + st - 1u) & 1u);        // (keeps up with the barrier's phases)
                     __syncwarp();
                     if (lane == 0) pc_arrive(p_half0 + 8u * slot);
                 }
@@ -742,7 +752,10 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
                 __syncwarp();
                 if (lane == 0) pc_arrive(p_full0 + 8u * slot);
             }
-            pv_cnt += steps;
+            if (CF::kTiles == 1) {
+                if (steps > 1u) pv_of(steps - 2u);
+                pv_of(steps - 1u);
+            }
             c0s += (steps + 1u) >> 1;
             c1s += steps >> 1;
             n0 += 2u * tiles * CF::kNU;
@@ -751,7 +764,6 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             asm volatile("" ::: "memory");
             w = *kept;
             ok = ok && pa_wait(o_full0 + 8u * gr, seg & 1u);
-            if (CF::kTiles == 1) ok = ok && pa_wait(pv_done, (pv_cnt - 1u) & 1u);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (!ok) l = __int_as_float(0x7fc00000);
             const bool whole = w.kt0 == 0u && w.kt1 == w.u.tiles;

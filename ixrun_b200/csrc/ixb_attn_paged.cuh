@@ -124,6 +124,12 @@ struct PaCfg {
 constexpr uint32_t kPaWaitLimit = 1u << 20;            // polls
 __device__ __forceinline__ bool pa_wait(uint32_t mbar, uint32_t parity)
 {
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+                 "selp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done) : "r"(mbar), "r"(parity) : "memory");
+    if (done) return true;
     for (uint32_t it = 0; it < kPaWaitLimit; ++it) {
         uint32_t done;
         asm volatile("{\n\t.reg .pred p;\n\t"
