@@ -508,6 +508,76 @@ def test_table_write_and_attention_together():
 
 
 # ------------------------------------------------------------------------------------------------ refusals
+@pytest.mark.parametrize("hq,hkv,d,page", [(16, 8, 128, 16), (8, 8, 64, 64), (12, 2, 256, 32)])
+def test_pairs_about_the_length_up_to_which_they_are_not_cut(hq, hkv, d, page):
+    """256 KB of a KV head's keys and values: 512 positions of 128 dimensions, 1024 of 64, 256 of 256; shorter and longer requests in
+    every order, few and many of them"""
+    edge = 65536 // d
+    near = [edge - 1, edge, edge + 1, edge + 128, 2 * edge, 2 * edge + 1, 3, 128, 129, 1]
+    for seed, lens in enumerate(([(1, edge + 1)], [(1, n) for n in near], [(1, n) for n in reversed(near)], [(1, near[7 * i % 10]) for i in range(70)],
+                                 [(1, 9 * edge), (1, 2), (1, edge), (0, 40), (1, 9 * edge + 5), (1, 17)])):
+        check_attn(batch(seed, lens, hq, hkv, d, page), hq, hkv, d, max_q=1)
+
+
+def test_captured_steps_of_changing_requests():
+    """tables, write and attention of a step as one graph of dependent launches, with chunks and single tokens side by side and other
+    numbers of new tokens at every replay: the bits of the same calls made one by one"""
+    from ixrun_b200.p6 import set_pdl
+    from ixrun_b200.paged import AttnPaged, PageStep, page_step, rope_kv_paged
+
+    hq, hkv, d, page, requests, rows, n_pages, width = 16, 8, 64, 16, 9, 400, 400, 60
+    g = torch.Generator(device=DEV).manual_seed(3)
+    rnd = lambda *s: torch.randn(*s, generator=g, device=DEV).bfloat16()  # noqa: E731
+    ang = torch.arange(width * page, device=DEV)[:, None] * 10000.0 ** (-torch.arange(d // 2, device=DEV) / (d // 2))
+    cos, sin = ang.cos(), ang.sin()
+    qkv = rnd(rows, (hq + 2 * hkv) * d)
+    steps = [[1, 300, 0, 5, 1, 17, 1, 1, 40], [1] * requests, [200, 1, 1, 1, 150, 1, 0, 1, 20], [0, 0, 1, 0, 0, 0, 0, 0, 0], [3, 1, 1, 2, 1, 1, 90, 1, 1]]
+
+    def new():
+        st = PageStep.empty(requests, rows, DEV)
+        state = {"length": torch.zeros(requests, dtype=torch.int32, device=DEV), "table": torch.full((requests, width), -1, dtype=torch.int32, device=DEV),
+                 "free": torch.arange(n_pages, dtype=torch.int32, device=DEV), "n_free": on_gpu([n_pages]), "q_len": on_gpu([0] * requests),
+                 "k": torch.zeros(n_pages, page, hkv, d, dtype=torch.bfloat16, device=DEV), "out": torch.zeros(rows, hq * d, dtype=torch.bfloat16, device=DEV)}
+        state["v"] = torch.zeros_like(state["k"])
+        state["step"] = st._replace(length=state["length"], n_free=state["n_free"])
+        state["attn"] = AttnPaged(hq, hkv, d, DEV)
+        state["q"] = torch.zeros(rows, hq * d, dtype=torch.bfloat16, device=DEV)
+        return state
+
+    def once(s, wait):
+        q, k, v = qkv[:, :hq * d], qkv[:, hq * d:(hq + hkv) * d], qkv[:, (hq + hkv) * d:]
+        page_step(s["q_len"], s["length"], s["table"], s["free"], s["n_free"], page, rows, out=s["step"])
+        wait()
+        rope_kv_paged(q, k, v, s["step"].pos, s["step"].slot, s["k"], s["v"], cos, sin, hq, hkv, d, out=s["q"])
+        wait()
+        s["attn"](s["q"], s["k"], s["v"], s["table"], s["length"], s["step"].cu_rows, out=s["out"])
+        wait()
+
+    plain, fast = new(), new()
+    prev = set_pdl(True)
+    try:
+        once(fast, lambda: None)                       # (nothing new: no row)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            once(fast, lambda: None)
+        for i in range(20):
+            n_new = on_gpu(steps[i % len(steps)] if i < 12 else [1] * requests)
+            fast["q_len"].copy_(n_new)
+            graph.replay()
+    finally:
+        torch.cuda.synchronize()
+        set_pdl(prev)
+    got = {n: fast[n].clone() for n in ("length", "n_free", "k", "v", "out")}
+    for i in range(20):
+        plain["q_len"].copy_(on_gpu(steps[i % len(steps)] if i < 12 else [1] * requests))
+        once(plain, torch.cuda.synchronize)
+        assert plain["step"].status[0].item() == 0
+    for n, t in got.items():
+        assert torch.equal(t, plain[n]), n
+    assert got["out"].float().abs().sum() > 0
+
+
 def test_refusals():
     from ixrun_b200 import _lib
     from ixrun_b200.paged import AttnPaged, PageStep, PageTables, page_release, page_step, rope_kv_paged
