@@ -34,6 +34,18 @@ def __getattr__(name):
         from . import p6
 
         return getattr(p6, name)
+    if name in ("PageStep", "page_step", "page_release", "PageTables", "rope_kv_paged", "AttnPaged"):
+        from . import paged
+
+        return getattr(paged, name)
+    if name == "apply_rules":
+        from . import logits
+
+        return logits.apply_rules
+    if name in ("PackedLlama", "BatchedGreedyDecoder", "Verifier", "PagedDecoder"):
+        from . import llama_runner
+
+        return getattr(llama_runner, name)
     if name == "PeerAllReduce":
         from . import parallel
 

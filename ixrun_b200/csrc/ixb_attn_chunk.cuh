@@ -21,6 +21,14 @@
 // multiplied beyond.  A value that is not finite counts for the rows that see it and for no other: where a key tile is not
 // seen by all rows, two warps look for such values, and the softmax warps take the tile's P V themselves if there is one.
 //
+// Bound: the tensor core for long chunks, with the exponentials (one per score, 16 a cycle and SM) close behind: 2048 rows of a prompt
+// behind 12000 keys, 16 / 8 heads of 128: 192 us, 69 % of cuBLAS's rate on their products; the tensor pipe and the special function
+// unit are each busy 45 % of the time, the rest is the chain scores, maximum, exponentials, P V.  Fixed: 10 us for a launch, the
+// first keys, the cut units' ends and the join.  Built and slower for that chunk: steps of 64 keys in slots of their own, so that
+// scores wait for no P V (224 us: Q K^T of 64 columns is bound by Q's reads, and a step's overheads come twice), these with two sets
+// of softmax warps that take steps in turn (228), an MMA warp per group (248: the groups then run in step and want the
+// exponentials at the same time; one warp keeps them apart), a quarter of the exponentials as polynomials (214).
+//
 // Every wait on an mbarrier is bounded and counts this CTA's own copies and products; where one runs out the CTA's outputs
 // become NaN, and it carries on to its end with nothing in flight and tensor memory released.
 #pragma once

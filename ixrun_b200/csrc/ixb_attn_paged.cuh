@@ -4,7 +4,8 @@
 //   out = softmax(scale * q . K[0 .. position]) V[0 .. position]
 //
 // A request's rows of one KV head are packed, row t * G + g, eight or sixteen to a group, so a key is read once for all of them.
-// Bound: HBM, every key and value once; mma.sync is used as an instruction that multiplies eight rows at a time: keys (or
+// Bound: HBM, every key and value once: 64 single tokens behind 3000 to 6000 keys, 16 / 8 heads of 128, take 184 us, 98 % of the copy rate;
+// one behind 1100 takes 7.7 us, a chain of trips to memory (lengths, table, keys, ticket, parts).  mma.sync is used as an instruction that multiplies eight rows at a time: keys (or
 // dimensions of values) are its M = 16, rows its N = 8, S^T = K Q^T and O^T = V^T P^T, so that a single token of a group of up to
 // eight heads wastes none of it and its sums take half the registers of rows as M.
 //

@@ -73,7 +73,8 @@ struct PageStep {
 
 // One cluster of up to eight CTAs.  Every CTA sums the requests up for itself (a few thousand numbers at most), a barrier of the
 // cluster lies between the last read of what is updated in place and the first write, and the rows and new pages are shared out
-// over all threads.  Latency is all there is: 200 KB of output for the largest steps.  Figures in the table of operators.
+// over all threads.  Latency is all there is: 200 KB of output for the largest steps.  3.6 us for 40 single tokens, 6.9 for 512 requests
+// with 16700 new tokens (13 with one CTA).
 //
 // A step that does not fit (too few free pages, rows or table entries) takes nothing: cu_rows is zero, no row has a slot, lengths
 // and stack stay; status says why.
@@ -215,7 +216,8 @@ struct RopePaged {
 // One CTA per row: D / 16 threads take a head (two pieces of eight elements each: a rotated pair of pieces, or two that pass
 // through), the CTA's HL heads at a time, so that a row's tables are read once.  Everything is held in fp32 and rounded to bf16
 // once (the static cache's kernel rounds where the eager path holds bf16 tensors).  A row without a slot (-1, or outside the pool)
-// is left alone.  Bound: HBM, each element read once and written once.
+// is left alone.  Bound: HBM, each element read once and written once: 7700 rows of 24 / 4 heads of 256 with norms take 50.6 us, 77 % of
+// the copy rate (five CTAs an SM, each with one row in flight; six with fewer registers: 51.6).
 template <int D>
 __global__ void __launch_bounds__(128)
 k_rope_paged(RopePaged s)

@@ -723,7 +723,8 @@ class PagedDecoder:
     @torch.no_grad()
     def step(self, max_rows: int = PackedLlama.PREFILL_ROWS) -> torch.Tensor:
         """Feeds the requests what they have, at most max_rows rows in all: single tokens first, then prompts in the order of
-        their numbers.  Returns tokens int64 [requests], -1 for those without a new one (a static tensor)."""
+        their numbers.  Returns tokens int64 [requests], -1 for those without a new one (a static tensor).  RuntimeError, and
+        nothing launched, where there is nothing to feed, a request has all max_seq tokens, or the pages do not suffice."""
         left, q_len = int(max_rows), [0] * self.b
         todo = {r: n - self._cached[r] for r, n in enumerate(self._known) if n is not None}
         for r in sorted(todo, key=lambda r: (todo[r] > 1, r)):

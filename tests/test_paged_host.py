@@ -84,3 +84,15 @@ def test_ctypes_arguments_match_the_names_here():
         assert len(types) == len(args), name
         for t, (key, value) in zip(types, args.items()):
             assert (t in (ctypes.c_float,)) == isinstance(value, float), (name, key)
+
+
+def test_names_of_the_package():
+    import ixrun_b200
+    from ixrun_b200 import llama_runner, logits, paged
+
+    for name in paged.__all__:
+        assert getattr(ixrun_b200, name) is getattr(paged, name)
+    assert ixrun_b200.apply_rules is logits.apply_rules
+    assert ixrun_b200.PagedDecoder is llama_runner.PagedDecoder
+    with pytest.raises(AttributeError):
+        ixrun_b200.no_such_name
