@@ -1,8 +1,8 @@
 // Causal attention of every request's new tokens over its pages: the form for many rows (chunks of prompts), on tcgen05.
 // Formulas and packing of rows as in ixb_attn_paged.cuh.
 //
-//   CTA      one per SM; a range of key tiles (128 keys) out of all (KV head, request, row tile) units' in one line, equal in cost, so
-//            lengths that differ cost nothing.  A unit that is cut leaves its parts in the scratch, k_attn_chunk_join adds them up.
+//   CTA      one per SM; a range of key tiles (128 keys) out of all (KV head, request, row tile) units' in one line, equal in cost (a
+//            unit's end has its own, behind its tiles), so lengths that differ cost nothing.  A unit that is cut leaves its parts in the scratch, k_attn_chunk_join adds them up.
 //   unit     128 or 256 packed rows (128 with heads of 256) of one request and KV head
 //   step     Q K^T of 128 rows and a key tile into tensor memory (S), softmax in registers (a thread is a row), the probabilities as
 //            bf16 over S in tensor memory, P V into the accumulator there.  Two steps are in flight in two slots: the two row tiles
@@ -52,6 +52,10 @@ struct PcCfg {
     static constexpr uint32_t kUnit = kUD / 64 * kPanel;
     static constexpr uint32_t kQTile = D / 64 * kPanel;
     static constexpr uint32_t kStages = D == 64 ? 8 : 5;
+    // Cost of a unit's end and the next one's start, in steps of 128 rows and a key tile: without it CTAs with ends of two units are the last
+    // (a prompt of 2048 tokens from its start, 16 / 8 heads of 128: 48.2 us with 0, 41.1 with 2, 39.4 with 4, 35.7 with 6, 36.6 with 8;
+    // drafts of heads of 256, whose steps are longer: 50.9 with 0, 47.6 with 1, 49.9 with 2).
+    static constexpr uint32_t kEnd = D == 256 ? 1 : 6;
     static constexpr uint32_t kRingOff = kTiles * kQTile;
     static constexpr uint32_t kBarOff = kRingOff + kStages * kUnit;
     static constexpr uint32_t kLook = 8;               // key tiles that may be looked through ahead
@@ -212,7 +216,7 @@ struct PcWalk {
     // the next segment; false: there is none
     __device__ __forceinline__ bool next(const PagedAttn &a)
     {
-        x += by_unit ? 1ull : (unsigned long long)(kt1 - kt0) * u.weight;
+        x += by_unit ? 1ull : (unsigned long long)(kt1 - kt0) * u.weight + (kt1 == u.tiles ? PcCfg<D>::kEnd : 0u);
         if (x >= x_end) return false;
         kt0 = 0;
         if (++tile * PcCfg<D>::kUnitRows >= rq.n * a.group) {
@@ -286,7 +290,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
     auto cost_of = [&](const PagedReq &q, uint32_t t) {
         if (t * CF::kUnitRows >= q.n * G) return 0u;
         const PcUnit u = pc_unit<D>(a, q, t);
-        return u.tiles * u.weight;
+        return u.tiles * u.weight + CF::kEnd;
     };
     auto note = [&](uint32_t r, const PagedReq &q, uint32_t cost) {
         const uint32_t n = cost ? (q.n * G + CF::kUnitRows - 1u) / CF::kUnitRows : 0u;
@@ -319,7 +323,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
     __syncthreads();
     // What the line is cut into: key tiles; or whole units where there is room for one per CTA and they are short, so that cutting them
     // would cost more than it saves (300 rows of a prompt, 16 / 8 heads of 128: 24 us cut, 16.8 whole)
-    const bool by_unit = (unsigned long long)sm_units * a.hkv <= gridDim.x && sm_cost <= kPcShortUnit * sm_units;
+    const bool by_unit = (unsigned long long)sm_units * a.hkv <= gridDim.x && sm_cost <= (kPcShortUnit + CF::kEnd) * sm_units;
     const uint32_t total = by_unit ? sm_units : sm_cost;
     {
         const uint32_t *const own_of = by_unit ? units : first;
@@ -399,8 +403,8 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             off -= __shfl_sync(0xffffffffu, v, 31);
         }
         w.u = pc_unit<D>(a, w.rq, w.tile);
-        w.kt0 = (off + w.u.weight - 1u) / w.u.weight;  // a tile that began before this range is its predecessor's
-        w.x += w.kt0 * w.u.weight - off;
+        w.kt0 = min((off + w.u.weight - 1u) / w.u.weight, w.u.tiles);          // a tile that began before this range is its predecessor's
+        w.x = w.x - off + w.kt0 * w.u.weight;
         w.kt1 = w.kt0;
         if (w.kt0 < w.u.tiles && w.x < w.x_end) w.cut();
     }
