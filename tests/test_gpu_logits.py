@@ -155,6 +155,29 @@ def test_a_graph_takes_what_the_history_has_become():
     assert torch.equal(out, want) and torch.equal(token, t)
 
 
+@pytest.mark.parametrize("b,v", [(1, 1), (4096, 33), (3, 393216), (2, 31), (300, 5001)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_smallest_and_largest_sizes_and_empty_rules(b, v, dtype):
+    from ixrun_b200.logits import apply_rules
+
+    x = torch.randn(b, v, generator=torch.Generator(device="cuda").manual_seed(b), device="cuda").to(dtype)
+    f, token = x.float(), torch.empty(b, dtype=torch.int64, device="cuda")
+    none, zero = torch.empty(b, 0, dtype=torch.int32, device="cuda"), torch.zeros(b, dtype=torch.int32, device="cuda")
+    best = (f == f.max(1, keepdim=True).values).int().argmax(1)                # the lowest index of the largest value
+    for rules in ({}, {"history": none, "n_tokens": zero}, {"bias_ids": none, "bias_values": none.float()},
+                  {"mask": torch.empty(0, (v + 31) // 32, dtype=torch.int32, device="cuda"), "mask_row": zero - 1}):
+        token.fill_(-7)
+        assert torch.equal(apply_rules(x, token=token, **rules), f)
+        assert torch.equal(token, best)
+    # a history that is shorter than its lengths say, with numbers outside the vocabulary
+    h = torch.randint(-5, v + 5, (b, 9), dtype=torch.int32, device="cuda")
+    got = apply_rules(x, h, zero + 100, zero + 3, presence=torch.ones(b, device="cuda"))
+    want = f.clone()
+    for i in range(b):
+        want[i, sorted({t for t in h[i, 3:].tolist() if 0 <= t < v})] -= 1.0
+    assert torch.equal(got, want)
+
+
 def test_refusals():
     from ixrun_b200 import _lib
     from ixrun_b200.logits import apply_rules

@@ -519,6 +519,33 @@ def test_pairs_about_the_length_up_to_which_they_are_not_cut(hq, hkv, d, page):
         check_attn(batch(seed, lens, hq, hkv, d, page), hq, hkv, d, max_q=1)
 
 
+@pytest.mark.parametrize("lens,hq,hkv,d,max_q", [
+    ([(1, 1 + i % 37) for i in range(4096)], 4, 2, 64, 1),                     # as many requests as there may be
+    ([(1 if i % 9 else 12, 12 + i % 37) for i in range(2000)], 4, 2, 64, None),
+    ([(0, 5)] * 4000 + [(70, 90)] + [(0, 0)] * 95, 4, 2, 128, None),
+    ([(1, 300), (1, 7), (3, 140)], 256, 1, 64, None),                          # more query heads of a KV head than rows of a tile
+    ([(1, 300)], 130, 1, 64, 1),
+    ([(2, 300), (1, 9)], 33, 1, 256, None),
+    ([(129, 129)] * 30, 2, 1, 128, None),                                      # units with one row in their second tile
+    ([(1000, 1100), (1000, 1000)], 3, 3, 256, None),
+], ids=lambda v: f"{len(v)}x{v[-1][0]}" if isinstance(v, list) else None)
+def test_many_requests_and_large_groups(lens, hq, hkv, d, max_q):
+    check_attn(batch(1, lens, hq, hkv, d, 16), hq, hkv, d, max_q=max_q)
+
+
+@pytest.mark.parametrize("requests,rows", [(1, 0), (1, 1), (4096, 0), (4096, 5000)])
+def test_tables_of_one_page_and_steps_without_rows(requests, rows):
+    from ixrun_b200.paged import PageTables
+
+    t = PageTables(requests, 5000, 16, 1, DEV)
+    st = t.step(on_gpu([0] * requests), rows)
+    assert st.status.tolist() == [0, 0] and (st.slot == -1).all() and (st.cu_rows == 0).all()
+    if rows:
+        st = t.step(on_gpu([1] * requests), rows)
+        assert st.status.tolist() == [0, requests] and st.owner[:requests].tolist() == list(range(requests)) and (st.owner[requests:] == -1).all()
+        assert t.n_free.item() == 5000 - requests and len(set(st.slot[:requests].tolist())) == requests
+
+
 def test_captured_steps_of_changing_requests():
     """tables, write and attention of a step as one graph of dependent launches, with chunks and single tokens side by side and other
     numbers of new tokens at every replay: the bits of the same calls made one by one"""
