@@ -328,7 +328,7 @@ PyObject *rope_paged(PyObject *, PyObject *const *a, Py_ssize_t nargs)
     if (a[13] != Py_None && (!take(a[13], qn, bf, dev) || !qn.is_contiguous() || qn.numel() != d)) Py_RETURN_NONE;
     if (a[14] != Py_None && (!take(a[14], kn, bf, dev) || !kn.is_contiguous() || kn.numel() != d)) Py_RETURN_NONE;
     if (rq.rows < 1 || rk.rows != rq.rows || rv.rows != rq.rows || ro.rows != rq.rows || rk.cols != hkv * d || rv.cols != rk.cols || rv.pitch != rk.pitch ||
-        rq.cols < hq * d || ro.cols < hq * d || pos.numel() < rq.rows || slot.numel() < rq.rows || n2 != pages || p2 != page || !cs.is_contiguous() ||
+        rq.cols < hq * d || (a[16] != a[0] && ro.cols != hq * d) || pos.numel() < rq.rows || slot.numel() < rq.rows || n2 != pages || p2 != page || !cs.is_contiguous() ||
         !sn.is_contiguous() || cs.dim() != 2 || sn.dim() != 2 || cs.size(1) != rot / 2 || cs.size(0) < 1 || cs.sizes() != sn.sizes())
         Py_RETURN_NONE;
     const float eps = (float)PyFloat_AS_DOUBLE(a[15]);

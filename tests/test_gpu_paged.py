@@ -646,3 +646,20 @@ def test_refusals():
     for bad in (dict(q=b(3, 260)[:, :256]), dict(q=b(3, 264)[:, 4:260])):
         with pytest.raises(_lib.IxbError):                          # rows of q that do not start on 16 bytes
             attn(**{**ok, **bad})
+
+
+def test_rope_kv_paged_refuses_an_output_of_other_columns():
+    from ixrun_b200.paged import rope_kv_paged
+
+    hq, hkv, d = 4, 2, 64
+    q, k, v = (torch.ones(3, n * d, dtype=torch.bfloat16, device=DEV) for n in (hq + 1, hkv, hkv))
+    pool = torch.zeros(2, 16, hkv, d, dtype=torch.bfloat16, device=DEV)
+    cos = torch.ones(9, d // 2, device=DEV)
+    args = (k, v, on_gpu([0, 1, 2]), on_gpu([0, 1, 2]), pool, pool.clone(), cos, cos, hq, hkv, d)
+    for columns in (hq - 1, hq + 1):
+        with pytest.raises(ValueError):
+            rope_kv_paged(q, *args, out=torch.zeros(3, columns * d, dtype=torch.bfloat16, device=DEV))
+    assert (pool == 0).all()
+    assert rope_kv_paged(q, *args) is q                # in place, in the first columns
+    # 1 * 1 - 1 * 1 and 1 * 1 + 1 * 1
+    assert (q[:, hq * d:] == 1).all() and (pool[0, :3, :, :d // 2] == 0).all() and (pool[0, :3, :, d // 2:] == 2).all()
