@@ -2,7 +2,8 @@
 // Formulas and packing of rows as in ixb_attn_paged.cuh.
 //
 //   CTA      one per SM; a range of key tiles (128 keys) out of all (KV head, request, row tile) units' in one line, equal in cost (a
-//            unit's end has its own, behind its tiles), so lengths that differ cost nothing.  A unit that is cut leaves its parts in the scratch, k_attn_chunk_join adds them up.
+//            unit's end has its own, behind its tiles), so lengths that differ cost nothing.  A unit that is cut leaves its parts in the
+//            scratch, k_attn_chunk_join adds them up.
 //   unit     128 or 256 packed rows (128 with heads of 256) of one request and KV head
 //   step     Q K^T of 128 rows and a key tile into tensor memory (S), softmax in registers (a thread is a row), the probabilities as
 //            bf16 over S in tensor memory, P V into the accumulator there.  Two steps are in flight in two slots: the two row tiles
@@ -14,7 +15,7 @@
 //                            not finite
 //
 // The accumulator is rescaled only when a row's maximum has grown by more than 2^8 (a running maximum that lags changes no ratio).
-// Precision: scores and sums fp32, probabilities bf16 for P V (half a step 2^-9 of each, as the result's own rounding; the tensor
+// Precision: scores and sums fp32, probabilities bf16 for P V (half a step, 2^-8 of each, as the result's own rounding; the tensor
 // core takes no wider operand beside bf16 values), their sum from the fp32 values.
 //
 // Keys that no row of the unit sees are not read; the rows of V behind the last key are zeroed up to a multiple of 16 and not
@@ -22,7 +23,7 @@
 // seen by all rows, two warps look for such values, and the softmax warps take the tile's P V themselves if there is one.
 //
 // Bound: the tensor core for long chunks, with the exponentials (one per score, 16 a cycle and SM) close behind: 2048 rows of a prompt
-// behind 12000 keys, 16 / 8 heads of 128: 192 us, 69 % of cuBLAS's rate on their products; the tensor pipe and the special function
+// behind 12000 keys, 16 / 8 heads of 128: 192 us, 69 % of the measured rate of dense products; the tensor pipe and the special function
 // unit are each busy 45 % of the time, the rest is the chain scores, maximum, exponentials, P V.  Fixed: 10 us for a launch, the
 // first keys, the cut units' ends and the join.  Built and slower for that chunk: steps of 64 keys in slots of their own, so that
 // scores wait for no P V (224 us: Q K^T of 64 columns is bound by Q's reads, and a step's overheads come twice), these with two sets

@@ -83,7 +83,8 @@ extern "C" int ixb_rope_paged(const void *q, const void *k, const void *v, const
     const RopePaged s = {(const __nv_bfloat16 *)q, (const __nv_bfloat16 *)k, (const __nv_bfloat16 *)v, (__nv_bfloat16 *)out, (__nv_bfloat16 *)k_pages,
                          (__nv_bfloat16 *)v_pages, pos, slot, (const __nv_bfloat16 *)q_norm, (const __nv_bfloat16 *)k_norm, cos_tab, sin_tab,
                          (uint32_t)hq, (uint32_t)hkv, (uint32_t)rot_dim, (uint32_t)max_seq, log_page(page), eps, (size_t)q_stride, (size_t)kv_stride,
-                         (size_t)out_stride, (size_t)k_page_stride, (size_t)v_page_stride, (size_t)(n_pages * page)};
+                         (size_t)out_stride, (size_t)k_page_stride, (size_t)v_page_stride, (size_t)(n_pages * page),
+                         (uint32_t)(2 * num_sms())};
     const uintptr_t all = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)out | (uintptr_t)q_norm |
                           (uintptr_t)k_norm | (uintptr_t)cos_tab | (uintptr_t)sin_tab;
     const cudaStream_t st = (cudaStream_t)stream;
