@@ -416,7 +416,8 @@ int ixb_gdn_conv_step(const void *qkv_raw_device, void *conv_state_device, const
  * ixb_attn_paged: causal attention of the new tokens of all requests, keys and values already in their pages: row
  *   cu_rows[r] + t of q [rows] (row pitch q_stride elements, heads contiguous) is token length[r] - (cu_rows[r + 1] -
  *   cu_rows[r]) + t of request r and sees the positions up to its own.  out [rows][hq][head_dim]; rows that belong to no
- *   request are left as they are, rows that see no position become zero.  max_q: the most new tokens that a request may
+ *   request are left as they are, rows that see no position become zero.  Positions that the table has no entry for (a
+ *   length above width * page) are seen by nobody.  max_q: the most new tokens that a request may
  *   have, by which kernels are chosen (results do not need it to be true).  A page number outside the pool counts as a page
  *   of zeros.  head_dim 64, 128 or 256; scale positive; pointers 16-byte aligned.  scratch: ixb_attn_paged_scratch_bytes of the current
  *   device, the first 4096 bytes of it zero before the first call and left zero by every call (a buffer of its own for

@@ -627,9 +627,10 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             // ---- this thread's row
             const uint32_t m = (two ? gr * 128u : 0u) + row_t;                 // in the unit
             const bool valid = m < w.u.rows;
-            const int32_t limit = valid ? w.rq.pos0 + (int32_t)a.by_group(m0 + m) : -1;
+            // (the last position that it sees: of those that the table holds, what lies behind them in the tile was not copied)
+            const int32_t len1 = (int32_t)w.rq.len - 1, limit = valid ? min(w.rq.pos0 + (int32_t)a.by_group(m0 + m), len1) : -1;
             const bool warp_on = (m & ~31u) < w.u.rows;                        // (warp uniform) some row is there
-            const int32_t low_warp = w.rq.pos0 + (int32_t)a.by_group(m0 + (m & ~31u));
+            const int32_t low_warp = min(w.rq.pos0 + (int32_t)a.by_group(m0 + (m & ~31u)), len1);
             const uint32_t look0 = max(w.looked(a), w.kt0);
             const uint32_t o_at = tmem + lanes + CF::kO + (CF::kTiles == 2 ? gr * 128u : 0u);
             float mb = -INFINITY, l = 0.f;             // the maximum that the sums are relative to (in units of log2), the denominator

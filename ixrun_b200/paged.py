@@ -221,9 +221,10 @@ class AttnPaged:
     def __call__(self, q, k_pages, v_pages, table, length, cu_rows, max_q: int | None = None, out=None, scale: float | None = None):
         """q [rows, >= hq*head_dim] (column slices allowed): rows cu_rows[r] .. cu_rows[r+1] - 1 are the newest tokens of request r, which
         has length[r] tokens (these among them) on the pages table [R, width] of the pools [pages, page, hkv, head_dim]; length [R],
-        cu_rows [R+1], table: int32.  Every row attends to the positions up to its own.  max_q: the most new tokens that a request has
-        (1 for a step of single tokens), by which the kernels are chosen.  Returns out [rows, hq*head_dim]; rows of no request are left
-        as they are (undefined without `out`), rows that see no position are zero."""
+        cu_rows [R+1], table: int32.  Every row attends to the positions up to its own, of those that the table has an entry for.
+        max_q: the most new tokens that a request has (1 for a step of single tokens), by which the kernels are chosen.  Returns
+        out [rows, hq*head_dim]; rows of no request are left as they are (undefined without `out`), rows that see no position are
+        zero."""
         done = _host().attn_paged(self.hq, self.hkv, self.d, self.scratch, q, k_pages, v_pages, table, length, cu_rows, max_q, out, scale)
         if done is not None:
             return done

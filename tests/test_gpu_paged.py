@@ -663,3 +663,12 @@ def test_rope_kv_paged_refuses_an_output_of_other_columns():
     assert rope_kv_paged(q, *args) is q                # in place, in the first columns
     # 1 * 1 - 1 * 1 and 1 * 1 + 1 * 1
     assert (q[:, hq * d:] == 1).all() and (pool[0, :3, :, :d // 2] == 0).all() and (pool[0, :3, :, d // 2:] == 2).all()
+
+
+@pytest.mark.parametrize("new,total,width,page", [(20, 60, 3, 16), (2, 60, 3, 16), (200, 700, 5, 32), (1, 129, 1, 128), (40, 600, 2, 256), (150, 149, 4, 16)])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_a_length_beyond_the_table(new, total, width, page, d):
+    """more positions than the table has entries for: the rows behind them see those that are there"""
+    s = batch(1, [(new, total), (3, 30)], 4, 2, d, page, poison=False)
+    s["table"] = s["table"][:, :width].contiguous()
+    check_attn(s, 4, 2, d)
