@@ -446,7 +446,7 @@ int ixb_attn_paged(const void *q_device, const void *k_pages_device, const void 
  * What stands between the logits and the token (the reference's generator leaves it to HuggingFace's logits processors):
  *   x = logits[b][v] (bf16, or fp32 with logits_f32; row pitch in elements); out [rows][vocab] fp32, may be the logits
  *   where v is among the first n_tokens[b] entries of history row b: x > 0 ? x / repetition[b] : x * repetition[b]
- *   with c of these behind the first n_prompt[b]:                    x - frequency[b] * c, and - presence[b] where c > 0
+ *   where c > 0 of these are behind the first n_prompt[b]:           x - frequency[b] * c, then - presence[b]
  *   where bias_ids row b [n_bias] names v (the last entry that does): x + its value
  *   where bit v of the row's mask is 0:                              -infinity
  * each step rounded to fp32, in this order.  history, n_prompt (then 0), the three penalties, biases and mask may be NULL.  Token numbers outside

@@ -3,7 +3,7 @@
 //   x    = logits[b][v] in fp32
 //   seen = v among the row's tokens (prompt and generated);  c = how often v was generated
 //   x    = x > 0 ? x / repetition : x * repetition            where seen
-//   x    = x - frequency * c,  then x - presence              where c > 0
+//   x    = (x - frequency * c) - presence                     where c > 0
 //   x    = x + bias                                           where a bias names v (of several, the last one)
 //   x    = -inf                                               where the row's grammar has no bit for v
 //   out[b][v] = x;  token[b] = the lowest v with the largest x (a NaN counts as the largest)
@@ -210,8 +210,7 @@ k_logits(LogitRules s)
     auto rules = [&](float x, uint32_t v, uint32_t bin) {
         const uint32_t c = bin & B::kCount;
         if (c || bin & B::kPrompt) x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
-        x = __fsub_rn(x, __fmul_rn(freq, (float)c));
-        if (c) x = __fsub_rn(x, pres);
+        if (c) x = __fsub_rn(__fsub_rn(x, __fmul_rn(freq, (float)c)), pres);       // (zero times an infinite penalty would be NaN)
         if (bin & B::kBias) x = __fadd_rn(x, __uint_as_float(lg_at(table, s.n_slots - 1u, v - v0).y));
         return x;
     };

@@ -30,7 +30,7 @@ def apply_rules(logits, history=None, n_tokens=None, n_prompt=None, repetition=N
                 bias_values=None, mask=None, mask_row=None, out=None, token=None):
     """logits [B, V], bf16 or fp32 (column slices of wider rows allowed).  Per row b, each step rounded to fp32, in this order:
       tokens among the first n_tokens[b] of history[b] (int32 [B, L]):  x > 0 ? x / repetition[b] : x * repetition[b]
-      and c times among those behind the first n_prompt[b]:            x - frequency[b] * c, then - presence[b] if c > 0
+      and c > 0 times among those behind the first n_prompt[b]:        x - frequency[b] * c, then - presence[b]
       tokens named by bias_ids[b] (int32 [B, K]):                      x + bias_values[b] (fp32 [B, K]; the last entry counts)
       tokens whose bit in the row's mask (int32 [M, ceil(V / 32)], bit v % 32 of word v / 32) is 0:  -inf
     Row b has mask mask_row[b] (int32 [B]; none if that is -1), or mask b without mask_row.  Numbers outside 0 .. V - 1 in history and

@@ -206,3 +206,22 @@ def test_long_histories(b, v, length, f32):
     s["n_tokens"].fill_(length)
     s["n_prompt"].fill_(length // 3)
     check(s)
+
+
+@pytest.mark.parametrize("penalty", ["frequency", "presence"])
+@pytest.mark.parametrize("length,v", [(4, 5), (17000, 4096)])
+def test_an_infinite_penalty_reaches_generated_tokens_only(penalty, length, v):
+    """not those of the prompt, nor those that a bias names; both widths of counters, single logits and eight at a time"""
+    from ixrun_b200.logits import apply_rules
+
+    inf = float("inf")
+    x = torch.arange(v, dtype=torch.float32, device=DEV)[None] + 1.0
+    hist = torch.full((1, length), 1, dtype=torch.int32, device=DEV)           # a token of the prompt, then one that was generated
+    hist[0, length // 2:] = 2
+    out, token = torch.empty(1, v, device=DEV), torch.empty(1, dtype=torch.int64, device=DEV)
+    apply_rules(x, hist, torch.tensor([length], dtype=torch.int32, device=DEV), torch.tensor([length // 2], dtype=torch.int32, device=DEV),
+                bias_ids=torch.tensor([[0, 2]], dtype=torch.int32, device=DEV), bias_values=torch.ones(1, 2, device=DEV), out=out, token=token,
+                **{penalty: torch.full((1,), inf, device=DEV)})
+    want = x.clone()
+    want[0, 0], want[0, 2] = 2.0, -inf
+    assert torch.equal(out, want) and token.item() == v - 1
