@@ -24,7 +24,9 @@
 // sums of every row (zero times infinity is NaN), and the pair's blocks are then gone through again, straight from memory and token
 // by token.
 //
-// Every wait on an mbarrier is bounded and counts the CTA's own copies; where one runs out the CTA's outputs become NaN.
+// Every wait on an mbarrier is bounded (kPaWaitLimit polls of 1.5 us) and counts the CTA's own copies; where one runs out the CTA's
+// outputs become NaN.  Going through blocks again takes up to 105 us a block (sixteen tokens), so for a pair of two million
+// positions it takes longer than a wait: the warp that asks for blocks waits on as long as the others say that they get on.
 #pragma once
 #include "ixb_common.cuh"
 #include <cuda.h>
@@ -204,11 +206,13 @@ k_attn_paged(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
     extern __shared__ __align__(1024) unsigned char pa_smem[];
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(pa_smem), full0 = ring + CF::kRing + CF::kSum, empty0 = full0 + 8u * ST;
     uint32_t *sm_warp = (uint32_t *)(pa_smem + CF::kRing + CF::kSum + 16 * ST), &sm_last = sm_warp[CF::kThreads / 32];
+    volatile uint32_t *sm_again = sm_warp + CF::kThreads / 32 + 1;     // slices that were gone through again
     const uint32_t tid = threadIdx.x, lane = tid & 31u, wid = __shfl_sync(0xffffffffu, tid >> 5, 0), g = lane >> 2, t = lane & 3u;
     float *sum = (float *)(pa_smem + CF::kRing);       // [NW][8][kPitch]; before that the blocks before every request
     uint32_t *first = (uint32_t *)sum;
     const uint32_t R = a.requests, G = a.group, page = 1u << a.log_page;
     if (tid == 0) {
+        *sm_again = 0u;
         for (int i = 0; i < ST; ++i) {
             asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(full0 + 8u * i) : "memory");
             asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(empty0 + 8u * i), "r"(NW) : "memory");
@@ -296,6 +300,14 @@ k_attn_paged(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
         // (of lane < boxes, at most 32: positions bk * bp .. of a block and 64 dimensions; with D = 256 and pages of 16 a lane has just one)
         static_assert(CF::kKeys / 16 * (D / 64) <= 32, "a box per lane");
         const uint32_t dst = (bk * bp / 128u * (D / 64) + panel) * CF::kPanel + bk * bp % 128u * 128u;
+        auto room = [&](uint32_t bar, uint32_t parity) {
+            uint32_t seen;
+            do {
+                seen = *sm_again;
+                if (pa_wait(bar, parity)) return true;
+            } while (*sm_again != seen);
+            return false;
+        };
         uint32_t n = 0;
         bool more = true;
         while (more && ok) {
@@ -314,7 +326,7 @@ k_attn_paged(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
 #pragma unroll
                 for (int i = 0; i < 2; ++i, ++n) {
                     const uint32_t st = n % ST, bar = full0 + 8u * st;
-                    ok = ok && pa_wait(empty0 + 8u * st, (n / ST & 1u) ^ 1u);
+                    ok = ok && room(empty0 + 8u * st, (n / ST & 1u) ^ 1u);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     if (lane == 0) asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(bar), "r"(bytes) : "memory");
@@ -500,6 +512,7 @@ k_attn_paged(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
             for (uint32_t b = s.b0; b < s.b1; ++b) {
                 const int32_t key0 = (int32_t)(b * CF::kKeys + wid * CF::kSlice);
                 if (key0 > len1) break;                // uniform
+                if (lane == 0) atomicAdd((uint32_t *)sm_again, 1u);
                 auto at = [&](const __nv_bfloat16 *pool, size_t stride, int32_t key) -> const __nv_bfloat16 * {        // null: zeros
                     if (key > len1) return nullptr;
                     const int32_t p = a.table[(size_t)s.r * a.width + ((uint32_t)key >> a.log_page)];

@@ -672,3 +672,31 @@ def test_a_length_beyond_the_table(new, total, width, page, d):
     s = batch(1, [(new, total), (3, 30)], 4, 2, d, page, poison=False)
     s["table"] = s["table"][:, :width].contiguous()
     check_attn(s, 4, 2, d)
+
+
+def test_a_pair_that_is_gone_through_again_for_longer_than_a_wait():
+    """An infinite value in sight of sixteen rows behind 2.1 million positions (the same page over and over): the slow way through
+    them takes more than a wait's 1.5 seconds, while the next pair's blocks are asked for."""
+    from ixrun_b200.paged import AttnPaged
+
+    d, page, requests, new, n_pages = 128, 256, 149, 16, 8400
+    g = torch.Generator(device=DEV).manual_seed(1)
+    kp, vp = (torch.randn(2, page, 1, d, generator=g, device=DEV).bfloat16() for _ in range(2))
+    vp[0, 0, 0, 3] = float("inf")
+    q = torch.randn(requests * new, d, generator=g, device=DEV).bfloat16()
+    cu = torch.arange(requests + 1, dtype=torch.int32, device=DEV) * new
+    table = torch.zeros(requests, n_pages + 1, dtype=torch.int32, device=DEV)
+    table[:, n_pages] = 1                              # the new tokens' own page
+    length = torch.full((requests,), n_pages * page + new, dtype=torch.int32, device=DEV)
+    got = AttnPaged(1, 1, d, DEV)(q, kp, vp, table, length, cu, max_q=new).double()
+    e = torch.exp(q.double() @ torch.cat([kp[0, :, 0], kp[1, :new, 0]]).double().t() * d ** -0.5)
+    seen = torch.cat([torch.full((requests * new, page), float(n_pages), device=DEV, dtype=torch.float64),
+                      (torch.arange(new, device=DEV) <= (torch.arange(requests * new, device=DEV) % new)[:, None]).double()], 1)
+    p = e * seen / (e * seen).sum(1, keepdim=True)
+    v = torch.cat([vp[0, :, 0], vp[1, :new, 0]]).double()
+    assert (got[:, 3] == float("inf")).all()
+    fine = [i for i in range(d) if i != 3]
+    want, mag = p @ v[:, fine], p @ v[:, fine].abs()
+    # a rounding of the result, probabilities of 17 bits, and 32-bit sums one after the other: a warp adds up 16801 slices' values, a lane of it
+    # twice as many probabilities
+    assert ((got[:, fine] - want).abs() <= BF16 * want.abs() + (2.0 ** -12 + 3 * 16801 * 2.0 ** -24) * mag).all()
