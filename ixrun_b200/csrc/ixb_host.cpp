@@ -241,6 +241,9 @@ bool rows_of(const at::Tensor &t, Rows &r)
     r = {t.size(0), t.size(1), t.size(0) > 1 ? t.stride(0) : t.size(1)};
     return true;
 }
+// what the entry points refuse in Python (paged.PAGES, paged.MAX_REQUESTS)
+bool page_holds(int64_t page) { return page == 16 || page == 32 || page == 64 || page == 128 || page == 256; }
+constexpr int64_t kMaxRequests = 4096;
 // [pages, page, heads, dimensions] whose pages are contiguous and may lie apart
 bool pool_of(const at::Tensor &t, int64_t heads, int64_t d, int64_t &pages, int64_t &page, int64_t &pitch)
 {
@@ -248,7 +251,7 @@ bool pool_of(const at::Tensor &t, int64_t heads, int64_t d, int64_t &pages, int6
     pages = t.size(0);
     page = t.size(1);
     pitch = pages > 1 ? t.stride(0) : page * heads * d;
-    return pitch >= page * heads * d && pitch % 8 == 0;
+    return page_holds(page) && pitch >= page * heads * d && pitch % 8 == 0;
 }
 bool number(PyObject *o, int64_t &v)
 {
@@ -294,8 +297,8 @@ PyObject *page_step(PyObject *, PyObject *const *a, Py_ssize_t nargs)
     at::Tensor q, len, table, free_, n_free, cu, nl, nf, slot, pos, owner, status;
     if (nargs != 14 || !g_page_step || !take_ints(a[0], q, -1, dev)) Py_RETURN_NONE;
     const int64_t r = q.numel();
-    if (r < 1 || !take_ints(a[1], len, r, dev) || !take_ints(a[2], table, -1, dev) || !take_ints(a[3], free_, -1, dev) || !take_ints(a[4], n_free, 1, dev) ||
-        !number(a[5], page) || !number(a[6], rows) || table.dim() != 2 || table.size(0) != r || !take_ints(a[7], cu, r + 1, dev) || !take_ints(a[8], nl, r, dev) ||
+    if (r < 1 || r > kMaxRequests || !take_ints(a[1], len, r, dev) || !take_ints(a[2], table, -1, dev) || !take_ints(a[3], free_, -1, dev) || !take_ints(a[4], n_free, 1, dev) ||
+        !number(a[5], page) || !page_holds(page) || !number(a[6], rows) || table.dim() != 2 || table.size(0) != r || !take_ints(a[7], cu, r + 1, dev) || !take_ints(a[8], nl, r, dev) ||
         !take_ints(a[9], nf, 1, dev) || !take_ints(a[10], slot, rows, dev) || !take_ints(a[11], pos, rows, dev) || !take_ints(a[12], owner, rows, dev) ||
         !take_ints(a[13], status, 2, dev) || rows < 1 || free_.numel() < 1 || table.numel() < 1)
         Py_RETURN_NONE;
@@ -355,7 +358,7 @@ PyObject *attn_paged(PyObject *, PyObject *const *a, Py_ssize_t nargs)
         !take(a[5], kpool, bf, dev) || !take(a[6], vpool, bf, dev) || !take_ints(a[7], table, -1, dev) || !take_ints(a[8], len, -1, dev) || !rows_of(q, rq))
         Py_RETURN_NONE;
     const int64_t r = len.numel();
-    if (r < 1 || !take_ints(a[9], cu, r + 1, dev) || table.dim() != 2 || table.size(0) != r || table.size(1) < 1 || rq.rows < 1 || rq.cols < hq * d ||
+    if (r < 1 || r > kMaxRequests || !take_ints(a[9], cu, r + 1, dev) || table.dim() != 2 || table.size(0) != r || table.size(1) < 1 || rq.rows < 1 || rq.cols < hq * d ||
         !pool_of(kpool, hkv, d, pages, page, kp) || !pool_of(vpool, hkv, d, n2, p2, vp) || n2 != pages || p2 != page)
         Py_RETURN_NONE;
     max_q = rq.rows;
@@ -367,7 +370,7 @@ PyObject *attn_paged(PyObject *, PyObject *const *a, Py_ssize_t nargs)
     if (a[12] != Py_None) {
         if (!PyFloat_Check(a[12])) Py_RETURN_NONE;
         scale = PyFloat_AS_DOUBLE(a[12]);
-        if (!(scale > 0.0)) Py_RETURN_NONE;
+        if (!(scale > 0.0) || std::isinf(scale)) Py_RETURN_NONE;
     }
     if (a[11] != Py_None && (!take(a[11], out, bf, dev) || !out.is_contiguous() || out.numel() != rq.rows * hq * d)) Py_RETURN_NONE;
     const bool given = out.defined();

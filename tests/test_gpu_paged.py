@@ -700,3 +700,30 @@ def test_a_pair_that_is_gone_through_again_for_longer_than_a_wait():
     # a rounding of the result, probabilities of 17 bits, and 32-bit sums one after the other: a warp adds up 16801 slices' values, a lane of it
     # twice as many probabilities
     assert ((got[:, fine] - want).abs() <= BF16 * want.abs() + (2.0 ** -12 + 3 * 16801 * 2.0 ** -24) * mag).all()
+
+
+def test_refusals_have_one_type_on_both_host_paths(monkeypatch):
+    """what the extension takes at once and what the Python path checks: the same ValueError, not an error of the C entry"""
+    from ixrun_b200 import _lib, paged
+    from ixrun_b200.paged import AttnPaged, PageStep, page_step, rope_kv_paged
+
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32, device=DEV)  # noqa: E731
+    b = lambda *s: torch.zeros(*s, dtype=torch.bfloat16, device=DEV)  # noqa: E731
+    cos = torch.zeros(9, 32, device=DEV)
+    attn = AttnPaged(4, 2, 64, DEV)
+    step = dict(q_len=i(2), length=i(2), table=i(2, 3), free=i(4), n_free=i(1), page=16, rows=5, out=PageStep.empty(2, 5, DEV))
+    many = dict(q_len=i(5000), length=i(5000), table=i(5000, 3), out=PageStep.empty(5000, 5, DEV))
+    rope = dict(q=b(3, 256), k=b(3, 128), v=b(3, 128), pos=i(3), slot=i(3), k_pages=b(4, 16, 2, 64), v_pages=b(4, 16, 2, 64), cos=cos, sin=cos, hq=4,
+                hkv=2, head_dim=64)
+    call = dict(q=b(3, 256), k_pages=b(4, 16, 2, 64), v_pages=b(4, 16, 2, 64), table=i(2, 2), length=i(2), cu_rows=i(3))
+    odd = dict(k_pages=b(4, 48, 2, 64), v_pages=b(4, 48, 2, 64))
+    cases = [(page_step, step, dict(page=24)), (page_step, step, dict(page=512)), (page_step, step, many), (rope_kv_paged, rope, odd), (attn, call, odd),
+             (attn, call, dict(table=i(5000, 2), length=i(5000), cu_rows=i(5001))), (attn, call, dict(scale=float("inf"))),
+             (attn, call, dict(scale=float("nan"))), (attn, call, dict(scale=0.0)), (attn, call, dict(max_q=0))]
+    for python in (False, True):
+        if python:
+            monkeypatch.setattr(paged, "_host", lambda: _lib._PythonHost)
+        for f, ok, bad in cases:
+            f(**ok)
+            with pytest.raises(ValueError):
+                f(**{**ok, **bad})
