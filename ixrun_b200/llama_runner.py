@@ -725,6 +725,8 @@ class PagedDecoder:
         """Feeds the requests what they have, at most max_rows rows in all: single tokens first, then prompts in the order of
         their numbers.  Returns tokens int64 [requests], -1 for those without a new one (a static tensor).  RuntimeError, and
         nothing launched, where there is nothing to feed, a request has all max_seq tokens, or the pages do not suffice."""
+        if max_rows < 1:
+            raise ValueError("max_rows must be positive")
         left, q_len = int(max_rows), [0] * self.b
         todo = {r: n - self._cached[r] for r, n in enumerate(self._known) if n is not None}
         for r in sorted(todo, key=lambda r: (todo[r] > 1, r)):
@@ -775,8 +777,8 @@ class PagedDecoder:
     def generate(self, prompts: list, n_new: int, eos: int | None = None, max_rows: int = PackedLlama.PREFILL_ROWS, **rules) -> list:
         """n_new tokens for every prompt (fewer for one that ends with eos or has all max_seq tokens), as lists; a prompt waits
         until a number and the pages for its whole answer are free."""
-        if n_new < 1:
-            raise ValueError("n_new must be positive")
+        if n_new < 1 or max_rows < 1:
+            raise ValueError("n_new and max_rows must be positive")
         if any(n is not None for n in self._known):
             raise RuntimeError("generate wants the decoder for itself: remove the requests that are there")
         whole = [self._n_pages(min(ids.numel() + n_new - 1, self.m.cfg.max_seq)) for ids in prompts]

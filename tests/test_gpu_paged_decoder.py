@@ -196,3 +196,19 @@ def test_refusals():
     dec.add(ids)
     assert dec.step()[0].item() == first
     assert dec.step()[0].item() >= 0
+
+
+def test_a_step_of_no_rows_is_refused_and_changes_nothing():
+    from ixrun_b200.llama_runner import PagedDecoder
+
+    cfg, model = tiny()
+    dec = PagedDecoder(model, 2, 8, page=16)
+    r = dec.add(torch.arange(5))
+    for rows in (0, -1, -7):
+        with pytest.raises(ValueError):
+            dec.step(rows)
+    assert dec._cached == [0, 0] == dec.pages.length.tolist() and dec._known == [5, None] and dec._pages_left == 8
+    dec.remove(r)
+    with pytest.raises(ValueError):
+        dec.generate([torch.arange(5)], 2, max_rows=0)
+    assert dec._known == [None, None]
