@@ -600,6 +600,8 @@ class PagedDecoder:
         # the host's account of the same: tokens known and tokens in the cache (None: no request), pages left
         self._known, self._cached = [None] * b, [0] * b
         self._pages_left, self._fed = n_pages, [0] * b
+        # steps made, the one in which a request last had rows (or was added), and the requests' order
+        self._steps, self._last, self._came, self._added = 0, [0] * b, [0] * b, 0
         self._step, self._bufs = self.pages.new_step(b), self._buffers(b)
         self.graph = None
 
@@ -687,7 +689,8 @@ class PagedDecoder:
         if bias:
             self.bias_ids[r, :len(bias)].copy_(torch.tensor(list(bias), dtype=torch.int32, device=dev))
             self.bias_values[r, :len(bias)].copy_(torch.tensor(list(bias.values()), dtype=torch.float32, device=dev))
-        self._known[r], self._cached[r] = n, 0
+        self._known[r], self._cached[r], self._last[r], self._came[r] = n, 0, self._steps, self._added
+        self._added += 1
         return r
 
     def allow(self, r: int, allowed: torch.Tensor | None):
@@ -720,18 +723,38 @@ class PagedDecoder:
     def _n_pages(self, tokens):
         return -(-tokens // self.pages.page)
 
+    def _share(self, max_rows):
+        """rows of every request in a step of at most max_rows"""
+        left, q_len = int(max_rows), [0] * self.b
+        todo = {r: n - self._cached[r] for r, n in enumerate(self._known) if n is not None}
+        singles = sorted((r for r in todo if todo[r] == 1), key=lambda r: (self._last[r], r))
+        prompts = sorted((r for r in todo if todo[r] > 1), key=lambda r: self._came[r])
+        waited = [r for r in prompts[:1] if self._last[r] < self._steps]
+        for r in waited + singles + prompts[len(waited):]:
+            q_len[r] = min(todo[r], left)
+            left -= q_len[r]
+        return q_len
+
+    def _account(self, q_len):
+        """what a step of these rows has done"""
+        self._steps += 1
+        for r, n in enumerate(q_len):
+            if not n:
+                continue
+            self._last[r] = self._steps
+            self._cached[r] += n
+            if self._cached[r] == self._known[r]:
+                self._known[r] += 1
+
     @torch.no_grad()
     def step(self, max_rows: int = PackedLlama.PREFILL_ROWS) -> torch.Tensor:
-        """Feeds the requests what they have, at most max_rows rows in all: single tokens first, then prompts in the order of
-        their numbers.  Returns tokens int64 [requests], -1 for those without a new one (a static tensor).  RuntimeError, and
+        """Feeds the requests what they have, at most max_rows rows in all: single tokens first, those that have waited longest before
+        others, then prompts in the order in which they were added; the first of these comes before the single tokens where it had
+        no row in the step before.  So every request gets on, however few rows there are.  Returns tokens int64 [requests], -1 for those without a new one (a static tensor).  RuntimeError, and
         nothing launched, where there is nothing to feed, a request has all max_seq tokens, or the pages do not suffice."""
         if max_rows < 1:
             raise ValueError("max_rows must be positive")
-        left, q_len = int(max_rows), [0] * self.b
-        todo = {r: n - self._cached[r] for r, n in enumerate(self._known) if n is not None}
-        for r in sorted(todo, key=lambda r: (todo[r] > 1, r)):
-            q_len[r] = min(todo[r], left)
-            left -= q_len[r]
+        q_len = self._share(max_rows)
         if not any(q_len):
             raise RuntimeError("no request to feed")
         if any(self._cached[r] + n > self.m.cfg.max_seq for r, n in enumerate(q_len)):
@@ -750,10 +773,7 @@ class PagedDecoder:
         else:
             self._forward(self.pages.new_step(sum(q_len)), self._buffers(sum(q_len)), max(q_len))
         self._pages_left -= need
-        for r, n in enumerate(q_len):
-            self._cached[r] += n
-            if n and self._cached[r] == self._known[r]:
-                self._known[r] += 1
+        self._account(q_len)
         return self.token
 
     @torch.no_grad()

@@ -212,3 +212,24 @@ def test_a_step_of_no_rows_is_refused_and_changes_nothing():
     with pytest.raises(ValueError):
         dec.generate([torch.arange(5)], 2, max_rows=0)
     assert dec._known == [None, None]
+
+
+@pytest.mark.parametrize("rows", [1, 3, 4])
+def test_every_request_gets_on_where_there_are_fewer_rows_than_requests(rows):
+    """answers and prompts in turns, with the logits that each has alone"""
+    from ixrun_b200.llama_runner import PagedDecoder
+
+    cfg, model = tiny()
+    dec = PagedDecoder(model, 8, 48, page=16).capture()
+    prompts = prompts_of(cfg, (3, 1, 1, 9, 1, 1, 1, 2))
+    tokens, logits = [p.tolist() for p in prompts], [[] for _ in prompts]
+    for p in prompts:
+        dec.add(p)
+    for _ in range(60):
+        for r, t in enumerate(dec.step(rows).tolist()):
+            if t >= 0:
+                tokens[r].append(t)
+                logits[r].append(dec.logits[r].clone())
+    assert min(len(x) for x in logits) >= 2
+    for r in (0, 3, 7):
+        check_alone(model, torch.tensor(tokens[r]), prompts[r].numel(), logits[r])

@@ -96,3 +96,39 @@ def test_names_of_the_package():
     assert ixrun_b200.PagedDecoder is llama_runner.PagedDecoder
     with pytest.raises(AttributeError):
         ixrun_b200.no_such_name
+
+
+def host_account(lengths):
+    """a PagedDecoder's account of its requests, without a model"""
+    from ixrun_b200.llama_runner import PagedDecoder
+
+    dec = PagedDecoder.__new__(PagedDecoder)
+    n = len(lengths)
+    dec.b, dec._known, dec._cached, dec._steps, dec._last, dec._came, dec._added = n, list(lengths), [0] * n, 0, [0] * n, list(range(n)), n
+    return dec
+
+
+@pytest.mark.parametrize("lengths", [(1,) * 8, (1, 1, 1, 40), (5, 9, 1, 30, 1, 1), (200, 100), (1,) * 20 + (7,) * 20])
+@pytest.mark.parametrize("rows", [1, 2, 4, 7])
+def test_no_request_of_a_paged_decoder_waits_for_good(lengths, rows):
+    """Single tokens in turns, a prompt at least in every second step, prompts one after the other: all have answered twice after as many
+    steps as that takes, with every second one for a prompt while there is one."""
+    dec = host_account(lengths)
+    answers = [0] * len(lengths)
+    n = len(lengths)
+    bound = 2 * sum(-(-p // rows) + 1 for p in lengths) + 4 * -(-n // rows) + 4
+    for _ in range(bound):
+        q = dec._share(rows)
+        assert 0 < sum(q) <= rows and min(q) >= 0
+        known = list(dec._known)
+        dec._account(q)
+        answers = [a + (x != y) for a, x, y in zip(answers, known, dec._known)]
+    assert min(answers) >= 2
+
+
+def test_rows_that_suffice_go_to_everybody():
+    dec = host_account((1, 30, 1, 4))
+    assert dec._share(100) == [1, 30, 1, 4]
+    assert dec._share(10) == [1, 8, 1, 0] and dec._share(2) == [1, 0, 1, 0] and dec._share(1) == [1, 0, 0, 0]
+    dec._account([1, 0, 1, 0])                         # the prompt that had nothing comes first
+    assert dec._share(3) == [0, 3, 0, 0] and dec._share(40) == [1, 30, 1, 4]
