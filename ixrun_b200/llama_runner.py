@@ -21,6 +21,7 @@ matmuls -- with eager glue the ground truth for greedy-token agreement.
 """
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 
 import torch
@@ -597,8 +598,8 @@ class PagedDecoder:
         self.logits = torch.zeros(b, cfg.vocab, dtype=torch.float32, device=dev)
         self.token = torch.full((b,), -1, dtype=torch.long, device=dev)
         self._best = torch.zeros(b, dtype=torch.long, device=dev)
-        # the host's account of the same: tokens known and tokens in the cache (None: no request), pages left
-        self._known, self._cached = [None] * b, [0] * b
+        # the host's account of the same: tokens known (None: no request), tokens in the cache, tokens that a bias bans; pages left
+        self._known, self._cached, self._banned = [None] * b, [0] * b, [[]] * b
         self._pages_left, self._fed = n_pages, [0] * b
         # steps made, the one in which a request last had rows (or was added), and the requests' order
         self._steps, self._last, self._came, self._added = 0, [0] * b, [0] * b, 0
@@ -664,8 +665,9 @@ class PagedDecoder:
     @torch.no_grad()
     def add(self, prompt: torch.Tensor, repetition: float = 1.0, presence: float = 0.0, frequency: float = 0.0, bias: dict | None = None,
             allowed: torch.Tensor | None = None) -> int:
-        """Takes a request in; returns its number (a free one).  The rules are those of ``logits.apply_rules``; bias: {token:
-        value}; allowed: a bool tensor [vocab]."""
+        """Takes a request in; returns its number (a free one).  The rules are those of ``logits.apply_rules``, penalties finite; bias:
+        {token: value}; allowed: a bool tensor [vocab].  Rules that leave no token (none allowed that has no bias of -inf) are
+        refused."""
         n = prompt.numel()
         if None not in self._known:
             raise RuntimeError("all requests are taken")
@@ -673,12 +675,19 @@ class PagedDecoder:
             raise ValueError(f"a prompt of 1..{self.m.cfg.max_seq} tokens")
         if prompt.is_floating_point() or prompt.min() < 0 or prompt.max() >= self.m.cfg.vocab:
             raise ValueError(f"tokens are whole numbers of 0..{self.m.cfg.vocab - 1}")
-        if not repetition > 0.0:
-            raise ValueError("repetition must be positive")
+        penalties = torch.tensor([repetition, presence, frequency], dtype=torch.float32)
+        if not penalties[0] > 0.0 or not penalties.isfinite().all():
+            raise ValueError("repetition must be positive, penalties finite")
         bias = bias or {}
         if len(bias) > self.bias_ids.shape[1]:
             raise ValueError(f"at most {self.bias_ids.shape[1]} biases")
+        values = torch.tensor(list(bias.values()), dtype=torch.float32)
+        if values.isnan().any():
+            raise ValueError("a bias is a number")
+        banned = [t for t, x in zip(bias, values.tolist()) if x == -math.inf and 0 <= t < self.m.cfg.vocab]
+        self._check_allowed(allowed, banned)
         r = self._known.index(None)
+        self._banned[r] = banned
         self._allow(r, allowed)
         dev = self.history.device
         self.history[r, :n].copy_(prompt.reshape(-1))
@@ -688,22 +697,30 @@ class PagedDecoder:
             self.bias_ids[r].fill_(-1)
         if bias:
             self.bias_ids[r, :len(bias)].copy_(torch.tensor(list(bias), dtype=torch.int32, device=dev))
-            self.bias_values[r, :len(bias)].copy_(torch.tensor(list(bias.values()), dtype=torch.float32, device=dev))
+            self.bias_values[r, :len(bias)].copy_(values)
         self._known[r], self._cached[r], self._last[r], self._came[r] = n, 0, self._steps, self._added
         self._added += 1
         return r
 
     def allow(self, r: int, allowed: torch.Tensor | None):
-        """The tokens that request r may have from now on (a bool tensor [vocab]; None: all), as a grammar moves on."""
-        self._allow(self._request(r), allowed)
+        """The tokens that request r may have from now on (a bool tensor [vocab]; None: all), as a grammar moves on.  At least one."""
+        self._check_allowed(allowed, self._banned[self._request(r)])
+        self._allow(r, allowed)
+
+    def _check_allowed(self, allowed, banned):
+        """refuses what leaves no token (the arg-max of a row of -inf would be token 0); banned: tokens with a bias of -inf"""
+        vocab = self.m.cfg.vocab
+        if allowed is not None and (allowed.dtype != torch.bool or allowed.shape != (vocab,)):
+            raise ValueError("allowed: a bool tensor [vocab]")
+        left = vocab - len(banned) if allowed is None else int(allowed.sum()) - (int(allowed[banned].sum()) if banned else 0)
+        if left < 1:
+            raise ValueError("the rules leave no token")
 
     @torch.no_grad()
     def _allow(self, r, allowed):
         if allowed is None:
             self.mask_row[r].fill_(-1)
             return
-        if allowed.dtype != torch.bool or allowed.shape != (self.m.cfg.vocab,):
-            raise ValueError("allowed: a bool tensor [vocab]")
         bits = F.pad(allowed.to(self.mask.device), (0, self.mask.shape[1] * 32 - allowed.numel())).view(-1, 32).long()
         words = (bits << torch.arange(32, device=bits.device)).sum(1)
         self.mask[r].copy_(torch.where(words >= 2**31, words - 2**32, words))

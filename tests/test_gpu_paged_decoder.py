@@ -233,3 +233,31 @@ def test_every_request_gets_on_where_there_are_fewer_rows_than_requests(rows):
     assert min(len(x) for x in logits) >= 2
     for r in (0, 3, 7):
         check_alone(model, torch.tensor(tokens[r]), prompts[r].numel(), logits[r])
+
+
+def test_rules_that_leave_no_token_are_refused():
+    from ixrun_b200.llama_runner import PagedDecoder
+
+    cfg, model = tiny()
+    inf, ids = float("inf"), torch.arange(9)
+    one = torch.zeros(cfg.vocab, dtype=torch.bool)
+    none = one.clone()
+    one[7] = True
+    dec = PagedDecoder(model, 2, 8, page=16, max_bias=4)
+    for bad in (dict(allowed=none), dict(allowed=none.cuda()), dict(allowed=one, bias={7: -inf}), dict(allowed=one, bias={7: -1e39, 3: 1.0}),
+                dict(bias={5: float("nan")}), dict(presence=inf), dict(frequency=float("nan")), dict(repetition=inf), dict(repetition=1e-60)):
+        with pytest.raises(ValueError):
+            dec.add(ids, **bad)
+    assert dec._known == [None, None] and dec.mask_row.tolist() == [-1, -1]
+    r, b = dec.add(ids, allowed=one, bias={8: -inf, -1: -inf}), dec.add(ids, bias={3: -inf})
+    assert dec.step()[r] == 7
+    for mask in (none, torch.arange(cfg.vocab) == 8):
+        with pytest.raises(ValueError):
+            dec.allow(r, mask)
+    assert dec.step()[r] == 7                          # (the mask that it had)
+    dec.allow(b, torch.arange(cfg.vocab) == 8)         # (another request's ban)
+    assert dec.step().tolist() == [7, 8]
+    # the next request of the number is not bound by its predecessor's bans
+    dec.remove(r)
+    assert dec.add(ids, allowed=torch.arange(cfg.vocab) == 8) == r
+    assert dec.step()[r] == 8
