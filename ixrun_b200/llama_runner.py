@@ -662,16 +662,9 @@ class PagedDecoder:
             raise ValueError(f"no request {r}")
         return r
 
-    @torch.no_grad()
-    def add(self, prompt: torch.Tensor, repetition: float = 1.0, presence: float = 0.0, frequency: float = 0.0, bias: dict | None = None,
-            allowed: torch.Tensor | None = None) -> int:
-        """Takes a request in; returns its number (a free one).  The rules are those of ``logits.apply_rules``, penalties finite; bias:
-        {token: value}; allowed: a bool tensor [vocab].  Rules that leave no token (none allowed that has no bias of -inf) are
-        refused."""
-        n = prompt.numel()
-        if None not in self._known:
-            raise RuntimeError("all requests are taken")
-        if not 1 <= n <= self.m.cfg.max_seq:
+    def _checked(self, prompt, repetition=1.0, presence=0.0, frequency=0.0, bias=None, allowed=None):
+        """the checks of ``add``; returns the biases' values and the tokens that they ban"""
+        if not 1 <= prompt.numel() <= self.m.cfg.max_seq:
             raise ValueError(f"a prompt of 1..{self.m.cfg.max_seq} tokens")
         if prompt.is_floating_point() or prompt.min() < 0 or prompt.max() >= self.m.cfg.vocab:
             raise ValueError(f"tokens are whole numbers of 0..{self.m.cfg.vocab - 1}")
@@ -686,7 +679,18 @@ class PagedDecoder:
             raise ValueError("a bias is a number")
         banned = [t for t, x in zip(bias, values.tolist()) if x == -math.inf and 0 <= t < self.m.cfg.vocab]
         self._check_allowed(allowed, banned)
-        r = self._known.index(None)
+        return values, banned
+
+    @torch.no_grad()
+    def add(self, prompt: torch.Tensor, repetition: float = 1.0, presence: float = 0.0, frequency: float = 0.0, bias: dict | None = None,
+            allowed: torch.Tensor | None = None) -> int:
+        """Takes a request in; returns its number (a free one).  The rules are those of ``logits.apply_rules``, penalties finite; bias:
+        {token: value}; allowed: a bool tensor [vocab].  Rules that leave no token (none allowed that has no bias of -inf) are
+        refused."""
+        if None not in self._known:
+            raise RuntimeError("all requests are taken")
+        values, banned = self._checked(prompt, repetition, presence, frequency, bias, allowed)
+        n, r = prompt.numel(), self._known.index(None)
         self._banned[r] = banned
         self._allow(r, allowed)
         dev = self.history.device
@@ -818,6 +822,8 @@ class PagedDecoder:
             raise ValueError("n_new and max_rows must be positive")
         if any(n is not None for n in self._known):
             raise RuntimeError("generate wants the decoder for itself: remove the requests that are there")
+        for ids in prompts:                            # (before the first one is taken in: a refusal leaves no request behind)
+            self._checked(ids, **rules)
         whole = [self._n_pages(min(ids.numel() + n_new - 1, self.m.cfg.max_seq)) for ids in prompts]
         if whole and max(whole) > self._pages_left:
             raise RuntimeError(f"a prompt and its answer need {max(whole)} pages, there are {self._pages_left}")

@@ -261,3 +261,17 @@ def test_rules_that_leave_no_token_are_refused():
     dec.remove(r)
     assert dec.add(ids, allowed=torch.arange(cfg.vocab) == 8) == r
     assert dec.step()[r] == 8
+
+
+@pytest.mark.parametrize("last", ["token", "length", "empty", "rules"])
+def test_generate_that_refuses_a_prompt_leaves_no_request_behind(last):
+    from ixrun_b200.llama_runner import PagedDecoder
+
+    cfg, model = tiny()
+    dec = PagedDecoder(model, 2, 12, page=16)
+    ids = torch.arange(5)
+    bad = {"token": torch.tensor([cfg.vocab]), "length": torch.zeros(cfg.max_seq + 1, dtype=torch.long), "empty": ids[:0], "rules": ids}[last]
+    with pytest.raises(ValueError):
+        dec.generate([ids, ids, ids, bad], 3, **({"bias": {i: 0.5 for i in range(65)}} if last == "rules" else {}))
+    assert dec._known == [None, None] and dec._pages_left == 12 == dec.pages.n_free.item()
+    assert [len(o) for o in dec.generate([ids, ids, ids], 3)] == [3, 3, 3]
