@@ -570,14 +570,17 @@ class PagedDecoder:
     penalties, biases and a mask of allowed tokens; the token is the arg-max behind them."""
 
     def __init__(self, model: PackedLlama, requests: int, n_pages: int, page: int = 64, max_bias: int = 64):
+        from .logits import MAX_BIASES, MAX_TOKENS, MAX_VOCAB
         from .paged import AttnPaged, PageTables
 
         if model.weights != "packed" or model.glue != "kernels":
             raise ValueError("the paged decoder runs on packed weights and the glue kernels")
         if not 1 <= requests <= 64:
             raise ValueError("1..64 requests")
-        if max_bias < 0:
-            raise ValueError("max_bias must not be negative")
+        if not 0 <= max_bias <= MAX_BIASES:
+            raise ValueError(f"0..{MAX_BIASES} biases")
+        if model.cfg.vocab > MAX_VOCAB or model.cfg.max_seq >= MAX_TOKENS:
+            raise ValueError(f"a vocabulary of at most {MAX_VOCAB}, less than {MAX_TOKENS} tokens of a request")
         self.m, self.b = model, int(requests)
         cfg, dev, b = model.cfg, model.embed.device, self.b
         self._attn = AttnPaged(cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, dev)

@@ -9,6 +9,8 @@ from . import _lib
 
 __all__ = ["apply_rules"]
 
+MAX_VOCAB, MAX_TOKENS, MAX_BIASES = 393216, 2**20 - 1, 2047        # of a row, as ixb_logits takes them
+
 
 def _on(dev: int, t, dtypes, shape, what: str):
     """a tensor of one of these types and of this shape (None: any size) with contiguous rows, on this device; its row pitch"""
@@ -36,7 +38,7 @@ def apply_rules(logits, history=None, n_tokens=None, n_prompt=None, repetition=N
     Row b has mask mask_row[b] (int32 [B]; none if that is -1), or mask b without mask_row.  Numbers outside 0 .. V - 1 in history and
     bias_ids are passed over (-1 as padding).  n_prompt None: everything counts as generated; penalties None: 1, 0, 0 (fp32 [B]).
     Writes out (fp32 [B, V], may be the fp32 logits; allocated if None) and token (int64 [B], may be None): the lowest index
-    of the largest value.  Returns out."""
+    of the largest value (of a row of -inf: 0).  V up to 393216, L up to 1048575, K up to 2047.  Returns out."""
     if out is None and logits.dim() == 2:
         out = torch.empty(logits.shape, dtype=torch.float32, device=logits.device)
     if out is not None and _lib.host().logits(logits, history, n_tokens, n_prompt, repetition, presence, frequency, bias_ids, bias_values, mask, mask_row, out, token):

@@ -132,3 +132,23 @@ def test_rows_that_suffice_go_to_everybody():
     assert dec._share(10) == [1, 8, 1, 0] and dec._share(2) == [1, 0, 1, 0] and dec._share(1) == [1, 0, 0, 0]
     dec._account([1, 0, 1, 0])                         # the prompt that had nothing comes first
     assert dec._share(3) == [0, 3, 0, 0] and dec._share(40) == [1, 30, 1, 4]
+
+
+@pytest.mark.parametrize("vocab,max_seq,max_bias", [(393217, 96, 4), (1000, 2**20 - 1, 4), (1000, 96, 2048), (1000, 96, -1)])
+def test_a_paged_decoder_beyond_the_limits_of_its_rules_is_refused(vocab, max_seq, max_bias):
+    """at the start, not in its first step, when tables and lengths have been written"""
+    from types import SimpleNamespace
+
+    from ixrun_b200.llama_runner import LlamaConfig, PagedDecoder
+
+    cfg = LlamaConfig(n_layers=1, hidden=256, intermediate=512, n_heads=4, n_kv_heads=2, head_dim=64, vocab=vocab, max_seq=max_seq)
+    with pytest.raises(ValueError):
+        PagedDecoder(SimpleNamespace(weights="packed", glue="kernels", cfg=cfg), 2, 4, max_bias=max_bias)
+
+
+def test_limits_of_the_rules_are_those_of_the_entry():
+    from ixrun_b200 import logits
+
+    v, n, k = logits.MAX_VOCAB, logits.MAX_TOKENS, logits.MAX_BIASES
+    for changed in (dict(vocab=v + 1, pitch=v + 1, out_pitch=v + 1), dict(hist_len=n + 1, hist_pitch=n + 1), dict(n_bias=k + 1, bias_ids=P, bias_values=P)):
+        assert call("ixb_logits", **changed)[0] == 2
