@@ -805,16 +805,17 @@ class PagedDecoder:
         """Captures the step of single tokens."""
         self.q_len.zero_()                     # (the warm-up feeds nothing)
         self._fed = [0] * self.b
-        side = torch.cuda.Stream(self.q_len.device)
-        side.wait_stream(torch.cuda.current_stream())
-        with torch.cuda.stream(side):
-            for _ in range(2):
+        with torch.cuda.device(self.q_len.device):         # (a capture takes what runs on the current device)
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                for _ in range(2):
+                    self._forward(self._step, self._bufs, 1)
+            torch.cuda.current_stream().wait_stream(side)
+            torch.cuda.synchronize()
+            self.graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(self.graph):
                 self._forward(self._step, self._bufs, 1)
-        torch.cuda.current_stream().wait_stream(side)
-        torch.cuda.synchronize()
-        self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph):
-            self._forward(self._step, self._bufs, 1)
         return self
 
     @torch.no_grad()

@@ -152,3 +152,34 @@ def test_limits_of_the_rules_are_those_of_the_entry():
     v, n, k = logits.MAX_VOCAB, logits.MAX_TOKENS, logits.MAX_BIASES
     for changed in (dict(vocab=v + 1, pitch=v + 1, out_pitch=v + 1), dict(hist_len=n + 1, hist_pitch=n + 1), dict(n_bias=k + 1, bias_ids=P, bias_values=P)):
         assert call("ixb_logits", **changed)[0] == 2
+
+
+def test_a_paged_decoder_is_captured_on_its_own_device(monkeypatch):
+    """whatever device is current: streams, synchronisation and the capture are those of the decoder's"""
+    from contextlib import contextmanager
+    from types import SimpleNamespace
+
+    from ixrun_b200.llama_runner import PagedDecoder
+
+    at, seen = ["cuda:0"], []
+
+    @contextmanager
+    def device(d):
+        at.append(d)
+        yield
+        at.pop()
+
+    @contextmanager
+    def on(*_):
+        yield
+
+    note = lambda what, result=None: lambda *_: (seen.append((what, at[-1])), result)[1]  # noqa: E731
+    stream = SimpleNamespace(wait_stream=lambda _: None)
+    for name, fake in (("device", device), ("stream", on), ("graph", on), ("Stream", note("stream", stream)), ("current_stream", note("current", stream)),
+                       ("synchronize", note("synchronize")), ("CUDAGraph", note("graph", "graph"))):
+        monkeypatch.setattr(torch.cuda, name, fake)
+    dec = PagedDecoder.__new__(PagedDecoder)
+    dec.b, dec._step, dec._bufs, dec._forward = 2, None, None, note("forward")
+    dec.q_len = SimpleNamespace(device="cuda:1", zero_=lambda: None)
+    assert dec.capture() is dec and dec.graph == "graph"
+    assert [w for w, _ in seen].count("forward") == 3 and {d for _, d in seen} == {"cuda:1"}
