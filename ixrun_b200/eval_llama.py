@@ -19,6 +19,12 @@ import torch
 from .llama_runner import LlamaConfig, PackedLlama, synthetic_llama
 
 
+def all_answering(dec):
+    """steps of a PagedDecoder until every request has its prompt behind it"""
+    while (dec.step() < 0).any():
+        pass
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--layers", type=int, default=24)
@@ -118,6 +124,7 @@ def main():
             dec = PagedDecoder(packed, b, b * (-(-cfg.max_seq // 64))).capture()
             for _ in range(b):
                 dec.add(torch.randint(0, cfg.vocab, (128,), generator=g))
+            all_answering(dec)
             for _ in range(4):
                 dec.step()
             torch.cuda.synchronize()

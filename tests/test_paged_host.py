@@ -183,3 +183,21 @@ def test_a_paged_decoder_is_captured_on_its_own_device(monkeypatch):
     dec.q_len = SimpleNamespace(device="cuda:1", zero_=lambda: None)
     assert dec.capture() is dec and dec.graph == "graph"
     assert [w for w, _ in seen].count("forward") == 3 and {d for _, d in seen} == {"cuda:1"}
+
+
+@pytest.mark.parametrize("requests", [1, 8, 64])
+def test_the_paged_figure_is_taken_behind_the_prompts(requests):
+    """64 prompts of 128 tokens take more than four steps of 2048 rows, as the first answers come between"""
+    from ixrun_b200.eval_llama import all_answering
+
+    dec = host_account((128,) * requests)
+
+    def step():
+        q = dec._share(2048)
+        known = list(dec._known)
+        dec._account(q)
+        return torch.tensor([1 if a != b else -1 for a, b in zip(known, dec._known)])
+
+    dec.step = step
+    all_answering(dec)
+    assert all(k - c == 1 for k, c in zip(dec._known, dec._cached))
