@@ -225,3 +225,32 @@ def test_an_infinite_penalty_reaches_generated_tokens_only(penalty, length, v):
     want = x.clone()
     want[0, 0], want[0, 2] = 2.0, -inf
     assert torch.equal(out, want) and token.item() == v - 1
+
+
+def test_dependent_launches_give_the_same_bits():
+    """each call in place on the logits of the one before, without a wait of the host"""
+    from ixrun_b200.logits import apply_rules
+    from ixrun_b200.p6 import set_pdl
+
+    s = [inputs(i, 9, 30000, 500 * i, 40, 3, f32=True) for i in range(1, 5)]
+    first = s[0].pop("logits").clone()
+    for r in s[1:]:
+        r.pop("logits")
+
+    def run(wait):
+        x, tokens = first.clone(), []
+        for r in s:
+            tokens.append(torch.empty(9, dtype=torch.int64, device=DEV))
+            wait()
+            apply_rules(x, **r, out=x, token=tokens[-1])
+        wait()
+        return [x] + tokens
+
+    want = run(torch.cuda.synchronize)
+    prev = set_pdl(True)
+    try:
+        for _ in range(10):
+            assert all(torch.equal(a, b) for a, b in zip(run(lambda: None), want))
+    finally:
+        torch.cuda.synchronize()
+        set_pdl(prev)

@@ -727,3 +727,67 @@ def test_refusals_have_one_type_on_both_host_paths(monkeypatch):
             f(**ok)
             with pytest.raises(ValueError):
                 f(**{**ok, **bad})
+
+
+@pytest.mark.parametrize("lens,max_q", [([(1, 900)] * 3 + [(1, 17)], 1), ([(1, 5000)], 1), ([(4, 300), (3, 3), (2, 900)], 4), ([(1, 2 + i) for i in range(40)], 1)],
+                         ids=lambda v: f"{len(v)}x{v[0][0]}-{v[0][1]}" if isinstance(v, list) else None)
+@pytest.mark.parametrize("hq,hkv,d", [(4, 2, 64), (4, 2, 128), (4, 2, 256), (4, 4, 128), (2, 1, 64)])
+def test_probabilities_of_few_rows_are_held_in_17_bits(lens, max_q, hq, hkv, d):
+    """Half a step of the result; beside it two bf16 numbers leave 2^-16 of a probability, and scores, sums of magnitudes up to 20 in some
+    sixteen 32-bit steps that may cut off a unit, 20 * 16 * 2^-23 < 2^-14 of it: less than 2^-13 together.  (With 8 bits
+    results of these lengths are off by 3 to 18 times that.)"""
+    from ixrun_b200.paged import AttnPaged
+
+    s = batch(5, lens, hq, hkv, d, 32)
+    got = AttnPaged(hq, hkv, d, DEV)(s["q"], s["k_pages"], s["v_pages"], s["table"], s["length"], s["cu_rows"], max_q=max_q).double()
+    want, mag = attn64(s, hq, hkv, d)
+    half = torch.exp2(torch.floor(torch.log2(want.abs().clamp(min=2.0 ** -100))) - 8)
+    assert ((got - want).abs() <= half + 2.0 ** -13 * mag).all()
+
+
+@pytest.mark.parametrize("rot,norm", [(64, False), (64, True), (36, True)])
+def test_steps_and_releases_in_dependent_launches(rot, norm):
+    """tables, write (rows that are not aligned among them), attention and release one behind the other without a wait of the host: the bits
+    of the same calls made one by one"""
+    from ixrun_b200.glue import rope_tables
+    from ixrun_b200.p6 import set_pdl
+    from ixrun_b200.paged import AttnPaged, PageTables, rope_kv_paged
+
+    hq, hkv, d, page, requests, rows, n_pages, width = 4, 2, 64, 16, 6, 120, 60, 9
+    g = torch.Generator(device=DEV).manual_seed(5)
+    cos, sin = rope_tables(width * page, rot, 10000.0, DEV)
+    x = torch.randn(12, rows, (hq + 2 * hkv) * d, generator=g, device=DEV).bfloat16()
+    w = (1 + 0.1 * torch.randn(d, generator=g, device=DEV)).bfloat16() if norm else None
+    new = [on_gpu([(7 * i + 5 * r) % 19 for r in range(requests)]) for i in range(12)]
+    done = [torch.tensor([(i + r) % 4 == 0 for r in range(requests)], device=DEV) for i in range(12)]
+
+    def run(wait):
+        t, attn, outs = PageTables(requests, n_pages, page, width, DEV), AttnPaged(hq, hkv, d, DEV), []
+        kp, vp = (torch.zeros(n_pages, page, hkv, d, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+        st, qs = t.new_step(rows), torch.zeros(rows, hq * d, dtype=torch.bfloat16, device=DEV)
+        for i in range(12):
+            q, k, v = x[i][:, :hq * d], x[i][:, hq * d:(hq + hkv) * d], x[i][:, (hq + hkv) * d:]
+            o = torch.zeros_like(qs)
+            wait()
+            t.step(new[i], rows, out=st)
+            wait()
+            rope_kv_paged(q, k, v, st.pos, st.slot, kp, vp, cos, sin, hq, hkv, d, rot_dim=rot, q_norm=w, k_norm=w, out=qs)
+            wait()
+            attn(qs, kp, vp, t.table, st.length, st.cu_rows, out=o)
+            wait()
+            outs += [o, t.release(done[i])]
+            wait()
+            outs += [t.table.clone(), t.free.clone(), t.n_free.clone(), t.length.clone()]
+        return outs + [kp, vp]
+
+    want = run(torch.cuda.synchronize)
+    assert all(s.tolist()[0] == 0 for s in want[1:-2:6])
+    prev = set_pdl(True)
+    try:
+        for _ in range(5):
+            got = run(lambda: None)
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+    finally:
+        torch.cuda.synchronize()
+        set_pdl(prev)

@@ -275,3 +275,23 @@ def test_generate_that_refuses_a_prompt_leaves_no_request_behind(last):
         dec.generate([ids, ids, ids, bad], 3, **({"bias": {i: 0.5 for i in range(65)}} if last == "rules" else {}))
     assert dec._known == [None, None] and dec._pages_left == 12 == dec.pages.n_free.item()
     assert [len(o) for o in dec.generate([ids, ids, ids], 3)] == [3, 3, 3]
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_dependent_launches_give_the_same_bits(captured):
+    from ixrun_b200.llama_runner import PagedDecoder
+    from ixrun_b200.p6 import set_pdl
+
+    cfg, model = tiny()
+    prompts = prompts_of(cfg, (17, 5, 30, 9))
+    numbers, want = run_of_requests(PagedDecoder(model, 3, 10, page=16), prompts, 7)
+    prev = set_pdl(True)
+    try:
+        dec = PagedDecoder(model, 3, 10, page=16)
+        n2, got = run_of_requests(dec.capture() if captured else dec, prompts, 7)
+    finally:
+        torch.cuda.synchronize()
+        set_pdl(prev)
+    assert n2 == numbers
+    for a, b in zip(want, got):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
