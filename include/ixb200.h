@@ -419,7 +419,8 @@ int ixb_gdn_conv_step(const void *qkv_raw_device, void *conv_state_device, const
  *   request are left as they are, rows that see no position become zero.  Positions that the table has no entry for (a
  *   length above width * page) are seen by nobody.  max_q: the most new tokens that a request may
  *   have, by which kernels are chosen (results do not need it to be true).  A page number outside the pool counts as a page
- *   of zeros.  head_dim 64, 128 or 256; scale positive; pointers 16-byte aligned.  scratch: ixb_attn_paged_scratch_bytes of the current
+ *   of zeros.  head_dim 64, 128 or 256; scale positive; pointers 16-byte aligned; (rows * hq / hkv / 8 + requests) * (width * page /
+ *   64 + 8) below 2^32 (100 million positions a table for thousands of rows).  scratch: ixb_attn_paged_scratch_bytes of the current
  *   device, the first 4096 bytes of it zero before the first call and left zero by every call (a buffer of its own for
  *   launches that may overlap).
  */

@@ -178,6 +178,11 @@ extern "C" int ixb_attn_paged(const void *q, const void *k_pages, const void *v_
     if (head_dim != 64 && head_dim != 128 && head_dim != 256) return fail(IXB_E_UNSUPPORTED, "head_dim=%lld: 64, 128 or 256", (long long)head_dim);
     if (rows <= 0 || rows > 0x7fffffffll / hq || max_q <= 0) return fail(IXB_E_ARG, "bad rows");
     if (rows * (hq / hkv) > 0xfffffff0ll / (hq / hkv)) return fail(IXB_E_UNSUPPORTED, "%lld rows of groups of %lld heads", (long long)rows, (long long)(hq / hkv));
+    // The kernels add the costs of a KV head's work up in 32 bits: groups of at least eight rows, a table's width of blocks or tiles of 128
+    // positions each, twice for two row tiles, and eight more for an end.  (All factors are below 2^32: no overflow here.)
+    if ((double)(rows * (hq / hkv) / 8 + requests) * (double)(2 * (width * page / 128) + 8) >= 4294967296.0)
+        return fail(IXB_E_UNSUPPORTED, "%lld rows and %lld requests behind tables of %lld positions are too much for one call", (long long)rows, (long long)requests,
+                    (long long)(width * page));
     if (q_stride < hq * head_dim || (q_stride & 7) || k_page_stride < page * hkv * head_dim || v_page_stride < page * hkv * head_dim ||
         ((k_page_stride | v_page_stride) & 7))
         return fail(IXB_E_ARG, "bad strides");

@@ -56,6 +56,20 @@ def test_bad_arguments_are_refused_before_any_cuda_call(name, changed, code):
     assert rc == code and text
 
 
+@pytest.mark.parametrize("requests,rows,hq,page,width,fits", [
+    (4096, 4096, 4, 256, 1 << 22, False),              # 4096 requests that share a table's pages, 2^30 positions each
+    (64, 2048, 16, 256, 1 << 22, False), (4096, 4096, 16, 16, 1 << 15, True), (1, 1, 16, 256, (1 << 23) - 1, True), (64, 16384, 16, 64, 1 << 14, True)])
+def test_work_that_32_bits_do_not_count_is_refused(requests, rows, hq, page, width, fits):
+    """before anything is launched: with a wrapped sum CTAs would take rows that are not there.  (What fits goes on to the next check, that of
+    the scratch.)"""
+    stride = page * 2 * 64
+    rc, text = call("ixb_attn_paged", requests=requests, rows=rows, hq=hq, q_stride=hq * 64, page=page, width=width, k_page_stride=stride, v_page_stride=stride,
+                    scratch_bytes=4096)
+    blocks = -(-rows * (hq // 2) // 8) * -(-width * page // 128)           # eight rows a group, the shortest blocks; at least
+    assert rc == (4 if fits else 2) and fits == (blocks < 2**32), text
+    assert fits or "too much" in text
+
+
 def test_scratch_sizes():
     from ixrun_b200 import _lib
 
