@@ -300,13 +300,14 @@ k_attn_paged(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
         // (of lane < boxes, at most 32: positions bk * bp .. of a block and 64 dimensions; with D = 256 and pages of 16 a lane has just one)
         static_assert(CF::kKeys / 16 * (D / 64) <= 32, "a box per lane");
         const uint32_t dst = (bk * bp / 128u * (D / 64) + panel) * CF::kPanel + bk * bp % 128u * 128u;
+        uint32_t seen = 0;                             // of *sm_again, when a wait last ran out
         auto room = [&](uint32_t bar, uint32_t parity) {
-            uint32_t seen;
-            do {
-                seen = *sm_again;
-                if (pa_wait(bar, parity)) return true;
-            } while (*sm_again != seen);
-            return false;
+            while (!pa_wait(bar, parity)) {
+                const uint32_t now = *sm_again;
+                if (now == seen) return false;
+                seen = now;
+            }
+            return true;
         };
         uint32_t n = 0;
         bool more = true;
