@@ -323,7 +323,7 @@ uint32_t ixb_allreduce_spin_limit(uint32_t polls);
  *   stride q_stride elements, heads contiguous) rotated in place, k and v
  *   [rows][hkv][head_dim] (row pitch kv_stride) written into the caches
  *   [max_seq][hkv][head_dim] at
- *   positions pos[0] + row.  head_dim 64, 128 or 256.
+ *   positions pos[0] + row.  A position outside the tables counts as the last one.  head_dim 64, 128 or 256.
  * ixb_attn_decode: one query per head (q [hq][head_dim]) over positions
  *   0 .. pos[0] of the static caches, grouped-query (hq a multiple of hkv),
  *   softmax(scale * q.k) v, the context cut into `splits` ranges that run on
@@ -411,17 +411,19 @@ int ixb_gdn_conv_step(const void *qkv_raw_device, void *conv_state_device, const
  * ixb_page_release: the pages of the requests with done[r] != 0 go back onto the stack, their lengths become 0.  status [2]:
  *   4 if the stack cannot take them (nothing is done then), and their number.
  * ixb_rope_paged: ixb_rope_kv with keys and values into slots: row i is at position pos[i] and goes to slot[i]; a row with a
- *   slot outside the pool is left alone.  The rotated q goes to out (row pitch out_stride; may be q).  Held in fp32 from
- *   the norm to the one rounding of the result.
+ *   slot outside the pool is left alone, a position outside the tables counts as the nearest one in them.  The rotated q goes
+ *   to out (row pitch out_stride; may be q).  Held in fp32 from the norm to the one rounding of the result.
  * ixb_attn_paged: causal attention of the new tokens of all requests, keys and values already in their pages: row
  *   cu_rows[r] + t of q [rows] (row pitch q_stride elements, heads contiguous) is token length[r] - (cu_rows[r + 1] -
  *   cu_rows[r]) + t of request r and sees the positions up to its own.  out [rows][hq][head_dim]; rows that belong to no
  *   request are left as they are, rows that see no position become zero.  Positions that the table has no entry for (a
- *   length above width * page) are seen by nobody.  max_q: the most new tokens that a request may
- *   have, by which kernels are chosen (results do not need it to be true).  A page number outside the pool counts as a page
- *   of zeros.  head_dim 64, 128 or 256; scale positive; pointers 16-byte aligned; (rows * hq / hkv / 8 + requests) * (width * page /
- *   64 + 8) below 2^32 (100 million positions a table for thousands of rows).  scratch: ixb_attn_paged_scratch_bytes of the current
- *   device, the first 4096 bytes of it zero before the first call and left zero by every call (a buffer of its own for
+ *   length above width * page) are seen by nobody.  max_q: the most new tokens that a request may have, by which kernels are
+ *   chosen (results do not need it to be true).  Probabilities are multiplied with the values in 17
+ *   bits for requests of few rows (new tokens times hq / hkv: up to 16, up to 8 with head_dim 256) and in calls with such a
+ *   max_q, in 8 bits (bf16) for others (a call of one request goes by max_q alone); a row's bits also depend on the other
+ *   requests' lengths, by which the work is cut.  A page number outside the pool counts as a page of zeros.  head_dim 64, 128
+ *   or 256; scale positive; pointers 16-byte aligned; (rows * hq / hkv / 8 + requests) * (width * page / 64 + 8) below 2^32 (tables of
+ *   100 million positions for some hundred rows and requests).  scratch: ixb_attn_paged_scratch_bytes of the current device, the first 4096 bytes of it zero before the first call and left zero by every call (a buffer of its own for
  *   launches that may overlap).
  */
 int ixb_page_step(const int32_t *q_len_device, const int32_t *length_device, int32_t *table_device, const int32_t *free_pages_device,

@@ -16,7 +16,10 @@
 //
 // The accumulator is rescaled only when a row's maximum has grown by more than 2^8 (a running maximum that lags changes no ratio).
 // Precision: scores and sums fp32, probabilities bf16 for P V (half a step, 2^-8 of each, as the result's own rounding; the tensor
-// core takes no wider operand beside bf16 values), their sum from the fp32 values.
+// core takes no wider operand beside bf16 values), their sum from the fp32 values: results 0.0023 from 64 bits, 0.0017 of it their own
+// rounding.  With the trailing bits as a second product, as the form for few rows has them, 0.0017; the chunk below then takes
+// 289 us instead of 224, drafts of heads of 256 57.5 instead of 49.9, and every value has to be looked through (a trailing part of
+// zero or less times infinity is NaN).
 //
 // Keys that no row of the unit sees are not read; the rows of V behind the last key are zeroed up to a multiple of 16 and not
 // multiplied beyond.  A value that is not finite counts for the rows that see it and for no other: where a key tile is not
@@ -24,7 +27,8 @@
 //
 // Bound: the tensor core for long chunks, with the exponentials (one per score, 16 a cycle and SM) close behind: 2048 rows of a prompt
 // behind 12000 keys, 16 / 8 heads of 128: 192 us, 69 % of the measured rate of dense products; the tensor pipe and the special function
-// unit are each busy 45 % of the time, the rest is the chain scores, maximum, exponentials, P V.  Fixed: 10 us for a launch, the
+// unit are each busy 45 % of the time, the rest is the chain scores, maximum, exponentials, P V.  (In a captured graph; among
+// other passes 224 us, 59 %, at the clocks that the power limit leaves.)  Fixed: 10 us for a launch, the
 // first keys, the cut units' ends and the join.  Built and slower for that chunk: steps of 64 keys in slots of their own, so that
 // scores wait for no P V (224 us: Q K^T of 64 columns is bound by Q's reads, and a step's overheads come twice), these with two sets
 // of softmax warps that take steps in turn (228), an MMA warp per group (248: the groups then run in step and want the
@@ -39,8 +43,14 @@
 namespace ixb {
 
 constexpr uint32_t kPcKeys = 128;
-constexpr uint32_t kPcMinCost = 4;                     // key tiles of a CTA, unless there are more units than that makes CTAs
-constexpr uint32_t kPcShortUnit = 12;                  // cost of a unit (key tiles times row tiles), on average, up to which it is not cut
+// Key tiles of a CTA, unless there are more units than that makes CTAs: parts that are joined against tiles one behind the other (64 rows
+// behind 6000 keys, 16 / 8 heads of 128: 23.0 us with 2, 21.7 with 4, 21.8 with 8, 27.6 with 16; behind 2000 16.6, 17.2, 20.1, 27.3;
+// 20 rows behind 4000, 12 / 2 heads of 256: 21.6, 23.7, 28.5, 39.6).
+constexpr uint32_t kPcMinCost = 4;
+// Cost of a unit (key tiles times row tiles), on average, up to which it is not cut (prompts from their start, 16 / 8 heads of 128: 300
+// tokens 17.8 us cut, 15.7 whole; 700 tokens 19.5 cut, 21.1 whole; 64 rows behind 1200 keys 16.2 cut, 20.9 whole, behind 2000, which
+// is above the limit, 17.1 cut, 26.2 whole; 300 tokens of 24 / 4 heads of 256 25.3 cut, 17.8 whole).
+constexpr uint32_t kPcShortUnit = 12;
 
 template <int D>
 struct PcCfg {
@@ -54,8 +64,9 @@ struct PcCfg {
     static constexpr uint32_t kQTile = D / 64 * kPanel;
     static constexpr uint32_t kStages = D == 64 ? 8 : 5;
     // Cost of a unit's end and the next one's start, in steps of 128 rows and a key tile: without it CTAs with ends of two units are the last
-    // (a prompt of 2048 tokens from its start, 16 / 8 heads of 128: 48.2 us with 0, 41.1 with 2, 39.4 with 4, 35.7 with 6, 36.6 with 8;
-    // drafts of heads of 256, whose steps are longer: 50.9 with 0, 47.6 with 1, 49.9 with 2).
+    // (a prompt of 2048 tokens from its start, 16 / 8 heads of 128: 50.7 us with 0, 43.2 with 2, 41.2 with 4, 37.3 with 6, 37.6 with 8;
+    // 32 / 8 heads of 64: 60.9, 50.1, 45.9, 45.2, 46.2; heads of 256, whose steps are longer: drafts 50.9 with 0, 47.6 with 1, 49.9 with
+    // 2, but a prompt of 2048 tokens, 24 / 4 heads, 143.8, 105.6 and 91.4).
     static constexpr uint32_t kEnd = D == 256 ? 1 : 6;
     static constexpr uint32_t kRingOff = kTiles * kQTile;
     static constexpr uint32_t kBarOff = kRingOff + kStages * kUnit;
@@ -323,7 +334,7 @@ k_attn_chunk(PagedAttn a, const __grid_constant__ CUtensorMap kmap, const __grid
     }
     __syncthreads();
     // What the line is cut into: key tiles; or whole units where there is room for one per CTA and they are short, so that cutting them
-    // would cost more than it saves (300 rows of a prompt, 16 / 8 heads of 128: 24 us cut, 16.8 whole)
+    // would cost more than it saves (figures at kPcShortUnit)
     const bool by_unit = (unsigned long long)sm_units * a.hkv <= gridDim.x && sm_cost <= (kPcShortUnit + CF::kEnd) * sm_units;
     const uint32_t total = by_unit ? sm_units : sm_cost;
     {

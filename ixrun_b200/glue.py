@@ -85,7 +85,7 @@ def rope_kv(q, k, v, pos, k_cache, v_cache, cos, sin, hq: int, hkv: int, head_di
     """q [rows, >= hq*head_dim] rotated in place; k, v [rows, hkv*head_dim] (column slices allowed) into the caches.
     batched=False: one sequence, caches [max_seq, hkv, head_dim], the rows are positions pos[0] + row (pos: int32 device
     tensor of one element).  batched=True: row r is the newest token of sequence r: caches [rows, max_seq, hkv, head_dim],
-    pos int32 [rows]."""
+    pos int32 [rows].  A position outside the tables counts as the last one."""
     _bf16(k_cache, v_cache, q_norm, k_norm)
     if pos.dtype != torch.int32 or not pos.is_cuda:
         raise ValueError("pos must be an int32 CUDA tensor")

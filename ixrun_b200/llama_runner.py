@@ -567,7 +567,8 @@ class PagedDecoder:
     generator does with one static cache row per sequence (ixrun/batching.py:88-234), for requests of different lengths in
     memory for the tokens that there are.  A step feeds every request the tokens that it has and the model has not seen: the
     next piece of its prompt, or its last token.  Steps of single tokens are one CUDA graph (``capture``).  Per request:
-    penalties, biases and a mask of allowed tokens; the token is the arg-max behind them."""
+    penalties, biases and a mask of allowed tokens; the token is the arg-max behind them.  Steps of several decoders of one model,
+    which share its buffer for decoded weights, must not overlap."""
 
     def __init__(self, model: PackedLlama, requests: int, n_pages: int, page: int = 64, max_bias: int = 64):
         from .logits import MAX_BIASES, MAX_TOKENS, MAX_VOCAB

@@ -156,7 +156,8 @@ def rope_kv_paged(q, k, v, pos, slot, k_pages, v_pages, cos, sin, hq: int, hkv: 
                   k_norm=None, eps: float = 1e-6, out=None):
     """``glue.rope_kv`` for a paged cache: q [rows, >= hq*head_dim] rotated (in place, or into out [rows, hq*head_dim]); k, v [rows,
     hkv*head_dim] into the pools at slot [rows]; pos, slot: int32 [rows] as ``page_step`` gives them.  Column slices are allowed.  A
-    row whose slot is outside the pools is left alone.  Between the norm and the result nothing is rounded."""
+    row whose slot is outside the pools is left alone; a position outside the tables is rotated as the nearest one in them.  Between the
+    norm and the result nothing is rounded."""
     if _host().rope_paged(q, k, v, pos, slot, k_pages, v_pages, cos, sin, hq, hkv, head_dim, rot_dim or head_dim, q_norm, k_norm, eps, q if out is None else out):
         return q if out is None else out
     _bf16(q_norm, k_norm)
@@ -224,7 +225,12 @@ class AttnPaged:
         cu_rows [R+1], table: int32.  Every row attends to the positions up to its own, of those that the table has an entry for.
         max_q: the most new tokens that a request has (1 for a step of single tokens), by which the kernels are chosen.  Returns
         out [rows, hq*head_dim]; rows of no request are left as they are (undefined without `out`), rows that see no position are
-        zero."""
+        zero.
+
+        Scores and sums are held in 32 bits.  Probabilities are multiplied with the values in 17 bits where a request has few rows (new
+        tokens times query heads of a KV head: up to 16, up to 8 with heads of 256) or max_q says so of all, in 8 bits (bf16) where it
+        has more (one request alone: by max_q): a token of a longer draft agrees with the same token alone to bf16 noise, not to the bit.  A row's last bits also depend
+        on the other requests of the call, whose lengths say where the work is cut; the same call gives the same bits."""
         done = _host().attn_paged(self.hq, self.hkv, self.d, self.scratch, q, k_pages, v_pages, table, length, cu_rows, max_q, out, scale)
         if done is not None:
             return done

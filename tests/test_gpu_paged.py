@@ -791,3 +791,22 @@ def test_steps_and_releases_in_dependent_launches(rot, norm):
     finally:
         torch.cuda.synchronize()
         set_pdl(prev)
+
+
+@pytest.mark.parametrize("rot,norm", [(64, False), (36, True)])
+def test_a_position_outside_the_tables_is_the_nearest_one_in_them(rot, norm):
+    from ixrun_b200.glue import rope_tables
+    from ixrun_b200.paged import rope_kv_paged
+
+    hq, hkv, d = 2, 1, 64
+    g = torch.Generator(device=DEV).manual_seed(2)
+    cos, sin = rope_tables(50, rot, 10000.0, DEV)
+    w = torch.randn(d, generator=g, device=DEV).bfloat16() if norm else None
+    x = [torch.randn(5, n * d, generator=g, device=DEV).bfloat16() for n in (hq, hkv, hkv)]
+    got = []
+    for pos in ([50, 51, 2**31 - 1, -1, -2**31], [49, 49, 49, 0, 0]):
+        kp, vp = (torch.zeros(1, 16, hkv, d, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+        got.append((rope_kv_paged(*x, on_gpu(pos), on_gpu([0, 1, 2, 3, 4]), kp, vp, cos, sin, hq, hkv, d, rot_dim=rot, q_norm=w, k_norm=w,
+                                  out=torch.empty_like(x[0])), kp, vp))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
