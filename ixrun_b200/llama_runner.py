@@ -775,8 +775,9 @@ class PagedDecoder:
     def step(self, max_rows: int = PackedLlama.PREFILL_ROWS) -> torch.Tensor:
         """Feeds the requests what they have, at most max_rows rows in all: single tokens first, those that have waited longest before
         others, then prompts in the order in which they were added; the first of these comes before the single tokens where it had
-        no row in the step before.  So every request gets on, however few rows there are.  Returns tokens int64 [requests], -1 for those without a new one (a static tensor).  RuntimeError, and
-        nothing launched, where there is nothing to feed, a request has all max_seq tokens, or the pages do not suffice."""
+        no row in the step before.  So every request gets on, however few rows there are.  Returns tokens int64 [requests], -1
+        for those without a new one (a static tensor).  RuntimeError, and nothing launched, where there is nothing to feed, a
+        request has all max_seq tokens, or the pages do not suffice."""
         if max_rows < 1:
             raise ValueError("max_rows must be positive")
         q_len = self._share(max_rows)
